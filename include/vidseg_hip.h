@@ -378,6 +378,23 @@ int vidseg_clip_blur_axis(const float* x, long long planes, int H, int W, const 
 int vidseg_clip_resize_patches(const float* x, int B, int H, int W, int S, int P, const float* mean3, const float* std3, float* out, int ldo,
                                vidseg_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------------------
+ * Operators that take their tensors' own type (dtype: 0 fp32, 1 fp16, 2 bf16) and carry gradients (csrc/norm_act.hip)
+ * ---------------------------------------------------------------------------------------------------- */
+/* GroupNorm32 (+ SiLU, act = 1) of a channels-last map (DU:276-278, OAI:267-271), fp32 arithmetic, any C % G == 0, C <= 8192: x [B][HW][C]
+ * with element strides x_batch_stride / x_row_stride (>= C), y contiguous; gamma / beta fp32 [C]; mean / rstd fp32 [B][G] (both or neither: what
+ * the backward pass needs).  rows_per_chunk: rows of one sample a block reduces, nchunk = ceil(HW / rows_per_chunk).
+ * scratch: 2 * B * nchunk * G floats. */
+int vidseg_groupnorm_act_fwd(const void* x, long long x_batch_stride, long long x_row_stride, int dtype, int B, long long HW, int C, int G,
+                             const float* gamma, const float* beta, float eps, int act, int rows_per_chunk, void* y, float* mean, float* rstd,
+                             float* scratch, long long scratch_floats, vidseg_stream_t stream);
+/* its gradients: dx contiguous [B][HW][C] in x's type, dgamma / dbeta fp32 [C] summed over the batch (fixed order, no atomics).
+ * scratch: B * ((nchunk + 1) * 2 * C + 2 * G) floats. */
+int vidseg_groupnorm_act_bwd(const void* dy, long long dy_batch_stride, long long dy_row_stride, const void* x, long long x_batch_stride,
+                             long long x_row_stride, int dtype, int B, long long HW, int C, int G, const float* gamma, const float* beta,
+                             const float* mean, const float* rstd, int act, int rows_per_chunk, void* dx, float* dgamma, float* dbeta,
+                             float* scratch, long long scratch_floats, vidseg_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

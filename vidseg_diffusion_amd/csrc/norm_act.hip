@@ -1,0 +1,469 @@
+// HIPCC_FLAGS: -fno-slp-vectorize -Xclang -target-feature -Xclang -packed-fp32-ops
+// GroupNorm with an optional SiLU on channels-last maps x [B][HW][C], forward and backward, fp32 / fp16 / bf16 storage.
+//
+//   xh = (x - mean_g) * rstd_g,  z = xh * gamma + beta,  y = z or z * sigmoid(z)
+//   dz = dy * act'(z),  dbeta = sum dz,  dgamma = sum dz * xh,
+//   dx = rstd_g * (gamma * dz - (mean over the group of gamma * dz) - xh * (mean over the group of gamma * dz * xh))
+//
+// Everything is held in fp32 between the load and the one rounding of the store.  A thread owns VEC neighbouring channels (16 bytes) of
+// every R-th row, so a wave reads whole rows; sums go channel -> group only after the rows are summed, so any C / G works, also
+// groups that end inside a 16-byte piece (320 channels in 32 groups of 10).  The forward pass is two launches (chunk statistics; merge and apply), the
+// backward three (channel sums; their merge over the chunks; dx, with dgamma and dbeta in extra blocks): no atomics, every sum has one order.
+// A chunk's row count depends on HW and C only, so a sample's result does not depend on the batch it is in.
+#include "common.h"
+
+namespace {
+
+constexpr int NT = 256;
+
+template <typename T> struct Stored;
+template <> struct Stored<float> {
+    typedef float type;
+    static __device__ __forceinline__ float up(float v) { return v; }
+    static __device__ __forceinline__ float down(float v) { return v; }
+};
+template <> struct Stored<_Float16> {
+    typedef _Float16 type;
+    static __device__ __forceinline__ float up(_Float16 v) { return (float)v; }
+    static __device__ __forceinline__ _Float16 down(float v) { return (_Float16)v; }
+};
+template <> struct Stored<__bf16> {
+    typedef __bf16 type;
+    static __device__ __forceinline__ float up(__bf16 v) { return (float)v; }
+    static __device__ __forceinline__ __bf16 down(float v) { return (__bf16)v; }
+};
+
+template <typename T, int VEC> __device__ __forceinline__ void load_vec(const T* p, float (&v)[VEC]) {
+    typedef T vec __attribute__((ext_vector_type(VEC)));
+    if constexpr (VEC == 1) {
+        v[0] = Stored<T>::up(*p);
+    } else {
+        const vec r = *reinterpret_cast<const vec*>(p);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = Stored<T>::up(r[e]);
+    }
+}
+template <typename T, int VEC> __device__ __forceinline__ void store_vec(T* p, const float (&v)[VEC]) {
+    typedef T vec __attribute__((ext_vector_type(VEC)));
+    if constexpr (VEC == 1) {
+        *p = Stored<T>::down(v[0]);
+    } else {
+        vec r;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) r[e] = Stored<T>::down(v[e]);
+        *reinterpret_cast<vec*>(p) = r;
+    }
+}
+
+__device__ __forceinline__ float sigmoid_f32(float z) {           // exp2 overflows to inf for z < -128 / log2 e: 1 / inf = 0, the limit
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896340736f));
+}
+
+struct NormArgs {
+    const void* x;
+    long long x_b, x_row;                 // element strides of a sample and of a row
+    const void* dy;
+    long long dy_b, dy_row;
+    long long HW;
+    int B, C, G, rows, nchunk, act;
+    float eps;
+    const float *gamma, *beta;
+    void* out;                            // y or dx, contiguous [B][HW][C]
+    float *mean, *rstd;                   // [B][G]
+    float* part;                          // forward: [B][nchunk][G][2] (mean, M2); backward: [B][nchunk][2][C]
+    float* chan;                          // backward: [B][2][C] sums of dz and dz * xh
+    float* coef;                          // backward: [B][G][2] group means of gamma * dz and gamma * dz * xh
+    float *dgamma, *dbeta;
+};
+
+// Sums over the R row lanes of a column pass: s[k][j] over j = 0..R-1 laid out [R][cols * VEC] in LDS; afterwards row 0 holds the totals.
+// (all NT threads call it)
+template <int VEC> __device__ __forceinline__ void fold_rows(float* s0, float* s1, int R, int width) {
+    __syncthreads();
+    for (int c = threadIdx.x; c < width; c += NT) {
+        float a = s0[c], b = s1[c];
+        for (int j = 1; j < R; ++j) {
+            a += s0[j * width + c];
+            b += s1[j * width + c];
+        }
+        s0[c] = a;
+        s1[c] = b;
+    }
+    __syncthreads();
+}
+
+// ---- forward, launch 1: (mean, M2) of every group over the rows of one chunk.
+// A channel is summed about its own first value of the chunk (x - x[row0]), then mean and sum of squared deviations of the group are put together
+// from the channels': no difference of large squares anywhere, so maps whose mean is far from zero keep their variance.
+template <typename T, int VEC> __global__ void __launch_bounds__(NT) k_gna_stats(NormArgs p) {
+    extern __shared__ float lds[];
+    const int C = p.C, cols = C / VEC, b = blockIdx.y, chunk = blockIdx.x;
+    const int pc = cols < NT ? cols : NT, R = NT / pc, width = pc * VEC;
+    float* ch_mean = lds;                 // [C]
+    float* ch_m2 = lds + C;               // [C]
+    float* s0 = lds + 2 * C;              // [R][width]
+    float* s1 = s0 + R * width;
+    const long long r0 = (long long)chunk * p.rows;
+    const int n = (int)(p.HW - r0 < p.rows ? p.HW - r0 : p.rows);
+    const T* x = (const T*)p.x + b * p.x_b + r0 * p.x_row;
+    const int col = threadIdx.x % pc, rl = threadIdx.x / pc;
+    for (int c0 = 0; c0 < cols; c0 += pc) {
+        const bool on = rl < R && c0 + col < cols;
+        float k[VEC], a[VEC], q[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) k[e] = a[e] = q[e] = 0.f;
+        if (on) {
+            const T* xc = x + (long long)(c0 + col) * VEC;
+            load_vec<T, VEC>(xc, k);
+#pragma unroll 4
+            for (int r = rl; r < n; r += R) {
+                float v[VEC];
+                load_vec<T, VEC>(xc + r * p.x_row, v);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const float d = v[e] - k[e];
+                    a[e] += d;
+                    q[e] += d * d;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                s0[rl * width + col * VEC + e] = a[e];
+                s1[rl * width + col * VEC + e] = q[e];
+            }
+        }
+        fold_rows<VEC>(s0, s1, R, width);
+        if (rl == 0 && on) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float s = s0[col * VEC + e], m = s / (float)n;
+                ch_mean[(c0 + col) * VEC + e] = k[e] + m;
+                ch_m2[(c0 + col) * VEC + e] = fmaxf(s1[col * VEC + e] - s * m, 0.f);
+            }
+        }
+        __syncthreads();
+    }
+    const int cg = C / p.G;
+    for (int g = threadIdx.x; g < p.G; g += NT) {
+        float m = 0.f, m2 = 0.f;
+        for (int c = 0; c < cg; ++c) m += ch_mean[g * cg + c];
+        m /= (float)cg;
+        for (int c = 0; c < cg; ++c) {
+            const float d = ch_mean[g * cg + c] - m;
+            m2 += ch_m2[g * cg + c] + (float)n * d * d;
+        }
+        float* o = p.part + (((long long)b * p.nchunk + chunk) * p.G + g) * 2;
+        o[0] = m;
+        o[1] = m2;
+    }
+}
+
+// ---- forward, launch 2: every block merges its sample's chunk statistics (a few KB out of L2) and writes one chunk of y
+template <typename T, int VEC> __global__ void __launch_bounds__(NT) k_gna_apply(NormArgs p) {
+    extern __shared__ float lds[];
+    const int C = p.C, cols = C / VEC, b = blockIdx.y, chunk = blockIdx.x, cg = C / p.G;
+    float* g_mean = lds;
+    float* g_rstd = lds + p.G;
+    for (int g = threadIdx.x; g < p.G; g += NT) {
+        const float* o = p.part + ((long long)b * p.nchunk * p.G + g) * 2;
+        float m = 0.f, m2 = 0.f;
+        for (int i = 0; i < p.nchunk; ++i) {
+            const float n = (float)(i + 1 < p.nchunk ? p.rows : (int)(p.HW - (long long)i * p.rows));
+            m += n * o[(long long)i * p.G * 2];
+        }
+        m /= (float)p.HW;
+        for (int i = 0; i < p.nchunk; ++i) {
+            const float n = (float)(i + 1 < p.nchunk ? p.rows : (int)(p.HW - (long long)i * p.rows)) * (float)cg;
+            const float d = o[(long long)i * p.G * 2] - m;
+            m2 += o[(long long)i * p.G * 2 + 1] + n * d * d;
+        }
+        const float rstd = 1.0f / sqrtf(m2 / ((float)p.HW * (float)cg) + p.eps);
+        g_mean[g] = m;
+        g_rstd[g] = rstd;
+        if (p.mean && chunk == 0) {
+            p.mean[(long long)b * p.G + g] = m;
+            p.rstd[(long long)b * p.G + g] = rstd;
+        }
+    }
+    __syncthreads();
+    const int pc = cols < NT ? cols : NT, R = NT / pc;
+    const long long r0 = (long long)chunk * p.rows;
+    const int n = (int)(p.HW - r0 < p.rows ? p.HW - r0 : p.rows);
+    const int col = threadIdx.x % pc, rl = threadIdx.x / pc;
+    if (rl >= R) return;
+    for (int c = col; c < cols; c += pc) {
+        float mean[VEC], scale[VEC], shift[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const int ch = c * VEC + e, g = ch / cg;
+            mean[e] = g_mean[g];
+            scale[e] = g_rstd[g] * p.gamma[ch];
+            shift[e] = p.beta[ch];
+        }
+        const T* x = (const T*)p.x + b * p.x_b + r0 * p.x_row + (long long)c * VEC;
+        T* y = (T*)p.out + ((long long)b * p.HW + r0) * C + (long long)c * VEC;
+#pragma unroll 4
+        for (int r = rl; r < n; r += R) {
+            float v[VEC];
+            load_vec<T, VEC>(x + r * p.x_row, v);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float z = (v[e] - mean[e]) * scale[e] + shift[e];
+                v[e] = p.act ? z * sigmoid_f32(z) : z;
+            }
+            store_vec<T, VEC>(y + (long long)r * C, v);
+        }
+    }
+}
+
+// dz of one value: act' (z) = sig (1 + z (1 - sig))
+__device__ __forceinline__ float dz_of(float dy, float z, int act) {
+    if (!act) return dy;
+    const float s = sigmoid_f32(z);
+    return dy * (s * (1.0f + z * (1.0f - s)));
+}
+
+// ---- backward, launch 1: per channel the sums of dz and dz * xh over the rows of one chunk
+template <typename T, int VEC> __global__ void __launch_bounds__(NT) k_gna_bwd_sums(NormArgs p) {
+    extern __shared__ float lds[];
+    const int C = p.C, cols = C / VEC, b = blockIdx.y, chunk = blockIdx.x, cg = C / p.G;
+    const int pc = cols < NT ? cols : NT, R = NT / pc, width = pc * VEC;
+    float* s0 = lds;
+    float* s1 = lds + R * width;
+    const long long r0 = (long long)chunk * p.rows;
+    const int n = (int)(p.HW - r0 < p.rows ? p.HW - r0 : p.rows);
+    const int col = threadIdx.x % pc, rl = threadIdx.x / pc;
+    float* o = p.part + ((long long)b * p.nchunk + chunk) * 2 * C;
+    for (int c0 = 0; c0 < cols; c0 += pc) {
+        const int c = c0 + col;
+        if (rl < R && c < cols) {
+            float mean[VEC], rstd[VEC], gm[VEC], bt[VEC], a[VEC], q[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const int ch = c * VEC + e, g = ch / cg;
+                mean[e] = p.mean[(long long)b * p.G + g];
+                rstd[e] = p.rstd[(long long)b * p.G + g];
+                gm[e] = p.gamma[ch];
+                bt[e] = p.beta[ch];
+                a[e] = q[e] = 0.f;
+            }
+            const T* x = (const T*)p.x + b * p.x_b + r0 * p.x_row + (long long)c * VEC;
+            const T* dy = (const T*)p.dy + b * p.dy_b + r0 * p.dy_row + (long long)c * VEC;
+#pragma unroll 2
+            for (int r = rl; r < n; r += R) {
+                float v[VEC], d[VEC];
+                load_vec<T, VEC>(x + r * p.x_row, v);
+                load_vec<T, VEC>(dy + r * p.dy_row, d);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const float xh = (v[e] - mean[e]) * rstd[e];
+                    const float dz = dz_of(d[e], xh * gm[e] + bt[e], p.act);
+                    a[e] += dz;
+                    q[e] += dz * xh;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                s0[rl * width + col * VEC + e] = a[e];
+                s1[rl * width + col * VEC + e] = q[e];
+            }
+        }
+        fold_rows<VEC>(s0, s1, R, width);
+        const int w = (cols - c0 < pc ? cols - c0 : pc) * VEC;
+        for (int i = threadIdx.x; i < w; i += NT) {
+            o[c0 * VEC + i] = s0[i];
+            o[C + c0 * VEC + i] = s1[i];
+        }
+        __syncthreads();
+    }
+}
+
+// ---- backward, launch 2: a block owns `gpb` groups of one sample; sums over the chunks, then the group means of gamma * dz, gamma * dz * xh
+__global__ void __launch_bounds__(NT) k_gna_bwd_merge(NormArgs p, int gpb) {
+    extern __shared__ float lds[];
+    const int C = p.C, b = blockIdx.y, cg = C / p.G;
+    const int g0 = blockIdx.x * gpb, g1 = g0 + gpb < p.G ? g0 + gpb : p.G, c0 = g0 * cg, w = (g1 - g0) * cg;
+    float* s0 = lds;
+    float* s1 = lds + gpb * cg;
+    const float* o = p.part + (long long)b * p.nchunk * 2 * C;
+    for (int c = threadIdx.x; c < w; c += NT) {
+        float a = 0.f, q = 0.f;
+#pragma unroll 8
+        for (int i = 0; i < p.nchunk; ++i) {
+            a += o[(long long)i * 2 * C + c0 + c];
+            q += o[(long long)i * 2 * C + C + c0 + c];
+        }
+        p.chan[(long long)b * 2 * C + c0 + c] = a;
+        p.chan[(long long)b * 2 * C + C + c0 + c] = q;
+        s0[c] = a * p.gamma[c0 + c];
+        s1[c] = q * p.gamma[c0 + c];
+    }
+    __syncthreads();
+    const float inv = 1.0f / ((float)p.HW * (float)cg);
+    for (int g = threadIdx.x; g < g1 - g0; g += NT) {
+        float a = 0.f, q = 0.f;
+        for (int c = 0; c < cg; ++c) {
+            a += s0[g * cg + c];
+            q += s1[g * cg + c];
+        }
+        float* f = p.coef + ((long long)b * p.G + g0 + g) * 2;
+        f[0] = a * inv;
+        f[1] = q * inv;
+    }
+}
+
+// ---- backward, launch 3: dx of one chunk; the blocks behind the chunks (x = nchunk, y = b < ceil(C / NT)) sum dgamma / dbeta over the batch
+template <typename T, int VEC> __global__ void __launch_bounds__(NT) k_gna_bwd_dx(NormArgs p) {
+    const int C = p.C, cols = C / VEC, b = blockIdx.y, chunk = blockIdx.x, cg = C / p.G;
+    if (chunk == p.nchunk) {
+        for (int c = b * NT + threadIdx.x; c < C; c += gridDim.y * NT) {
+            float a = 0.f, q = 0.f;
+            for (int i = 0; i < p.B; ++i) {
+                a += p.chan[(long long)i * 2 * C + c];
+                q += p.chan[(long long)i * 2 * C + C + c];
+            }
+            p.dbeta[c] = a;
+            p.dgamma[c] = q;
+        }
+        return;
+    }
+    const int pc = cols < NT ? cols : NT, R = NT / pc;
+    const long long r0 = (long long)chunk * p.rows;
+    const int n = (int)(p.HW - r0 < p.rows ? p.HW - r0 : p.rows);
+    const int col = threadIdx.x % pc, rl = threadIdx.x / pc;
+    if (rl >= R) return;
+    for (int c = col; c < cols; c += pc) {
+        float mean[VEC], rstd[VEC], gm[VEC], bt[VEC], ka[VEC], kb[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const int ch = c * VEC + e, g = ch / cg;
+            const long long bg = (long long)b * p.G + g;
+            mean[e] = p.mean[bg];
+            rstd[e] = p.rstd[bg];
+            gm[e] = p.gamma[ch];
+            bt[e] = p.beta[ch];
+            ka[e] = p.coef[bg * 2];
+            kb[e] = p.coef[bg * 2 + 1];
+        }
+        const T* x = (const T*)p.x + b * p.x_b + r0 * p.x_row + (long long)c * VEC;
+        const T* dy = (const T*)p.dy + b * p.dy_b + r0 * p.dy_row + (long long)c * VEC;
+        T* dx = (T*)p.out + ((long long)b * p.HW + r0) * C + (long long)c * VEC;
+#pragma unroll 2
+        for (int r = rl; r < n; r += R) {
+            float v[VEC], d[VEC];
+            load_vec<T, VEC>(x + r * p.x_row, v);
+            load_vec<T, VEC>(dy + r * p.dy_row, d);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float xh = (v[e] - mean[e]) * rstd[e];
+                const float dz = dz_of(d[e], xh * gm[e] + bt[e], p.act);
+                v[e] = rstd[e] * (gm[e] * dz - ka[e] - xh * kb[e]);
+            }
+            store_vec<T, VEC>(dx + (long long)r * C, v);
+        }
+    }
+}
+
+bool aligned16(const void* p, long long s0, long long s1, int esize) {
+    return ((uintptr_t)p % 16) == 0 && (s0 * esize) % 16 == 0 && (s1 * esize) % 16 == 0;
+}
+
+int check_args(const char* name, const void* x, long long x_b, long long x_row, int dtype, int B, long long HW, int C, int G, const float* gamma,
+               const float* beta, int act, int rows) {
+    VS_REQUIRE(x && gamma && beta, "%s: null operand", name);
+    VS_REQUIRE(dtype >= 0 && dtype <= 2, "%s: dtype %d (0 fp32, 1 fp16, 2 bf16)", name, dtype);
+    VS_REQUIRE(B >= 1 && B <= 65535 && HW >= 1 && C >= 1 && C <= 8192 && G >= 1 && C % G == 0, "%s: B=%d HW=%lld C=%d G=%d", name, B, HW, C, G);
+    VS_REQUIRE(act == 0 || act == 1, "%s: act %d (0 none, 1 SiLU)", name, act);
+    VS_REQUIRE(rows >= 1 && (HW + rows - 1) / rows <= (1 << 20), "%s: rows_per_chunk=%d", name, rows);
+    VS_REQUIRE(x_row >= C && x_b >= 0, "%s: row stride %lld below C=%d", name, x_row, C);
+    return VS_OK;
+}
+
+// CALL(T, VEC): 16-byte accesses where every operand allows them, single values otherwise
+#define GNA_DISPATCH(dtype, wide, CALL)                      \
+    do {                                                     \
+        if ((dtype) == 0) {                                  \
+            if (wide) { CALL(float, 4); } else { CALL(float, 1); }        \
+        } else if ((dtype) == 1) {                           \
+            if (wide) { CALL(_Float16, 8); } else { CALL(_Float16, 1); }  \
+        } else {                                             \
+            if (wide) { CALL(__bf16, 8); } else { CALL(__bf16, 1); }      \
+        }                                                    \
+    } while (0)
+
+size_t fold_floats(int C, int VEC) {
+    const int cols = C / VEC, pc = cols < NT ? cols : NT, R = NT / pc;
+    return (size_t)2 * R * pc * VEC;
+}
+
+}  // namespace
+
+extern "C" {
+
+int vidseg_groupnorm_act_fwd(const void* x, long long x_batch_stride, long long x_row_stride, int dtype, int B, long long HW, int C, int G,
+                             const float* gamma, const float* beta, float eps, int act, int rows_per_chunk, void* y, float* mean, float* rstd,
+                             float* scratch, long long scratch_floats, hipStream_t s) {
+    const int rc = check_args("groupnorm_act", x, x_batch_stride, x_row_stride, dtype, B, HW, C, G, gamma, beta, act, rows_per_chunk);
+    if (rc) return rc;
+    VS_REQUIRE(y && scratch && (!mean == !rstd), "groupnorm_act: null output or scratch");
+    NormArgs p{};
+    p.x = x; p.x_b = x_batch_stride; p.x_row = x_row_stride; p.HW = HW; p.B = B; p.C = C; p.G = G; p.rows = rows_per_chunk;
+    p.nchunk = (int)((HW + rows_per_chunk - 1) / rows_per_chunk);
+    p.act = act; p.eps = eps; p.gamma = gamma; p.beta = beta; p.out = y; p.mean = mean; p.rstd = rstd; p.part = scratch;
+    VS_REQUIRE((long long)B * p.nchunk * G * 2 <= scratch_floats, "groupnorm_act: scratch of %lld floats, needs %lld", scratch_floats,
+               (long long)B * p.nchunk * G * 2);
+    const int es = dtype == 0 ? 4 : 2, vec = 16 / es;
+    const bool wide = C % vec == 0 && aligned16(x, x_batch_stride, x_row_stride, es) && aligned16(y, 0, 0, es);
+    const dim3 grid(p.nchunk, B);
+    const size_t l1 = (2 * (size_t)C + fold_floats(C, wide ? vec : 1)) * 4, l2 = 2 * (size_t)G * 4;
+#define CALL(T, V)                                                   \
+    static VsOncePerDevice once;                                     \
+    if (once.needs()) {                                              \
+        hipError_t e = hipFuncSetAttribute((const void*)k_gna_stats<T, V>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024); \
+        if (e != hipSuccess) VS_FAIL(VS_ERR_HIP, "groupnorm_act: %s", hipGetErrorString(e)); \
+        once.mark();                                                 \
+    }                                                                \
+    hipLaunchKernelGGL((k_gna_stats<T, V>), grid, dim3(NT), l1, s, p); \
+    hipLaunchKernelGGL((k_gna_apply<T, V>), grid, dim3(NT), l2, s, p)
+    GNA_DISPATCH(dtype, wide, CALL);
+#undef CALL
+    VS_CHECK_LAUNCH("groupnorm_act");
+    return VS_OK;
+}
+
+int vidseg_groupnorm_act_bwd(const void* dy, long long dy_batch_stride, long long dy_row_stride, const void* x, long long x_batch_stride,
+                             long long x_row_stride, int dtype, int B, long long HW, int C, int G, const float* gamma, const float* beta,
+                             const float* mean, const float* rstd, int act, int rows_per_chunk, void* dx, float* dgamma, float* dbeta,
+                             float* scratch, long long scratch_floats, hipStream_t s) {
+    const int rc = check_args("groupnorm_act_bwd", x, x_batch_stride, x_row_stride, dtype, B, HW, C, G, gamma, beta, act, rows_per_chunk);
+    if (rc) return rc;
+    VS_REQUIRE(dy && mean && rstd && dx && dgamma && dbeta && scratch, "groupnorm_act_bwd: null operand");
+    VS_REQUIRE(dy_row_stride >= C && dy_batch_stride >= 0, "groupnorm_act_bwd: gradient row stride %lld below C=%d", dy_row_stride, C);
+    NormArgs p{};
+    p.x = x; p.x_b = x_batch_stride; p.x_row = x_row_stride; p.dy = dy; p.dy_b = dy_batch_stride; p.dy_row = dy_row_stride;
+    p.HW = HW; p.B = B; p.C = C; p.G = G; p.rows = rows_per_chunk;
+    p.nchunk = (int)((HW + rows_per_chunk - 1) / rows_per_chunk);
+    p.act = act; p.gamma = gamma; p.beta = beta; p.out = dx; p.mean = const_cast<float*>(mean); p.rstd = const_cast<float*>(rstd);
+    p.part = scratch;
+    p.chan = scratch + (long long)B * p.nchunk * 2 * C;
+    p.coef = p.chan + (long long)B * 2 * C;
+    p.dgamma = dgamma; p.dbeta = dbeta;
+    const long long need = (long long)B * ((long long)(p.nchunk + 1) * 2 * C + 2 * G);
+    VS_REQUIRE(need <= scratch_floats, "groupnorm_act_bwd: scratch of %lld floats, needs %lld", scratch_floats, need);
+    const int es = dtype == 0 ? 4 : 2, vec = 16 / es;
+    const bool wide = C % vec == 0 && aligned16(x, x_batch_stride, x_row_stride, es) && aligned16(dy, dy_batch_stride, dy_row_stride, es) &&
+                      aligned16(dx, 0, 0, es);
+    const dim3 grid(p.nchunk, B), grid3(p.nchunk + 1, B);
+    const size_t l1 = fold_floats(C, wide ? vec : 1) * 4;
+    const int cg = C / G, gpb = cg >= NT ? 1 : (NT / cg < G ? NT / cg : G);       // about one channel per thread
+#define CALL(T, V)                                                        \
+    hipLaunchKernelGGL((k_gna_bwd_sums<T, V>), grid, dim3(NT), l1, s, p); \
+    hipLaunchKernelGGL(k_gna_bwd_merge, dim3((G + gpb - 1) / gpb, B), dim3(NT), 2 * (size_t)gpb * cg * 4, s, p, gpb); \
+    hipLaunchKernelGGL((k_gna_bwd_dx<T, V>), grid3, dim3(NT), 0, s, p)
+    GNA_DISPATCH(dtype, wide, CALL);
+#undef CALL
+    VS_CHECK_LAUNCH("groupnorm_act_bwd");
+    return VS_OK;
+}
+
+}  // extern "C"

@@ -573,3 +573,7 @@ def add_rowvec(x, vec, rows_per_sample):
     out = torch.empty_like(x)
     call("vidseg_add_rowvec_a16", ptr(x), ptr(vec), x.numel() // C, C, rows_per_sample, vec.shape[0], ptr(out), stream())
     return out
+
+
+# ----------------------------------------------------------------------------- operators of their tensors' own type, with gradients
+from .context_ops import groupnorm_act  # noqa: E402,F401
