@@ -394,6 +394,18 @@ int vidseg_groupnorm_act_bwd(const void* dy, long long dy_batch_stride, long lon
                              long long x_row_stride, int dtype, int B, long long HW, int C, int G, const float* gamma, const float* beta,
                              const float* mean, const float* rstd, int act, int rows_per_chunk, void* dx, float* dgamma, float* dbeta,
                              float* scratch, long long scratch_floats, vidseg_stream_t stream);
+/* Attention over contexts (ATT:286-364 with other head widths, lengths and contexts; csrc/context_attn.hip; dtype 1 or 2): every query of sample b
+ * attends, as one softmax, to Np prefix keys that all samples share and to the sample's own keys 0 .. lens[b] - 1 (lens NULL: all Nk) for which
+ * mask[b * mask_b + key] != 0 (mask NULL: all); causal: query i sees own keys up to lens[b] - Nq + i (no mask then).  Heads of width d (8..128, d % 8
+ * == 0), query head h on key head h * Hk / H; element strides per sample, row and head (multiples of 8; 0 shares one sample), 16-byte aligned.
+ * out [B][Nq][H][d]; lse (opt) fp32 [B][H][Nq].  A query without a key: out 0, lse -inf.  Keys that do not exist are not read for their value.
+ * scratch: vidseg_context_attention_scratch_kib(...) KiB (0: none; -1: sizes refused). */
+int vidseg_context_attention_scratch_kib(int B, int Nq, int Np, int Nk, int H, int Hk, int d);
+int vidseg_context_attention_fwd(const void* q, long long q_b, long long q_n, long long q_h, const void* k_prefix, long long kp_n, long long kp_h,
+                                 const void* v_prefix, long long vp_n, long long vp_h, const void* k, long long k_b, long long k_n, long long k_h,
+                                 const void* v, long long v_b, long long v_n, long long v_h, const int* lens, const void* mask, long long mask_b,
+                                 void* out, float* lse, int dtype, int B, int Nq, int Np, int Nk, int H, int Hk, int d, float scale, int causal,
+                                 void* scratch, long long scratch_kib, vidseg_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -576,4 +576,4 @@ def add_rowvec(x, vec, rows_per_sample):
 
 
 # ----------------------------------------------------------------------------- operators of their tensors' own type, with gradients
-from .context_ops import groupnorm_act  # noqa: E402,F401
+from .context_ops import cross_attention, groupnorm_act, prefix_attention  # noqa: E402,F401
