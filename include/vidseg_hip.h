@@ -406,6 +406,16 @@ int vidseg_context_attention_fwd(const void* q, long long q_b, long long q_n, lo
                                  const void* v, long long v_b, long long v_n, long long v_h, const int* lens, const void* mask, long long mask_b,
                                  void* out, float* lse, int dtype, int B, int Nq, int Np, int Nk, int H, int Hk, int d, float scale, int causal,
                                  void* scratch, long long scratch_kib, vidseg_stream_t stream);
+/* its gradients (no prefix, not causal): out and lse as the forward call wrote them, dq [B][Nq][H][d], dk / dv [Bk][Nk][Hk][d] contiguous.  Bk = 1 < B: one sample of
+ * k / v serves all (k_b = v_b = 0) and its gradients are summed over the batch.  dk = dv = NULL: dq alone (more than 128 keys only).  Sums in a fixed order, no atomics.
+ * fp16: exact powers of two keep the intermediate gradients in range for |v| below 500.
+ * scratch: vidseg_context_attention_bwd_scratch_kib(...) KiB (-1: sizes refused). */
+int vidseg_context_attention_bwd_scratch_kib(int B, int Bk, int Nq, int Nk, int H, int Hk, int d);
+int vidseg_context_attention_bwd(const void* dout, long long g_b, long long g_n, long long g_h, const void* q, long long q_b, long long q_n, long long q_h,
+                                 const void* k, long long k_b, long long k_n, long long k_h, const void* v, long long v_b, long long v_n,
+                                 long long v_h, const int* lens, const void* mask, long long mask_b, const void* out, const float* lse, void* dq, void* dk,
+                                 void* dv, int dtype, int B, int Bk, int Nq, int Nk, int H, int Hk, int d, float scale, void* scratch,
+                                 long long scratch_kib, vidseg_stream_t stream);
 
 #ifdef __cplusplus
 }

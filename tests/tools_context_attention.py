@@ -5,6 +5,12 @@ Tolerance of an output o = sum p v / sum p whose probabilities p are rounded onc
     u sum p |v| / sum p                every p off by u relative (the sum itself is kept in fp32)
     2^-25 sum |v| / sum p              fp16 only: a p below 2^-14 is a subnormal, off by half of 2^-24 (the largest p of a part is 1)
     2 e sum p |v| / sum p              e: relative error of p from the fp32 scores, 2^-24 (d + 32) scale max sum |q k| + 2^-21 (exp2 and rescaling)
+
+Tolerance of the gradients, with ds = p (dp - D), dp = do v^T, D = sum do o:
+    dv: u |dv| + (u + 4 e) p^T |do|                                 p rounded once; its error now includes the saved log-sum-exp's
+    ds: (u + 4 e) |ds| + p (sum |do| tol(o)) + 2^-24 (d + 8) p (|do| |v|^T + sum |do o|)        rounded once; D is taken from the rounded o
+        + 2^-25 max|do| in fp16                                     (ds is scaled by a power of two >= 1 / max|do|, off by half a subnormal step)
+    dq: u |dq| + scale tol(ds) |k|,   dk: u |dk| + scale tol(ds)^T |q|,   each plus half a subnormal step of fp16
 """
 import math
 
@@ -70,6 +76,36 @@ class Reference:
             assert torch.equal(none, torch.isinf(g)) and (g[none] < 0).all()
             err = (g - self.lse).abs()[~none]
             assert (err <= 2 * self.e + 2.0 ** -22 * (1 + self.lse[~none].abs())).all(), f"{what} lse: worst {err.max():.3g}"
+
+    def check_gradients(self, dout, dq, dk, dv, shared, what=""):
+        B, H, Nq, Nk = self.p.shape
+        go = split(dout, self.heads)
+        u = U[self.dtype]
+        sub = 2.0 ** -25 if self.dtype == torch.float16 else 0.0
+        dp = go @ self.v.transpose(2, 3)
+        D = (go * self.o).sum(-1, keepdim=True)
+        ds = self.p * (dp - D)
+        r_dv, t_dv = self.p.transpose(2, 3) @ go, (u + 4 * self.e) * (self.p.transpose(2, 3) @ go.abs())
+        t_ds = (u + 4 * self.e) * ds.abs() + self.p * (go.abs() * self.tol).sum(-1, keepdim=True) + \
+            2.0 ** -24 * (self.d + 8) * self.p * (go.abs() @ self.v.abs().transpose(2, 3) + (go * self.o).abs().sum(-1, keepdim=True))
+        t_ds = (t_ds + sub * float(go.abs().max())) * self.live
+        r_dq, t_dq = self.scale * (ds @ self.k), self.scale * (t_ds @ self.k.abs())
+        r_dk, t_dk = self.scale * (ds.transpose(2, 3) @ self.q), self.scale * (t_ds.transpose(2, 3) @ self.q.abs())
+
+        def fold(t):                                                               # heads of a group, and the batch where one context serves it
+            t = t.view(B, self.kv_heads, H // self.kv_heads, Nk, self.d).sum(2)
+            return t.sum(0, keepdim=True) if shared else t
+        for n, got, r, t, heads in (("dq", dq, r_dq, t_dq, H), ("dk", dk, fold(r_dk), fold(t_dk), self.kv_heads), ("dv", dv, fold(r_dv), fold(t_dv), self.kv_heads)):
+            if got is None:
+                continue
+            g = split(got, heads)
+            tol = t + u * r.abs() + sub + 1e-30
+            bad = ~((g - r).abs() <= tol)
+            assert not bad.any(), f"{what} {n}: {int(bad.sum())} of {bad.numel()} outside, worst {((g - r).abs() / tol).max():.3g} of the tolerance"
+            if n != "dq":
+                dead = ~self.live.any(2)[:, 0]                                     # [B, Nk]
+                dead = dead.all(0, keepdim=True) if shared else dead
+                assert not got[dead.to(got.device)].any(), f"{what} {n}: a key that does not exist has a gradient"
 
 
 def randn(shape, seed, dtype, scale=1.0):

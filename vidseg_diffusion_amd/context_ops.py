@@ -1,7 +1,8 @@
 """Operators around the UNet's contexts (csrc/norm_act.hip, csrc/context_attn.hip): reached as `ops.<name>`.
 
     groupnorm_act       GroupNorm (+ SiLU) of a channels-last map, any C / G, fp32 / fp16 / bf16; differentiable
-    cross_attention     attention to an encoder's states of another length, per-sample lengths / key mask, heads of 8..128, grouped heads
+    cross_attention     attention to an encoder's states of another length, per-sample lengths / key mask, heads of 8..128, grouped heads;
+                        differentiable
     prefix_attention    attention of a batch to keys that all samples share and to each sample's own keys
 
 Unlike the `*_a16` operators of ops.py, which run in the library's one 16-bit type, these take the type of their tensors.  They launch
@@ -24,6 +25,8 @@ _lib.register({
     "vidseg_groupnorm_act_fwd": [_P, _L, _L, _I, _I, _L, _I, _I, _P, _P, _F, _I, _I, _P, _P, _P, _P, _L, _P],
     "vidseg_context_attention_scratch_kib": [_I, _I, _I, _I, _I, _I, _I],
     "vidseg_context_attention_fwd": [_P, _L, _L, _L] + [_P, _L, _L] * 2 + [_P, _L, _L, _L] * 2 + [_P, _P, _L, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _L, _P],
+    "vidseg_context_attention_bwd_scratch_kib": [_I, _I, _I, _I, _I, _I, _I],
+    "vidseg_context_attention_bwd": [_P, _L, _L, _L] * 4 + [_P, _P, _L, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _P, _L, _P],
     "vidseg_groupnorm_act_bwd": [_P, _L, _L, _P, _L, _L, _I, _I, _L, _I, _I, _P, _P, _P, _P, _I, _I, _P, _P, _P, _P, _L, _P],
 })
 
@@ -199,12 +202,49 @@ def _context_attention(q, k_prefix, v_prefix, k, v, heads, kv_heads, d, k_lens, 
     return out, lse
 
 
+class _CrossAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, heads, kv_heads, d, k_lens, key_mask, scale):
+        out, lse = _context_attention(q, None, None, k, v, heads, kv_heads, d, k_lens, key_mask, scale, 0, True)
+        ctx.save_for_backward(q, k, v, k_lens, key_mask, out, lse)
+        ctx.sizes = heads, kv_heads, d, scale
+        ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
+        return out, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout, _):
+        none = (None,) * 6
+        if dout is None:
+            return (None, None, None, *none)
+        q, k, v, k_lens, key_mask, out, lse = ctx.saved_tensors
+        heads, kv_heads, d, scale = ctx.sizes
+        (B, Nq), (Bk, Nk) = q.shape[:2], k.shape[:2]
+        if out.numel() == 0 or Nk == 0:
+            return (torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), *none)
+        want_kv = Nk <= 128 or ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) if on else None for t, on in ((q, True), (k, want_kv), (v, want_kv)))
+        operands = ()
+        for n, t, h in (("dout", dout, heads), ("q", q, heads), ("k", k, kv_heads), ("v", v, kv_heads)):
+            t, *strides = _heads_of(n, t, h, d)
+            operands += ((t, *strides),)
+        flat = [x for t, *strides in operands for x in (t.data_ptr(), *strides)]
+        kib = _lib.lib().vidseg_context_attention_bwd_scratch_kib(B, Bk, Nq, Nk, heads, kv_heads, d)
+        scratch = torch.empty(kib * 256, dtype=F32, device=q.device) if kib > 0 else None
+        mb = key_mask.stride(0) if key_mask is not None and key_mask.shape[0] > 1 else 0
+        _launch(q.device, "vidseg_context_attention_bwd", *flat, ptr(k_lens), ptr(key_mask), mb, out.data_ptr(), lse.data_ptr(), dq.data_ptr(), ptr(dk), ptr(dv),
+                _DTYPE[q.dtype], B, Bk, Nq, Nk, heads, kv_heads, d, scale, ptr(scratch), max(kib, 0))
+        return (dq, dk, dv, *none)
+
+
 def cross_attention(q, k, v, heads, *, kv_heads=None, k_lens=None, key_mask=None, scale=None, return_lse=False):
     """softmax(scale q k^T over the keys that exist) v, heads side by side: q [B, Nq, heads * d], k / v [B or 1, Nk, kv_heads * d] (the heads may also
     be a dimension of their own, in any order of strides; d a multiple of 8 up to 128; fp16 / bf16, fp32 inside; scale defaults to d^-1/2).
     Query head h reads key head h * kv_heads // heads.  One sample of k / v serves the whole batch.  A key exists if it lies below k_lens[b] (int32 [B] on the device)
     and key_mask[b or 0, key] (bool) is true; what k / v hold elsewhere, NaN included, reaches nothing, and a query without any key gets zeros.
-    return_lse: also log(sum exp) of the scores, fp32 [B, heads, Nq] (-inf without a key)  (attention.py:286-364)."""
+    return_lse: also log(sum exp) of the scores, fp32 [B, heads, Nq] (-inf without a key).  Differentiable (once) in q, k and v, not through the
+    log-sum-exp; in fp16 the gradients hold for |v| below 500.  Gradients of one shared k / v are summed over the batch  (attention.py:286-364)."""
     name = "cross_attention"
     B = q.shape[0] if q.dim() else 0
     d, kv_heads = _attention_shapes(name, q, heads, kv_heads, {"k": (k, (1, B)), "v": (v, (1, B))})
@@ -217,8 +257,10 @@ def cross_attention(q, k, v, heads, *, kv_heads=None, k_lens=None, key_mask=None
     scale = d ** -0.5 if scale is None else float(scale)
     _need(0 < scale < float("inf"), f"{name}: scale must be positive and finite")
     _need(q.is_cuda, f"{name}: q must be a HIP device tensor (no CPU path)")
-    _need(not (torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v))), f"{name}: carries no gradients (use it under torch.no_grad())")
-    out, lse = _context_attention(q, None, None, k, v, heads, kv_heads, d, k_lens, key_mask, scale, 0, return_lse)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        out, lse = _CrossAttention.apply(q, k, v, heads, kv_heads, d, k_lens, key_mask, scale)
+    else:
+        out, lse = _context_attention(q, None, None, k, v, heads, kv_heads, d, k_lens, key_mask, scale, 0, return_lse)
     return (out, lse) if return_lse else out
 
 

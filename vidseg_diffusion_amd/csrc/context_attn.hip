@@ -419,6 +419,442 @@ void launch_attn(AttnArgs p, int dtype, bool ws, long long tiles, long long head
     }
 }
 
+// ------------------------------------------------------------------------------------------------------------------------------------
+// Backward.  With L = lse log2 e and D = sum_d do o of a row:  p = exp2(s c - L),  dp = do v^T,  ds = p (dp - D),
+//   dv = p^T do,   dk = scale ds^T q,   dq = scale ds k.
+// p and ds are rounded once to the storage type before they enter a product.  fp16 needs both kept away from its subnormals (p of a row over
+// 4096 keys is 2^-12, its ds smaller still): p is carried as 2^12 p, ds with a power of two that brings the largest |do| in sight to [1, 2) --
+// exact factors that leave in fp32 at the end.  |ds| 2^k <= d max|v| then, inside fp16 for |v| below 500.
+struct BwdArgs {
+    const u16 *q, *k, *v, *o, *go;
+    long long q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h, g_b, g_n, g_h;
+    const float* lse;
+    float* delta;              // [B][H][Nq]: D, written by the dq kernel for the dk / dv kernel
+    const int* lens;
+    const unsigned char* mask;
+    long long mask_b;
+    u16 *dq, *dk, *dv;         // contiguous [B][Nq][H][d], [Bk][Nk][Hk][d]
+    float* part;               // [chunks][2][Bk][Nk][Hk][d] or null: one chunk, written as it is
+    int B, Bk, Nq, Nk, H, Hk, G, d;
+    float c, scale;
+    int xtiles, chunks, per_chunk;
+};
+
+template <bool BF> __device__ __forceinline__ float dot2(unsigned a, unsigned b, float acc) {
+    if constexpr (BF) return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, a), __builtin_bit_cast(b2, b), acc, false);
+    else return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, a), __builtin_bit_cast(h2, b), acc, false);
+}
+__device__ __forceinline__ unsigned max_abs2(unsigned m, unsigned w) {          // the larger magnitude of each half (fp16 bits order like integers)
+    typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(us2, m), __builtin_bit_cast(us2, w & 0x7fff7fffu)));
+}
+// 2^-floor(log2 a) of the larger half, 1 for zero
+__device__ __forceinline__ float scale_of(unsigned m) {
+    const unsigned h = max(m & 0xffffu, m >> 16);
+    const float a = (float)__builtin_bit_cast(_Float16, (unsigned short)h);
+    const unsigned e = __float_as_uint(a) >> 23;
+    return h ? __uint_as_float((254u - min(e, 253u)) << 23) : 1.0f;
+}
+
+constexpr float P_LOG2 = 12.f;                                                   // fp16: p as 2^12 p
+
+// dq: a wave owns 32 rows as accumulator columns, the block's waves share key tiles of 64 (the forward kernel's arrangement)
+template <bool BF, int DP> __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) k_ctx_bwd_q(BwdArgs p) {
+    constexpr int KT = 64, SL = DP / 8, NST = KT * SL / 256, ND = DP / 32;
+    __shared__ __attribute__((aligned(16))) u16 sK[2][KT * DP], sV[2][KT * DP];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, hi = lane >> 5;
+    int y, xt;
+    block_of(p.xtiles, y, xt);
+    const int hk = y % p.Hk, b = y / p.Hk, rows = p.Nq * p.G;
+    const int r = xt * 128 + wave * 32 + l31;
+    const bool on = r < rows;
+    const int rr = min(r, rows - 1), qi = rr / p.G, h = hk * p.G + rr % p.G;
+    const long long id = ((long long)b * p.Nq + qi) * p.H + h;
+    u32x4 fq[DP / 16], fg[DP / 16];
+    float D = 0.f;
+    unsigned amax = 0;
+    {
+        const u16 *qp = p.q + b * p.q_b + qi * p.q_n + h * p.q_h, *gp = p.go + b * p.g_b + qi * p.g_n + h * p.g_h, *op = p.o + id * p.d;
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) {
+            const int at = s * 16 + hi * 8, a = at < p.d ? at : 0;
+            fq[s] = *reinterpret_cast<const u32x4*>(qp + a);
+            fg[s] = *reinterpret_cast<const u32x4*>(gp + a);
+            const u32x4 fo = *reinterpret_cast<const u32x4*>(op + a);
+            if (at >= p.d) fq[s] = fg[s] = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                D = dot2<BF>(fg[s][e], fo[e], D);
+                if (!BF) amax = max_abs2(amax, fg[s][e]);
+            }
+        }
+    }
+    D = half_sum(D);
+    const long long bhq = ((long long)b * p.H + h) * p.Nq + qi;
+    const float lse = p.lse[bhq];
+    const float L = lse == -INFINITY ? INFINITY : lse * LOG2E;                  // a row without a key: p = 0
+    if (on && hi == 0) p.delta[bhq] = D;
+    float fs = 1.f, back = p.scale;
+    if (!BF) {
+        const auto t = __builtin_amdgcn_permlane32_swap(amax, amax, false, false);
+        fs = scale_of(max_abs2(t[0], t[1]));
+        back = p.scale / fs;
+    }
+    const int len = p.lens ? max(0, min(p.lens[b], p.Nk)) : p.Nk, T = (len + KT - 1) / KT;
+    const u16 *kb = p.k + b * p.k_b + hk * p.k_h, *vb = p.v + b * p.v_b + hk * p.v_h;
+    const unsigned char* mk = p.mask ? p.mask + b * p.mask_b : nullptr;
+    u32x4 rk[NST], rv[NST];
+    unsigned long long live = 0;
+    auto load_tile = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < NST; ++i) {
+            const int id = tid + 256 * i, row = id / SL, slot = id % SL, key = t * KT + row, kk = min(key, len - 1);
+            const bool ok = key < len && slot * 8 < p.d && (!mk || mk[kk]);
+            const int at = slot * 8 < p.d ? slot * 8 : 0;
+            rk[i] = *reinterpret_cast<const u32x4*>(kb + kk * p.k_n + at);
+            rv[i] = *reinterpret_cast<const u32x4*>(vb + kk * p.v_n + at);
+            if (!ok) rk[i] = rv[i] = u32x4{0u, 0u, 0u, 0u};
+        }
+        const int key = t * KT + lane;
+        live = __ballot(key < len && (!mk || mk[min(key, len - 1)]));
+    };
+    auto store_tile = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < NST; ++i) {
+            const int id = tid + 256 * i;
+            *reinterpret_cast<u32x4*>(&sK[buf][slot_at<DP>(id / SL, id % SL)]) = rk[i];
+            *reinterpret_cast<u32x4*>(&sV[buf][slot_at<DP>(id / SL, id % SL)]) = rv[i];
+        }
+    };
+    f32x16 acc[ND];
+#pragma unroll
+    for (int n = 0; n < ND; ++n)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[n][e] = 0.f;
+    if (T > 0) {
+        load_tile(0);
+        store_tile(0);
+    }
+    __syncthreads();
+    for (int t = 0; t < T; ++t) {
+        const int buf = t & 1;
+        const unsigned long long now = live;
+        if (t + 1 < T) load_tile(t + 1);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const unsigned keys = (unsigned)(now >> (32 * j));
+            if (keys == 0) continue;
+            f32x16 s, dp;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
+#pragma unroll
+            for (int e = 0; e < DP / 16; ++e) {
+                s = mfma<BF>(read_row<DP>(sK[buf], j * 32 + l31, e * 2 + hi), fq[e], s);
+                dp = mfma<BF>(read_row<DP>(sV[buf], j * 32 + l31, e * 2 + hi), fg[e], dp);
+            }
+            if (keys != ~0u) {
+                const unsigned bits = keys >> (4 * hi);
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (!((bits >> ((e & 3) + 8 * (e >> 2))) & 1u)) s[e] = -INFINITY;
+            }
+            u32x4 fd[2];
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+                float a = __builtin_amdgcn_exp2f(fmaf(s[e], p.c, -L)) * (dp[e] - D), d = __builtin_amdgcn_exp2f(fmaf(s[e + 1], p.c, -L)) * (dp[e + 1] - D);
+                if (!BF) {
+                    a *= fs;
+                    d *= fs;
+                }
+                fd[e >> 3][(e >> 1) & 3] = pack2<BF>(a, d);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int n = 0; n < ND; ++n) acc[n] = mfma<BF>(read_tr<DP>(sK[buf], j * 32 + e * 16, n * 32, lane), fd[e], acc[n]);
+        }
+        if (t + 1 < T) store_tile(buf ^ 1);
+        __syncthreads();
+    }
+    if (!on) return;
+#pragma unroll
+    for (int n = 0; n < ND; ++n)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const int c = n * 32 + 2 * e + 4 * hi;
+            if (c < p.d) *reinterpret_cast<u32x2*>(p.dq + id * p.d + c) = u32x2{pack2<BF>(acc[n][e] * back, acc[n][e + 1] * back), pack2<BF>(acc[n][e + 2] * back, acc[n][e + 3] * back)};
+        }
+}
+
+// dk and dv: a wave owns 32 keys as accumulator columns (K, V in registers), the block 128, and walks over tiles of 64 rows; the rows of all samples
+// where they share one context.  FUSED (at most 128 keys): the block holds every key of its rows, so dq comes out of the same pass -- ds goes
+// through LDS once more, each wave takes its share of the [64][d] tile of ds k -- and q, o and do are read once in all.
+template <bool BF, int DP, bool FUSED> __global__ void __launch_bounds__(256, DP == 64 ? 2 : 1) k_ctx_bwd_kv(BwdArgs p) {
+    constexpr int RT = 64, SLP = DP == 64 ? 8 : 16, NST = RT * SLP / 256, ND = DP / 32;
+    __shared__ __attribute__((aligned(16))) u16 sQ[2][RT * DP], sG[2][RT * DP], sK[FUSED ? 128 * DP : 8], sS[FUSED ? 128 * RT : 8];
+    __shared__ __attribute__((aligned(16))) float sL[2][RT], sD[2][RT];
+    __shared__ unsigned sM[2][4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, hi = lane >> 5;
+    int y, kt;
+    block_of(p.xtiles, y, kt);
+    const int chunk = y % p.chunks;
+    y /= p.chunks;
+    const int hk = y % p.Hk, bk = y / p.Hk;                                      // bk: sample of k and v
+    const bool shared = p.Bk < p.B;
+    const int rows = p.Nq * p.G, tiles = (rows + RT - 1) / RT;
+    const long long all = (long long)tiles * (shared ? p.B : 1);
+    const long long t0 = (long long)chunk * p.per_chunk, t1 = t0 + p.per_chunk < all ? t0 + p.per_chunk : all;
+    const int key = kt * 128 + wave * 32 + l31;
+    const bool in = key < p.Nk;
+    // a key that no sample of this block has is taken as zero, so nothing that lies there reaches a product
+    auto lives = [&](int b) { return in && (!p.lens || key < p.lens[b]) && (!p.mask || p.mask[b * p.mask_b + key]); };
+    bool any = false;
+    if (shared) {
+        for (int b = 0; b < p.B; ++b) any |= lives(b);
+    } else {
+        any = lives(bk);
+    }
+    u32x4 fk[DP / 16], fv[DP / 16];
+    {
+        const int kk = in ? key : 0;
+        const u16 *kp = p.k + bk * p.k_b + kk * p.k_n + hk * p.k_h, *vp = p.v + bk * p.v_b + kk * p.v_n + hk * p.v_h;
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) {
+            const int at = s * 16 + hi * 8, a = at < p.d ? at : 0;
+            fk[s] = *reinterpret_cast<const u32x4*>(kp + a);
+            fv[s] = *reinterpret_cast<const u32x4*>(vp + a);
+            if (at >= p.d || !any) fk[s] = fv[s] = u32x4{0u, 0u, 0u, 0u};
+            if (FUSED) *reinterpret_cast<u32x4*>(sK + slot_at<DP>(wave * 32 + l31, s * 2 + hi)) = fk[s];
+        }
+    }
+    u32x4 rq[NST], rg[NST];
+    float rL = INFINITY, rD = 0.f, rDf[NST];
+    unsigned rmax = 0;
+    const int slot = tid % SLP, trow = tid / SLP;
+    auto load_tile = [&](long long t) {
+        const int b = shared ? (int)(t / tiles) : bk, base = (int)(t % tiles) * RT;
+        rmax = 0;
+#pragma unroll
+        for (int i = 0; i < NST; ++i) {
+            const int r = base + trow + i * (256 / SLP), rr = min(r, rows - 1), qi = rr / p.G, h = hk * p.G + rr % p.G;
+            const bool ok = r < rows && slot * 8 < p.d;
+            const int at = slot * 8 < p.d ? slot * 8 : 0;
+            rq[i] = *reinterpret_cast<const u32x4*>(p.q + b * p.q_b + qi * p.q_n + h * p.q_h + at);
+            rg[i] = *reinterpret_cast<const u32x4*>(p.go + b * p.g_b + qi * p.g_n + h * p.g_h + at);
+            if (!ok) rq[i] = rg[i] = u32x4{0u, 0u, 0u, 0u};
+            if (FUSED) {
+                const u32x4 fo = *reinterpret_cast<const u32x4*>(p.o + (((long long)b * p.Nq + qi) * p.H + h) * p.d + at);
+                rDf[i] = 0.f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) rDf[i] = dot2<BF>(rg[i][e], fo[e], rDf[i]);
+            }
+            if (!BF)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) rmax = max_abs2(rmax, rg[i][e]);
+        }
+        if (tid < RT) {
+            const int r = base + tid, rr = min(r, rows - 1);
+            const long long at = ((long long)b * p.H + hk * p.G + rr % p.G) * p.Nq + rr / p.G;
+            const float lse = p.lse[at];
+            rL = r >= rows || lse == -INFINITY ? INFINITY : lse * LOG2E - (BF ? 0.f : P_LOG2);
+            if (!FUSED) rD = r < rows ? p.delta[at] : 0.f;
+        }
+    };
+    auto store_tile = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < NST; ++i) {
+            const int r = trow + i * (256 / SLP);
+            if (DP != 96 || slot < DP / 8) {
+                *reinterpret_cast<u32x4*>(&sQ[buf][slot_at<DP>(r, slot)]) = rq[i];
+                *reinterpret_cast<u32x4*>(&sG[buf][slot_at<DP>(r, slot)]) = rg[i];
+            }
+            if (FUSED) {
+                float x = rDf[i];
+#pragma unroll
+                for (int o = SLP / 2; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
+                if (slot == 0) sD[buf][r] = x;
+            }
+        }
+        if (tid < RT) {
+            sL[buf][tid] = rL;
+            if (!FUSED) sD[buf][tid] = rD;
+        }
+        if (!BF) {
+            unsigned m = rmax;
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) m = max_abs2(m, __shfl_xor(m, o, 64));
+            if (lane == 0) sM[buf][wave] = m;
+        }
+    };
+    f32x16 ak[ND], av[ND];
+#pragma unroll
+    for (int n = 0; n < ND; ++n)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) ak[n][e] = av[n][e] = 0.f;
+    float run = BF ? 1.f : 1.152921504606846976e18f;                            // 2^60: any tile with a gradient in it lowers it
+    if (t0 < t1) {
+        load_tile(t0);
+        store_tile(0);
+    }
+    __syncthreads();
+    for (long long t = t0; t < t1; ++t) {
+        const int buf = (int)(t - t0) & 1;
+        const int b = shared ? (int)(t / tiles) : bk, base = (int)(t % tiles) * RT;
+        if (t + 1 < t1) load_tile(t + 1);
+        const bool live = lives(b), whole = __all(live);
+        float fs = 1.f;
+        if (!BF) {
+            unsigned m = max_abs2(max_abs2(sM[buf][0], sM[buf][1]), max_abs2(sM[buf][2], sM[buf][3]));
+            const float now = scale_of(m);
+            if (m && now < run) {
+                const float f = now / run;
+#pragma unroll
+                for (int n = 0; n < ND; ++n)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) ak[n][e] *= f;
+                run = now;
+            }
+            fs = run * 2.44140625e-4f;                                          // 2^-12 takes p's factor out of ds
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            f32x16 s, dp;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
+#pragma unroll
+            for (int e = 0; e < DP / 16; ++e) {
+                s = mfma<BF>(read_row<DP>(sQ[buf], i * 32 + l31, e * 2 + hi), fk[e], s);
+                dp = mfma<BF>(read_row<DP>(sG[buf], i * 32 + l31, e * 2 + hi), fv[e], dp);
+            }
+            if (!whole)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (!live) s[e] = -INFINITY;
+            u32x4 fp[2], fd[2];
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const f32x4 L = *reinterpret_cast<const f32x4*>(&sL[buf][i * 32 + 2 * e + 4 * hi]), D = *reinterpret_cast<const f32x4*>(&sD[buf][i * 32 + 2 * e + 4 * hi]);
+                float x[4], z[4];
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    x[w] = __builtin_amdgcn_exp2f(fmaf(s[e + w], p.c, -L[w]));
+                    z[w] = x[w] * (dp[e + w] - D[w]);
+                    if (!BF) z[w] *= fs;
+                }
+#pragma unroll
+                for (int w = 0; w < 4; w += 2) {
+                    fp[e >> 3][((e + w) >> 1) & 3] = pack2<BF>(x[w], x[w + 1]);
+                    fd[e >> 3][((e + w) >> 1) & 3] = pack2<BF>(z[w], z[w + 1]);
+                }
+                if (FUSED)                                                      // [key][row]: rows i 32 + 2 e + 4 hi + 0..3
+                    *reinterpret_cast<u32x2*>(sS + slot_at<RT>(wave * 32 + l31, i * 4 + (e >> 2)) + 4 * hi) = u32x2{fd[e >> 3][(e >> 1) & 3], fd[e >> 3][((e >> 1) & 3) + 1]};
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int n = 0; n < ND; ++n) {
+                    av[n] = mfma<BF>(read_tr<DP>(sG[buf], i * 32 + e * 16, n * 32, lane), fp[e], av[n]);
+                    ak[n] = mfma<BF>(read_tr<DP>(sQ[buf], i * 32 + e * 16, n * 32, lane), fd[e], ak[n]);
+                }
+        }
+        if (t + 1 < t1) store_tile(buf ^ 1);
+        __syncthreads();
+        if constexpr (FUSED) {
+            const float back = p.scale / run;
+            for (int w = wave; w < 2 * ND; w += 4) {
+                const int i = w & 1, n = w >> 1;
+                f32x16 acc;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) acc = mfma<BF>(read_tr<DP>(sK, e * 16, n * 32, lane), read_tr<RT>(sS, e * 16, i * 32, lane), acc);
+                const int r = base + i * 32 + l31;
+                if (r < rows) {
+                    const long long id = ((long long)b * p.Nq + r / p.G) * p.H + hk * p.G + r % p.G;
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) {
+                        const int c = n * 32 + 2 * e + 4 * hi;
+                        if (c < p.d)
+                            *reinterpret_cast<u32x2*>(p.dq + id * p.d + c) = u32x2{pack2<BF>(acc[e] * back, acc[e + 1] * back), pack2<BF>(acc[e + 2] * back, acc[e + 3] * back)};
+                    }
+                }
+            }
+            __syncthreads();                                                    // sS is written again in the next round
+        }
+    }
+    if (!in) return;
+    const float bk_ = p.scale / run, bv_ = BF ? 1.f : 2.44140625e-4f;
+    const long long at = (((long long)bk * p.Nk + key) * p.Hk + hk) * p.d, plane = (long long)p.Bk * p.Nk * p.Hk * p.d;
+#pragma unroll
+    for (int n = 0; n < ND; ++n)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const int c = n * 32 + 2 * e + 4 * hi;
+            if (c >= p.d) continue;
+            if (p.part) {
+                float* o = p.part + 2 * chunk * plane + at + c;
+                *reinterpret_cast<f32x4*>(o) = f32x4{ak[n][e] * bk_, ak[n][e + 1] * bk_, ak[n][e + 2] * bk_, ak[n][e + 3] * bk_};
+                *reinterpret_cast<f32x4*>(o + plane) = f32x4{av[n][e] * bv_, av[n][e + 1] * bv_, av[n][e + 2] * bv_, av[n][e + 3] * bv_};
+            } else {
+                *reinterpret_cast<u32x2*>(p.dk + at + c) = u32x2{pack2<BF>(ak[n][e] * bk_, ak[n][e + 1] * bk_), pack2<BF>(ak[n][e + 2] * bk_, ak[n][e + 3] * bk_)};
+                *reinterpret_cast<u32x2*>(p.dv + at + c) = u32x2{pack2<BF>(av[n][e] * bv_, av[n][e + 1] * bv_), pack2<BF>(av[n][e + 2] * bv_, av[n][e + 3] * bv_)};
+            }
+        }
+}
+
+// dk (y = 0) and dv (y = 1): the chunks' partial sums in their order
+template <bool BF> __global__ void __launch_bounds__(256) k_ctx_bwd_sum(const float* __restrict__ part, int chunks, long long plane, u16* __restrict__ dk, u16* __restrict__ dv) {
+    const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= plane) return;
+    const float* o = part + blockIdx.y * plane + i;
+    f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int c = 0; c < chunks; ++c) {
+        const f32x4 t = *reinterpret_cast<const f32x4*>(o + 2 * c * plane);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] += t[e];
+    }
+    *reinterpret_cast<u32x2*>((blockIdx.y ? dv : dk) + i) = u32x2{pack2<BF>(a[0], a[1]), pack2<BF>(a[2], a[3])};
+}
+
+struct BwdPlan {
+    bool fused;
+    int ktiles, chunks, per_chunk;
+    long long delta_floats, part_floats;
+};
+BwdPlan make_bwd_plan(int B, int Bk, int Nq, int Nk, int H, int Hk, int d) {
+    BwdPlan s{};
+    s.fused = Nk <= 128;
+    s.ktiles = (Nk + 127) / 128;
+    const long long tiles = ((long long)Nq * (H / Hk) + 63) / 64 * (Bk < B ? B : 1), blocks = (long long)Bk * Hk * s.ktiles;
+    const long long want = blocks >= 384 ? 1 : (512 + blocks - 1) / blocks;      // about two blocks a CU, at least two tiles each
+    long long per = (tiles + want - 1) / want;
+    if (per < 2) per = 2;
+    s.per_chunk = (int)per;
+    s.chunks = (int)((tiles + per - 1) / per);
+    s.delta_floats = s.fused ? 0 : ((long long)B * H * Nq + 3) / 4 * 4;
+    s.part_floats = s.chunks > 1 ? 2ll * s.chunks * Bk * Nk * Hk * d : 0;
+    return s;
+}
+
+template <bool BF, int DP> void launch_bwd(BwdArgs p, const BwdPlan& s, bool want_kv, hipStream_t st) {
+    const unsigned kv_blocks = (unsigned)(s.ktiles * s.chunks * (long long)p.Bk * p.Hk);
+    if (s.fused) {
+        p.xtiles = 1;
+        hipLaunchKernelGGL((k_ctx_bwd_kv<BF, DP, true>), dim3(kv_blocks), dim3(256), 0, st, p);
+    } else {
+        p.xtiles = (p.Nq * p.G + 127) / 128;
+        hipLaunchKernelGGL((k_ctx_bwd_q<BF, DP>), dim3((unsigned)(p.xtiles * (long long)p.B * p.Hk)), dim3(256), 0, st, p);
+        if (!want_kv) return;
+        p.xtiles = s.ktiles;
+        hipLaunchKernelGGL((k_ctx_bwd_kv<BF, DP, false>), dim3(kv_blocks), dim3(256), 0, st, p);
+    }
+    if (s.chunks > 1) {
+        const long long plane = (long long)p.Bk * p.Nk * p.Hk * p.d;
+        hipLaunchKernelGGL((k_ctx_bwd_sum<BF>), dim3((unsigned)((plane / 4 + 255) / 256), 2), dim3(256), 0, st, p.part, s.chunks, plane, p.dk, p.dv);
+    }
+}
+
 bool row_strides_ok(const void* p, long long a, long long b, long long c) { return ((uintptr_t)p % 16) == 0 && a % 8 == 0 && b % 8 == 0 && c % 8 == 0; }
 
 int check_sizes(const char* name, int dtype, int B, int Nq, int Np, int Nk, int H, int Hk, int d, float scale) {
@@ -487,6 +923,49 @@ int vidseg_context_attention_fwd(const void* q, long long q_b, long long q_n, lo
         else hipLaunchKernelGGL((k_ctx_join<false>), dim3(blocks), dim3(256), 0, st, p.po, p.pml, s.parts, total, d, Nq, H, p.o, lse);
     }
     VS_CHECK_LAUNCH("context_attention");
+    return VS_OK;
+}
+
+int vidseg_context_attention_bwd_scratch_kib(int B, int Bk, int Nq, int Nk, int H, int Hk, int d) {
+    if (check_sizes("context_attention_bwd", 1, B, Nq, 0, Nk, H, Hk, d, 1.f) || (Bk != 1 && Bk != B)) return -1;
+    const BwdPlan s = make_bwd_plan(B, Bk, Nq, Nk, H, Hk, d);
+    return (int)(((s.delta_floats + s.part_floats) * 4 + 1023) / 1024);
+}
+
+int vidseg_context_attention_bwd(const void* dout, long long g_b, long long g_n, long long g_h, const void* q, long long q_b, long long q_n, long long q_h,
+                                 const void* k, long long k_b, long long k_n, long long k_h, const void* v, long long v_b, long long v_n,
+                                 long long v_h, const int* lens, const void* mask, long long mask_b, const void* out, const float* lse, void* dq, void* dk,
+                                 void* dv, int dtype, int B, int Bk, int Nq, int Nk, int H, int Hk, int d, float scale, void* scratch,
+                                 long long scratch_kib, hipStream_t st) {
+    const int rc = check_sizes("context_attention_bwd", dtype, B, Nq, 0, Nk, H, Hk, d, scale);
+    if (rc) return rc;
+    VS_REQUIRE(Nk >= 1 && (Bk == 1 || Bk == B), "context_attention_bwd: Nk=%d, %d samples of k for %d", Nk, Bk, B);
+    VS_REQUIRE(dout && q && k && v && out && lse && dq && (!dk == !dv), "context_attention_bwd: null operand");
+    VS_REQUIRE(row_strides_ok(dout, g_b, g_n, g_h) && row_strides_ok(q, q_b, q_n, q_h) && row_strides_ok(k, k_b, k_n, k_h) && row_strides_ok(v, v_b, v_n, v_h) &&
+                   row_strides_ok(out, 0, 0, 0) && row_strides_ok(dq, 0, 0, 0) && row_strides_ok(dk, 0, 0, 0) && row_strides_ok(dv, 0, 0, 0),
+               "context_attention_bwd: operands must be 16-byte aligned with strides that are multiples of 8 elements");
+    const BwdPlan s = make_bwd_plan(B, Bk, Nq, Nk, H, Hk, d);
+    VS_REQUIRE((long long)s.ktiles * s.chunks * Bk * Hk < (1ll << 24), "context_attention_bwd: Nk=%d, Hk=%d are too many blocks", Nk, Hk);
+    VS_REQUIRE(dk || !s.fused, "context_attention_bwd: up to 128 keys all three gradients come out of one pass");
+    const long long need = ((s.delta_floats + s.part_floats) * 4 + 1023) / 1024;
+    VS_REQUIRE(need == 0 || (scratch && scratch_kib >= need), "context_attention_bwd: scratch of %lld KiB, needs %lld", scratch_kib, need);
+    BwdArgs p{};
+    p.q = (const u16*)q; p.q_b = q_b; p.q_n = q_n; p.q_h = q_h; p.k = (const u16*)k; p.k_b = k_b; p.k_n = k_n; p.k_h = k_h;
+    p.v = (const u16*)v; p.v_b = v_b; p.v_n = v_n; p.v_h = v_h; p.go = (const u16*)dout; p.g_b = g_b; p.g_n = g_n; p.g_h = g_h;
+    p.o = (const u16*)out; p.lse = lse; p.delta = (float*)scratch; p.lens = lens; p.mask = (const unsigned char*)mask; p.mask_b = mask_b;
+    p.dq = (u16*)dq; p.dk = (u16*)dk; p.dv = (u16*)dv; p.part = s.part_floats ? (float*)scratch + s.delta_floats : nullptr;
+    p.B = B; p.Bk = Bk; p.Nq = Nq; p.Nk = Nk; p.H = H; p.Hk = Hk; p.G = H / Hk; p.d = d; p.c = scale * LOG2E; p.scale = scale;
+    p.chunks = s.chunks; p.per_chunk = s.per_chunk;
+    if (dtype == 2) {
+        if (d <= 64) launch_bwd<true, 64>(p, s, dk != nullptr, st);
+        else if (d <= 96) launch_bwd<true, 96>(p, s, dk != nullptr, st);
+        else launch_bwd<true, 128>(p, s, dk != nullptr, st);
+    } else {
+        if (d <= 64) launch_bwd<false, 64>(p, s, dk != nullptr, st);
+        else if (d <= 96) launch_bwd<false, 96>(p, s, dk != nullptr, st);
+        else launch_bwd<false, 128>(p, s, dk != nullptr, st);
+    }
+    VS_CHECK_LAUNCH("context_attention_bwd");
     return VS_OK;
 }
 
