@@ -389,7 +389,7 @@ int vidseg_groupnorm_act_fwd(const void* x, long long x_batch_stride, long long 
                              const float* gamma, const float* beta, float eps, int act, int rows_per_chunk, void* y, float* mean, float* rstd,
                              float* scratch, long long scratch_floats, vidseg_stream_t stream);
 /* its gradients: dx contiguous [B][HW][C] in x's type, dgamma / dbeta fp32 [C] summed over the batch (fixed order, no atomics).
- * scratch: B * ((nchunk + 1) * 2 * C + 2 * G) floats. */
+ * scratch: 2 * B * nchunk * (C + G) floats. */
 int vidseg_groupnorm_act_bwd(const void* dy, long long dy_batch_stride, long long dy_row_stride, const void* x, long long x_batch_stride,
                              long long x_row_stride, int dtype, int B, long long HW, int C, int G, const float* gamma, const float* beta,
                              const float* mean, const float* rstd, int act, int rows_per_chunk, void* dx, float* dgamma, float* dbeta,

@@ -7,14 +7,15 @@
 //
 // Everything is held in fp32 between the load and the one rounding of the store.  A thread owns VEC neighbouring channels (16 bytes) of
 // every R-th row, so a wave reads whole rows; sums go channel -> group only after the rows are summed, so any C / G works, also
-// groups that end inside a 16-byte piece (320 channels in 32 groups of 10).  The forward pass is two launches (chunk statistics; merge and apply), the
-// backward three (channel sums; their merge over the chunks; dx, with dgamma and dbeta in extra blocks): no atomics, every sum has one order.
+// groups that end inside a 16-byte piece (320 channels in 32 groups of 10).  Two launches forward (chunk statistics; merge and apply) and
+// two backward (channel and group sums of a chunk; merge and dx, with dgamma and dbeta in extra blocks): no atomics, every sum has one order.
 // A chunk's row count depends on HW and C only, so a sample's result does not depend on the batch it is in.
 #include "common.h"
 
 namespace {
 
 constexpr int NT = 256;
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 template <typename T> struct Stored;
 template <> struct Stored<float> {
@@ -70,9 +71,8 @@ struct NormArgs {
     const float *gamma, *beta;
     void* out;                            // y or dx, contiguous [B][HW][C]
     float *mean, *rstd;                   // [B][G]
-    float* part;                          // forward: [B][nchunk][G][2] (mean, M2); backward: [B][nchunk][2][C]
-    float* chan;                          // backward: [B][2][C] sums of dz and dz * xh
-    float* coef;                          // backward: [B][G][2] group means of gamma * dz and gamma * dz * xh
+    float* part;                          // [B][nchunk][G][2]; forward (mean, M2) of a group over a chunk, backward its sums of gamma * dz and gamma * dz * xh
+    float* chan;                          // backward: [B][nchunk][2][C] sums of dz and dz * xh over a chunk
     float *dgamma, *dbeta;
 };
 
@@ -90,6 +90,17 @@ template <int VEC> __device__ __forceinline__ void fold_rows(float* s0, float* s
         s1[c] = b;
     }
     __syncthreads();
+}
+
+// Lanes that share the work of one group: a power of two up to a wave's 64, so that G * lanes fills the block
+__device__ __forceinline__ int lanes_per(int G) {
+    int l = 1;
+    while (l < 64 && G * l * 2 <= NT) l *= 2;
+    return l;
+}
+__device__ __forceinline__ float lanes_sum(float v, int lanes) {
+    for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
 }
 
 // ---- forward, launch 1: (mean, M2) of every group over the rows of one chunk.
@@ -143,18 +154,18 @@ template <typename T, int VEC> __global__ void __launch_bounds__(NT) k_gna_stats
         }
         __syncthreads();
     }
-    const int cg = C / p.G;
-    for (int g = threadIdx.x; g < p.G; g += NT) {
+    const int cg = C / p.G, lanes = lanes_per(p.G), sub = threadIdx.x % lanes, stride = NT / lanes;
+    for (int g0 = 0; g0 < p.G; g0 += stride) {                      // whole waves take part in the shuffles; lanes past G work on the last group
+        const int g = min(g0 + (int)threadIdx.x / lanes, p.G - 1);
         float m = 0.f, m2 = 0.f;
-        for (int c = 0; c < cg; ++c) m += ch_mean[g * cg + c];
-        m /= (float)cg;
-        for (int c = 0; c < cg; ++c) {
+        for (int c = sub; c < cg; c += lanes) m += ch_mean[g * cg + c];
+        m = lanes_sum(m, lanes) / (float)cg;
+        for (int c = sub; c < cg; c += lanes) {
             const float d = ch_mean[g * cg + c] - m;
             m2 += ch_m2[g * cg + c] + (float)n * d * d;
         }
-        float* o = p.part + (((long long)b * p.nchunk + chunk) * p.G + g) * 2;
-        o[0] = m;
-        o[1] = m2;
+        m2 = lanes_sum(m2, lanes);
+        if (sub == 0) *reinterpret_cast<f32x2*>(p.part + (((long long)b * p.nchunk + chunk) * p.G + g) * 2) = f32x2{m, m2};
     }
 }
 
@@ -164,25 +175,31 @@ template <typename T, int VEC> __global__ void __launch_bounds__(NT) k_gna_apply
     const int C = p.C, cols = C / VEC, b = blockIdx.y, chunk = blockIdx.x, cg = C / p.G;
     float* g_mean = lds;
     float* g_rstd = lds + p.G;
-    for (int g = threadIdx.x; g < p.G; g += NT) {
-        const float* o = p.part + ((long long)b * p.nchunk * p.G + g) * 2;
-        float m = 0.f, m2 = 0.f;
-        for (int i = 0; i < p.nchunk; ++i) {
+    const int lanes = lanes_per(p.G), sub = threadIdx.x % lanes, stride = NT / lanes;
+    for (int g0 = 0; g0 < p.G; g0 += stride) {
+        const int g = min(g0 + (int)threadIdx.x / lanes, p.G - 1);
+        const f32x2* o = reinterpret_cast<const f32x2*>(p.part) + (long long)b * p.nchunk * p.G + g;
+        // one pass about the first chunk's mean k: mean = k + s / HW, M2 = q - HW cg (mean - k)^2, where |mean - k| is of the spread's size
+        const float k = o[0][0];
+        float s = 0.f, q = 0.f;
+#pragma unroll 4
+        for (int i = sub; i < p.nchunk; i += lanes) {
             const float n = (float)(i + 1 < p.nchunk ? p.rows : (int)(p.HW - (long long)i * p.rows));
-            m += n * o[(long long)i * p.G * 2];
+            const f32x2 t = o[(long long)i * p.G];
+            const float d = t[0] - k;
+            s += n * d;
+            q += t[1] + n * (float)cg * d * d;
         }
-        m /= (float)p.HW;
-        for (int i = 0; i < p.nchunk; ++i) {
-            const float n = (float)(i + 1 < p.nchunk ? p.rows : (int)(p.HW - (long long)i * p.rows)) * (float)cg;
-            const float d = o[(long long)i * p.G * 2] - m;
-            m2 += o[(long long)i * p.G * 2 + 1] + n * d * d;
-        }
-        const float rstd = 1.0f / sqrtf(m2 / ((float)p.HW * (float)cg) + p.eps);
-        g_mean[g] = m;
-        g_rstd[g] = rstd;
-        if (p.mean && chunk == 0) {
-            p.mean[(long long)b * p.G + g] = m;
-            p.rstd[(long long)b * p.G + g] = rstd;
+        s = lanes_sum(s, lanes) / (float)p.HW;
+        q = lanes_sum(q, lanes) / ((float)p.HW * (float)cg) - s * s;
+        const float m = k + s, rstd = 1.0f / sqrtf(fmaxf(q, 0.f) + p.eps);
+        if (sub == 0) {
+            g_mean[g] = m;
+            g_rstd[g] = rstd;
+            if (p.mean && chunk == 0) {
+                p.mean[(long long)b * p.G + g] = m;
+                p.rstd[(long long)b * p.G + g] = rstd;
+            }
         }
     }
     __syncthreads();
@@ -223,17 +240,19 @@ __device__ __forceinline__ float dz_of(float dy, float z, int act) {
     return dy * (s * (1.0f + z * (1.0f - s)));
 }
 
-// ---- backward, launch 1: per channel the sums of dz and dz * xh over the rows of one chunk
+// ---- backward, launch 1: over the rows of one chunk, per channel the sums of dz and dz * xh, and from them per group those of gamma * dz, gamma * dz * xh
 template <typename T, int VEC> __global__ void __launch_bounds__(NT) k_gna_bwd_sums(NormArgs p) {
     extern __shared__ float lds[];
     const int C = p.C, cols = C / VEC, b = blockIdx.y, chunk = blockIdx.x, cg = C / p.G;
     const int pc = cols < NT ? cols : NT, R = NT / pc, width = pc * VEC;
-    float* s0 = lds;
-    float* s1 = lds + R * width;
+    float* ch0 = lds;                     // [C] gamma * sums
+    float* ch1 = lds + C;
+    float* s0 = lds + 2 * C;
+    float* s1 = s0 + R * width;
     const long long r0 = (long long)chunk * p.rows;
     const int n = (int)(p.HW - r0 < p.rows ? p.HW - r0 : p.rows);
     const int col = threadIdx.x % pc, rl = threadIdx.x / pc;
-    float* o = p.part + ((long long)b * p.nchunk + chunk) * 2 * C;
+    float* o = p.chan + ((long long)b * p.nchunk + chunk) * 2 * C;
     for (int c0 = 0; c0 < cols; c0 += pc) {
         const int c = c0 + col;
         if (rl < R && c < cols) {
@@ -271,62 +290,77 @@ template <typename T, int VEC> __global__ void __launch_bounds__(NT) k_gna_bwd_s
         fold_rows<VEC>(s0, s1, R, width);
         const int w = (cols - c0 < pc ? cols - c0 : pc) * VEC;
         for (int i = threadIdx.x; i < w; i += NT) {
+            const float gm = p.gamma[c0 * VEC + i];
             o[c0 * VEC + i] = s0[i];
             o[C + c0 * VEC + i] = s1[i];
+            ch0[c0 * VEC + i] = gm * s0[i];
+            ch1[c0 * VEC + i] = gm * s1[i];
         }
         __syncthreads();
     }
+    const int lanes = lanes_per(p.G), sub = threadIdx.x % lanes, stride = NT / lanes;
+    for (int g0 = 0; g0 < p.G; g0 += stride) {
+        const int g = min(g0 + (int)threadIdx.x / lanes, p.G - 1);
+        float a = 0.f, q = 0.f;
+        for (int c = sub; c < cg; c += lanes) {
+            a += ch0[g * cg + c];
+            q += ch1[g * cg + c];
+        }
+        a = lanes_sum(a, lanes);
+        q = lanes_sum(q, lanes);
+        if (sub == 0) *reinterpret_cast<f32x2*>(p.part + (((long long)b * p.nchunk + chunk) * p.G + g) * 2) = f32x2{a, q};
+    }
 }
 
-// ---- backward, launch 2: a block owns `gpb` groups of one sample; sums over the chunks, then the group means of gamma * dz, gamma * dz * xh
-__global__ void __launch_bounds__(NT) k_gna_bwd_merge(NormArgs p, int gpb) {
+// ---- backward, launch 2: the group means from the chunks' sums, then dx of one chunk.  The first p.tail blocks (they run longest)
+// sum dgamma and dbeta instead, 64 channels each: 64 lanes x 4 runs of the B * nchunk chunk sums, joined in order.
+template <typename T, int VEC> __global__ void __launch_bounds__(NT) k_gna_bwd_dx(NormArgs p, int tail) {
     extern __shared__ float lds[];
-    const int C = p.C, b = blockIdx.y, cg = C / p.G;
-    const int g0 = blockIdx.x * gpb, g1 = g0 + gpb < p.G ? g0 + gpb : p.G, c0 = g0 * cg, w = (g1 - g0) * cg;
-    float* s0 = lds;
-    float* s1 = lds + gpb * cg;
-    const float* o = p.part + (long long)b * p.nchunk * 2 * C;
-    for (int c = threadIdx.x; c < w; c += NT) {
+    const int C = p.C, cols = C / VEC, cg = C / p.G;
+    if ((int)blockIdx.x < tail) {
+        const int c = blockIdx.x * 64 + (threadIdx.x & 63), run = threadIdx.x >> 6;
+        const long long all = (long long)p.B * p.nchunk, per = (all + 3) / 4, i0 = run * per, i1 = i0 + per < all ? i0 + per : all;
         float a = 0.f, q = 0.f;
+        if (c < C) {
+            const float* o = p.chan + c;
 #pragma unroll 8
-        for (int i = 0; i < p.nchunk; ++i) {
-            a += o[(long long)i * 2 * C + c0 + c];
-            q += o[(long long)i * 2 * C + C + c0 + c];
-        }
-        p.chan[(long long)b * 2 * C + c0 + c] = a;
-        p.chan[(long long)b * 2 * C + C + c0 + c] = q;
-        s0[c] = a * p.gamma[c0 + c];
-        s1[c] = q * p.gamma[c0 + c];
-    }
-    __syncthreads();
-    const float inv = 1.0f / ((float)p.HW * (float)cg);
-    for (int g = threadIdx.x; g < g1 - g0; g += NT) {
-        float a = 0.f, q = 0.f;
-        for (int c = 0; c < cg; ++c) {
-            a += s0[g * cg + c];
-            q += s1[g * cg + c];
-        }
-        float* f = p.coef + ((long long)b * p.G + g0 + g) * 2;
-        f[0] = a * inv;
-        f[1] = q * inv;
-    }
-}
-
-// ---- backward, launch 3: dx of one chunk; the blocks behind the chunks (x = nchunk, y = b < ceil(C / NT)) sum dgamma / dbeta over the batch
-template <typename T, int VEC> __global__ void __launch_bounds__(NT) k_gna_bwd_dx(NormArgs p) {
-    const int C = p.C, cols = C / VEC, b = blockIdx.y, chunk = blockIdx.x, cg = C / p.G;
-    if (chunk == p.nchunk) {
-        for (int c = b * NT + threadIdx.x; c < C; c += gridDim.y * NT) {
-            float a = 0.f, q = 0.f;
-            for (int i = 0; i < p.B; ++i) {
-                a += p.chan[(long long)i * 2 * C + c];
-                q += p.chan[(long long)i * 2 * C + C + c];
+            for (long long i = i0; i < i1; ++i) {
+                a += o[i * 2 * C];
+                q += o[i * 2 * C + C];
             }
-            p.dbeta[c] = a;
-            p.dgamma[c] = q;
+        }
+        lds[threadIdx.x] = a;
+        lds[NT + threadIdx.x] = q;
+        __syncthreads();
+        if (run == 0 && c < C) {
+            p.dbeta[c] = (lds[threadIdx.x] + lds[64 + threadIdx.x]) + (lds[128 + threadIdx.x] + lds[192 + threadIdx.x]);
+            p.dgamma[c] = (lds[NT + threadIdx.x] + lds[NT + 64 + threadIdx.x]) + (lds[NT + 128 + threadIdx.x] + lds[NT + 192 + threadIdx.x]);
         }
         return;
     }
+    const int id = blockIdx.x - tail, chunk = id % p.nchunk, b = id / p.nchunk;
+    float* ga = lds;                      // [G]
+    float* gq = lds + p.G;
+    const int lanes = lanes_per(p.G), sub = threadIdx.x % lanes, stride = NT / lanes;
+    const float inv = 1.0f / ((float)p.HW * (float)cg);
+    for (int g0 = 0; g0 < p.G; g0 += stride) {
+        const int g = min(g0 + (int)threadIdx.x / lanes, p.G - 1);
+        const f32x2* o = reinterpret_cast<const f32x2*>(p.part) + (long long)b * p.nchunk * p.G + g;
+        float a = 0.f, q = 0.f;
+#pragma unroll 4
+        for (int i = sub; i < p.nchunk; i += lanes) {
+            const f32x2 t = o[(long long)i * p.G];
+            a += t[0];
+            q += t[1];
+        }
+        a = lanes_sum(a, lanes);
+        q = lanes_sum(q, lanes);
+        if (sub == 0) {
+            ga[g] = a * inv;
+            gq[g] = q * inv;
+        }
+    }
+    __syncthreads();
     const int pc = cols < NT ? cols : NT, R = NT / pc;
     const long long r0 = (long long)chunk * p.rows;
     const int n = (int)(p.HW - r0 < p.rows ? p.HW - r0 : p.rows);
@@ -342,8 +376,8 @@ template <typename T, int VEC> __global__ void __launch_bounds__(NT) k_gna_bwd_d
             rstd[e] = p.rstd[bg];
             gm[e] = p.gamma[ch];
             bt[e] = p.beta[ch];
-            ka[e] = p.coef[bg * 2];
-            kb[e] = p.coef[bg * 2 + 1];
+            ka[e] = ga[g];
+            kb[e] = gq[g];
         }
         const T* x = (const T*)p.x + b * p.x_b + r0 * p.x_row + (long long)c * VEC;
         const T* dy = (const T*)p.dy + b * p.dy_b + r0 * p.dy_row + (long long)c * VEC;
@@ -396,6 +430,17 @@ size_t fold_floats(int C, int VEC) {
     return (size_t)2 * R * pc * VEC;
 }
 
+// More than 64 KB of LDS has to be asked for; the widest maps (C = 8192) need 80 KB
+template <void (*K)(NormArgs)> int allow_lds() {
+    static VsOncePerDevice once;
+    if (once.needs()) {
+        hipError_t e = hipFuncSetAttribute((const void*)K, hipFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024);
+        if (e != hipSuccess) VS_FAIL(VS_ERR_HIP, "groupnorm_act: %s", hipGetErrorString(e));
+        once.mark();
+    }
+    return VS_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -416,14 +461,9 @@ int vidseg_groupnorm_act_fwd(const void* x, long long x_batch_stride, long long 
     const bool wide = C % vec == 0 && aligned16(x, x_batch_stride, x_row_stride, es) && aligned16(y, 0, 0, es);
     const dim3 grid(p.nchunk, B);
     const size_t l1 = (2 * (size_t)C + fold_floats(C, wide ? vec : 1)) * 4, l2 = 2 * (size_t)G * 4;
-#define CALL(T, V)                                                   \
-    static VsOncePerDevice once;                                     \
-    if (once.needs()) {                                              \
-        hipError_t e = hipFuncSetAttribute((const void*)k_gna_stats<T, V>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024); \
-        if (e != hipSuccess) VS_FAIL(VS_ERR_HIP, "groupnorm_act: %s", hipGetErrorString(e)); \
-        once.mark();                                                 \
-    }                                                                \
-    hipLaunchKernelGGL((k_gna_stats<T, V>), grid, dim3(NT), l1, s, p); \
+#define CALL(T, V)                                                       \
+    if (int rc2 = allow_lds<k_gna_stats<T, V>>()) return rc2; \
+    hipLaunchKernelGGL((k_gna_stats<T, V>), grid, dim3(NT), l1, s, p);   \
     hipLaunchKernelGGL((k_gna_apply<T, V>), grid, dim3(NT), l2, s, p)
     GNA_DISPATCH(dtype, wide, CALL);
 #undef CALL
@@ -445,21 +485,20 @@ int vidseg_groupnorm_act_bwd(const void* dy, long long dy_batch_stride, long lon
     p.nchunk = (int)((HW + rows_per_chunk - 1) / rows_per_chunk);
     p.act = act; p.gamma = gamma; p.beta = beta; p.out = dx; p.mean = const_cast<float*>(mean); p.rstd = const_cast<float*>(rstd);
     p.part = scratch;
-    p.chan = scratch + (long long)B * p.nchunk * 2 * C;
-    p.coef = p.chan + (long long)B * 2 * C;
+    p.chan = scratch + 2ll * B * p.nchunk * G;
     p.dgamma = dgamma; p.dbeta = dbeta;
-    const long long need = (long long)B * ((long long)(p.nchunk + 1) * 2 * C + 2 * G);
+    const long long need = 2ll * B * p.nchunk * ((long long)C + G), tail = (C + 63) / 64;
     VS_REQUIRE(need <= scratch_floats, "groupnorm_act_bwd: scratch of %lld floats, needs %lld", scratch_floats, need);
     const int es = dtype == 0 ? 4 : 2, vec = 16 / es;
     const bool wide = C % vec == 0 && aligned16(x, x_batch_stride, x_row_stride, es) && aligned16(dy, dy_batch_stride, dy_row_stride, es) &&
                       aligned16(dx, 0, 0, es);
-    const dim3 grid(p.nchunk, B), grid3(p.nchunk + 1, B);
-    const size_t l1 = fold_floats(C, wide ? vec : 1) * 4;
-    const int cg = C / G, gpb = cg >= NT ? 1 : (NT / cg < G ? NT / cg : G);       // about one channel per thread
+    VS_REQUIRE((long long)p.nchunk * B + tail < (1ll << 24), "groupnorm_act_bwd: B=%d HW=%lld are too many chunks of %d rows", B, HW, rows_per_chunk);
+    const dim3 grid(p.nchunk, B), grid2((unsigned)(p.nchunk * (long long)B + tail));
+    const size_t l1 = (2 * (size_t)C + fold_floats(C, wide ? vec : 1)) * 4, l2 = (size_t)(2 * G > 2 * NT ? 2 * G : 2 * NT) * 4;
 #define CALL(T, V)                                                        \
+    if (int rc2 = allow_lds<k_gna_bwd_sums<T, V>>()) return rc2; \
     hipLaunchKernelGGL((k_gna_bwd_sums<T, V>), grid, dim3(NT), l1, s, p); \
-    hipLaunchKernelGGL(k_gna_bwd_merge, dim3((G + gpb - 1) / gpb, B), dim3(NT), 2 * (size_t)gpb * cg * 4, s, p, gpb); \
-    hipLaunchKernelGGL((k_gna_bwd_dx<T, V>), grid3, dim3(NT), 0, s, p)
+    hipLaunchKernelGGL((k_gna_bwd_dx<T, V>), grid2, dim3(NT), l2, s, p, (int)tail)
     GNA_DISPATCH(dtype, wide, CALL);
 #undef CALL
     VS_CHECK_LAUNCH("groupnorm_act_bwd");
