@@ -71,15 +71,20 @@ struct AttnArgs {
     long long mask_b;
     u16* o;                    // [B][Nq][H][d]
     float* lse;                // [B][H][Nq] or null
-    float *po, *pml;           // partial results: [split][B * Nq * H][d], [..][2] = (maximum in log2 units, sum)
+    float *po, *pml;           // partial results: [part][B * Nq * H][d], [..][2] = (maximum in log2 units, sum)
     int B, Nq, Np, Nk, H, Hk, G, d, causal;
     float c;                   // scale * log2 e
-    int splits, per_split, split0;     // key tiles are dealt out in runs of per_split; the partial results start at index split0
-    int xtiles;                // row tiles of a key head
-    int stacked;               // rows run over (sample, query, head of the group) and see the prefix only
+};
+// A share of a launch's blocks: row tiles x runs of key tiles x key heads (x samples).  A call has up to two of them.
+struct Deal {
+    int blocks, xtiles;        // row tiles of a key head
+    int splits, per_split;     // key tiles are dealt out in runs of per_split
+    int part0;                 // index of its first partial result
+    int stacked;               // rows run over (sample, query, head of the group) and see the prefix alone; else the rows of one sample
+    int np;                    // prefix keys that it visits
 };
 
-// One row (query, head) per accumulator column.  rows of a key head: r = (sample, query, head of its group), heads fastest.
+// One row (query, head) per accumulator column.  Rows of a key head: r = (sample, query, head of its group), heads fastest.
 struct Row {
     int b, qi, h;
     bool on;
@@ -89,7 +94,7 @@ __device__ __forceinline__ Row row_of(const AttnArgs& p, int b, int hk, long lon
     x.on = r < rows;
     if (!x.on) r = rows - 1;
     const int per = p.Nq * p.G;
-    const int bb = p.stacked ? (int)(r / per) : 0, rem = (int)(r - (long long)bb * per);
+    const int bb = (int)(r / per), rem = (int)(r - (long long)bb * per);
     x.b = b + bb;
     x.qi = rem / p.G;
     x.h = hk * p.G + rem % p.G;
@@ -98,264 +103,474 @@ __device__ __forceinline__ Row row_of(const AttnArgs& p, int b, int hk, long lon
 
 // Blocks reach the 8 XCDs round-robin by their index: every XCD gets one contiguous run of the (key head, split, row tile) space, so the row
 // tiles that read the same keys share them through one L2.
+__device__ __forceinline__ unsigned swizzled(unsigned i, unsigned tot) {
+    const unsigned q = tot / 8, r = tot % 8, xcd = i % 8;
+    return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + i / 8;
+}
 __device__ __forceinline__ void block_of(int xtiles, int& y, int& xt) {
-    const unsigned tot = gridDim.x, q = tot / 8, r = tot % 8, xcd = blockIdx.x % 8, idx = blockIdx.x / 8;
-    const unsigned id = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + idx;
+    const unsigned id = swizzled(blockIdx.x, gridDim.x);
     y = (int)(id / xtiles);
     xt = (int)(id % xtiles);
 }
+struct Place {
+    int b, hk, split, xt, len;         // len: own keys
+    long long rows;
+};
+__device__ __forceinline__ Place place_of(const AttnArgs& p, const Deal& w, unsigned i) {
+    Place x;
+    const unsigned id = swizzled(i, w.blocks);
+    x.xt = id % w.xtiles;
+    unsigned y = id / w.xtiles;
+    x.split = y % w.splits;
+    y /= w.splits;
+    x.hk = y % p.Hk;
+    x.b = y / p.Hk;
+    x.rows = (long long)(w.stacked ? p.B : 1) * p.Nq * p.G;
+    x.len = w.stacked ? 0 : (p.lens ? max(0, min(p.lens[x.b], p.Nk)) : p.Nk);
+    return x;
+}
 
-// WS false: the block's four waves own 32 QB rows each and share key tiles of 64.  WS true (at most 32 rows): every wave holds the same rows
-// and takes 32 of each 128 keys; the four partial results are merged at the end.
-template <bool BF, int DP, int QB, bool WS> __global__ void __launch_bounds__(256, (DP == 64 || (QB == 1 && !WS)) ? 2 : 1) k_ctx_attn(AttnArgs p) {
-    constexpr int KT = WS ? 128 : 64, SL = DP / 8, NST = KT * SL / 256, NBUF = WS ? 1 : 2, NJ = WS ? 1 : 2, ND = DP / 32;
-    __shared__ __attribute__((aligned(16))) u16 sK[NBUF][KT * DP], sV[NBUF][KT * DP];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, hi = lane >> 5;
-    int y, xt;
-    block_of(p.xtiles, y, xt);
-    const int split = y % p.splits;
-    y /= p.splits;
-    const int hk = y % p.Hk, b = y / p.Hk;                            // stacked: b = 0
-    const long long rows = (long long)(p.stacked ? p.B : 1) * p.Nq * p.G;
-    const long long r0 = (long long)xt * (WS ? 32 : 128 * QB);
-    Row row[QB];
-    u32x4 fq[QB][DP / 16];
+// Q^T of one row as B operands: lane (l31, hi) holds d = 16 s + 8 hi + 0..7 of its row
+template <int DP> __device__ __forceinline__ void load_q(const AttnArgs& p, const Row& x, int hi, u32x4 (&f)[DP / 16]) {
+    const u16* qp = p.q + x.b * p.q_b + x.qi * p.q_n + x.h * p.q_h;
 #pragma unroll
-    for (int i = 0; i < QB; ++i) {
-        row[i] = row_of(p, b, hk, r0 + (WS ? 0 : wave * 32 * QB) + i * 32 + l31, rows);
-        const u16* qp = p.q + row[i].b * p.q_b + row[i].qi * p.q_n + row[i].h * p.q_h;
-#pragma unroll
-        for (int s = 0; s < DP / 16; ++s) {
-            const int at = s * 16 + hi * 8;
-            fq[i][s] = *reinterpret_cast<const u32x4*>(qp + (at < p.d ? at : 0));
-            if (at >= p.d) fq[i][s] = u32x4{0u, 0u, 0u, 0u};
-        }
+    for (int s = 0; s < DP / 16; ++s) {
+        const int at = s * 16 + hi * 8;
+        f[s] = *reinterpret_cast<const u32x4*>(qp + (at < p.d ? at : 0));
+        if (at >= p.d) f[s] = u32x4{0u, 0u, 0u, 0u};
     }
-    // the key tiles this block visits: prefix tiles first, then the sample's own
-    const int len = p.stacked ? 0 : (p.lens ? max(0, min(p.lens[b], p.Nk)) : p.Nk);
-    const long long last_r = (r0 + (WS ? 32 : 128 * QB) < rows ? r0 + (WS ? 32 : 128 * QB) : rows) - 1;
-    const int seen = p.causal ? max(0, min(len, len - p.Nq + 1 + (int)(last_r / p.G))) : len;      // own keys that the block's last row sees
-    const int all_see = p.causal ? len - p.Nq + 1 + (int)(r0 / p.G) : len;                          // own keys that every row sees
-    const int np = p.Np;
-    const int T0 = (np + KT - 1) / KT, T1 = (seen + KT - 1) / KT;
-    const int tb = min(split * p.per_split, T0 + T1), te = p.splits == 1 ? T0 + T1 : min(tb + p.per_split, T0 + T1);
+}
+
+// 32 columns n * 32 .. of one row out of its accumulator, times f, as 16-byte pieces: the lane halves hold the rows 4 hi .. of every
+// 8 channels, one exchange of two registers gives each half 8 neighbouring channels.  All lanes call it.
+template <bool BF> __device__ __forceinline__ void store_row(u16* row, const f32x16& a, float f, int n, int hi, int d, bool on) {
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+        const auto x = __builtin_amdgcn_permlane32_swap(pack2<BF>(a[8 * g] * f, a[8 * g + 1] * f), pack2<BF>(a[8 * g + 4] * f, a[8 * g + 5] * f), false, false);
+        const auto y = __builtin_amdgcn_permlane32_swap(pack2<BF>(a[8 * g + 2] * f, a[8 * g + 3] * f), pack2<BF>(a[8 * g + 6] * f, a[8 * g + 7] * f), false, false);
+        const int c = n * 32 + 16 * g + 8 * hi;
+        if (on && c < d) *reinterpret_cast<u32x4*>(row + c) = u32x4{x[0], y[0], x[1], y[1]};
+    }
+}
+
+// One step of the running softmax on NJ blocks of 32 scores: probabilities as B operands; m in log2 units, acc and l rescaled where it moved
+template <bool BF, int NJ, int ND> __device__ __forceinline__ void soften(const f32x16 (&s)[NJ], float c, float& m, float& l, f32x16 (&acc)[ND], u32x4 (&fp)[NJ][2]) {
+    float mx = s[0][0];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[j][r]);
+    const float m_new = fmaxf(m, half_max(mx) * c);
+    const float ref = m_new == -INFINITY ? 0.f : m_new;               // a row without a key so far: every exp2 below gives 0
+    if (__any(m_new > m)) {
+        const float alpha = __builtin_amdgcn_exp2f(m - ref);
+        l *= alpha;
+#pragma unroll
+        for (int n = 0; n < ND; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[n][r] *= alpha;
+        m = m_new;
+    }
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[j][r], c, -ref)), p1 = __builtin_amdgcn_exp2f(fmaf(s[j][r + 1], c, -ref));
+            sum += p0 + p1;
+            fp[j][r >> 3][(r >> 1) & 3] = pack2<BF>(p0, p1);          // p in (0, 1]: the one rounding of the probabilities
+        }
+    l += half_sum(sum);
+}
+
+// -inf into the scores of keys that do not exist (bits) or lie behind lim (in this lane's numbering)
+__device__ __forceinline__ void hide(f32x16& s, unsigned bits, int lim, int hi) {
+    bits >>= 4 * hi;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const int at = (r & 3) + 8 * (r >> 2);
+        if (!((bits >> at) & 1u) || at > lim) s[r] = -INFINITY;
+    }
+}
+
+// Many rows: the block's four waves own 32 rows each and share key tiles of 64 in LDS, staged through registers one tile ahead.
+template <bool BF, int DP> __device__ __forceinline__ void many_rows(const AttnArgs& p, const Deal& w, unsigned block, u16* lds) {
+    constexpr int KT = 64, SL = DP / 8, NST = KT * SL / 256, ND = DP / 32, TILE = KT * DP;
+    u16 *sK = lds, *sV = lds + 2 * TILE;                              // two buffers each
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, hi = lane >> 5;
+    const Place at = place_of(p, w, block);
+    const long long r0 = (long long)at.xt * 128;
+    const Row row = row_of(p, at.b, at.hk, r0 + wave * 32 + l31, at.rows);
+    u32x4 fq[DP / 16];
+    load_q<DP>(p, row, hi, fq);
+    const long long last_r = (r0 + 128 < at.rows ? r0 + 128 : at.rows) - 1;
+    const int seen = p.causal ? max(0, min(at.len, at.len - p.Nq + 1 + (int)(last_r / p.G))) : at.len;      // own keys that the block's last row sees
+    const int all_see = p.causal ? at.len - p.Nq + 1 + (int)(r0 / p.G) : at.len;                             // own keys that every row sees
+    const int T0 = (w.np + KT - 1) / KT, T1 = (seen + KT - 1) / KT;
+    const int tb = min(at.split * w.per_split, T0 + T1), te = w.splits == 1 ? T0 + T1 : min(tb + w.per_split, T0 + T1);
 
     u32x4 rk[NST], rv[NST];
-    unsigned long long live = 0;                                      // keys of the staged tile that exist (WS: of this wave's 32)
-    const u16* kown = p.k + b * p.k_b + hk * p.k_h;
-    const u16* vown = p.v + b * p.v_b + hk * p.v_h;
-    const unsigned char* mrow = p.mask ? p.mask + b * p.mask_b : nullptr;
+    unsigned long long live = 0;                                      // keys of the staged tile that exist
+    const u16 *kown = p.k + at.b * p.k_b + at.hk * p.k_h, *vown = p.v + at.b * p.v_b + at.hk * p.v_h;
+    const unsigned char* mrow = p.mask ? p.mask + at.b * p.mask_b : nullptr;
     auto load_tile = [&](int t) {
         const bool own = t >= T0;
-        const int k0 = (own ? t - T0 : t) * KT, n = own ? seen : np;
-        const u16* kb = own ? kown : p.kp + hk * p.kp_h;
-        const u16* vb = own ? vown : p.vp + hk * p.vp_h;
+        const int k0 = (own ? t - T0 : t) * KT, n = own ? seen : w.np;
+        const u16 *kb = own ? kown : p.kp + at.hk * p.kp_h, *vb = own ? vown : p.vp + at.hk * p.vp_h;
         const long long kn = own ? p.k_n : p.kp_n, vn = own ? p.v_n : p.vp_n;
         const unsigned char* mk = own ? mrow : nullptr;
 #pragma unroll
         for (int i = 0; i < NST; ++i) {
             const int id = tid + 256 * i, r = id / SL, slot = id % SL, key = k0 + r, kk = min(key, n - 1);
             const bool ok = key < n && slot * 8 < p.d && (!mk || mk[kk]);
-            const int at = slot * 8 < p.d ? slot * 8 : 0;
-            rk[i] = *reinterpret_cast<const u32x4*>(kb + kk * kn + at);
-            rv[i] = *reinterpret_cast<const u32x4*>(vb + kk * vn + at);
+            const int c = slot * 8 < p.d ? slot * 8 : 0;
+            rk[i] = *reinterpret_cast<const u32x4*>(kb + kk * kn + c);
+            rv[i] = *reinterpret_cast<const u32x4*>(vb + kk * vn + c);
             if (!ok) rk[i] = rv[i] = u32x4{0u, 0u, 0u, 0u};
         }
-        const int key = k0 + (WS ? wave * 32 + l31 : lane);
+        const int key = k0 + lane;
         live = __ballot(key < n && (!mk || mk[min(key, n - 1)]));
     };
     auto store_tile = [&](int buf) {
 #pragma unroll
         for (int i = 0; i < NST; ++i) {
             const int id = tid + 256 * i, r = id / SL, slot = id % SL;
-            *reinterpret_cast<u32x4*>(&sK[buf][slot_at<DP>(r, slot)]) = rk[i];
-            *reinterpret_cast<u32x4*>(&sV[buf][slot_at<DP>(r, slot)]) = rv[i];
+            *reinterpret_cast<u32x4*>(sK + buf * TILE + slot_at<DP>(r, slot)) = rk[i];
+            *reinterpret_cast<u32x4*>(sV + buf * TILE + slot_at<DP>(r, slot)) = rv[i];
         }
     };
-
-    f32x16 oacc[QB][ND];
-    float m_run[QB], l_run[QB];
+    f32x16 acc[ND];
+    float m = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int i = 0; i < QB; ++i) {
-        m_run[i] = -INFINITY;
-        l_run[i] = 0.f;
+    for (int n = 0; n < ND; ++n)
 #pragma unroll
-        for (int n = 0; n < ND; ++n)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) oacc[i][n][r] = 0.f;
-    }
-
+        for (int r = 0; r < 16; ++r) acc[n][r] = 0.f;
     if (tb < te) {
         load_tile(tb);
         store_tile(0);
     }
     __syncthreads();
     for (int t = tb; t < te; ++t) {
-        const int buf = NBUF == 2 ? (t - tb) & 1 : 0;
+        const int buf = (t - tb) & 1;
+        const u16 *tk = sK + buf * TILE, *tv = sV + buf * TILE;
         const unsigned long long now = live;
         if (t + 1 < te) load_tile(t + 1);
-        const int k0 = (t >= T0 ? t - T0 : t) * KT + (WS ? wave * 32 : 0);
-        const bool edge = p.causal && t >= T0 && k0 + 32 * NJ > all_see;
+        const int k0 = (t >= T0 ? t - T0 : t) * KT;
+        const bool edge = p.causal && t >= T0 && k0 + KT > all_see;
+        f32x16 s[2];
 #pragma unroll
-        for (int i = 0; i < QB; ++i) {
-            f32x16 s[NJ];
+        for (int j = 0; j < 2; ++j) {
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) {
+            for (int r = 0; r < 16; ++r) s[j][r] = 0.f;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[j][r] = 0.f;
-#pragma unroll
-                for (int e = 0; e < DP / 16; ++e)
-                    s[j] = mfma<BF>(read_row<DP>(sK[buf], (WS ? wave * 32 : j * 32) + l31, e * 2 + hi), fq[i][e], s[j]);
-            }
-            if (now != ~0ull || edge) {
-                const int lim = edge ? len - p.Nq + row[i].qi - k0 - 4 * hi : 1 << 30;              // keys up to this one (in this lane's numbering) are seen
-#pragma unroll
-                for (int j = 0; j < NJ; ++j) {
-                    const unsigned bits = (unsigned)(now >> (32 * j)) >> (4 * hi);
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int at = (r & 3) + 8 * (r >> 2);
-                        if (!((bits >> at) & 1u) || 32 * j + at > lim) s[j][r] = -INFINITY;
-                    }
-                }
-            }
-            float mx = s[0][0];
-#pragma unroll
-            for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[j][r]);
-            mx = half_max(mx) * p.c;
-            const float m_new = fmaxf(m_run[i], mx);
-            const float ref = m_new == -INFINITY ? 0.f : m_new;       // a row without a key so far: every exp2 below gives 0
-            if (__any(m_new > m_run[i])) {
-                const float alpha = __builtin_amdgcn_exp2f(m_run[i] - ref);
-                l_run[i] *= alpha;
-#pragma unroll
-                for (int n = 0; n < ND; ++n)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) oacc[i][n][r] *= alpha;
-                m_run[i] = m_new;
-            }
-            float sum = 0.f;
-            u32x4 fp[NJ][2];
-#pragma unroll
-            for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                for (int r = 0; r < 16; r += 2) {
-                    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[j][r], p.c, -ref)), p1 = __builtin_amdgcn_exp2f(fmaf(s[j][r + 1], p.c, -ref));
-                    sum += p0 + p1;
-                    fp[j][r >> 3][(r >> 1) & 3] = pack2<BF>(p0, p1);          // p in (0, 1]: the one rounding of the probabilities
-                }
-            l_run[i] += half_sum(sum);
-#pragma unroll
-            for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-#pragma unroll
-                    for (int n = 0; n < ND; ++n)
-                        oacc[i][n] = mfma<BF>(read_tr<DP>(sV[buf], (WS ? wave * 32 : j * 32) + e * 16, n * 32, lane), fp[j][e], oacc[i][n]);
+            for (int e = 0; e < DP / 16; ++e) s[j] = mfma<BF>(read_row<DP>(tk, j * 32 + l31, e * 2 + hi), fq[e], s[j]);
         }
-        if (NBUF == 1) __syncthreads();
-        if (t + 1 < te) store_tile(NBUF == 2 ? buf ^ 1 : 0);
+        if (now != ~0ull || edge) {
+            const int lim = edge ? at.len - p.Nq + row.qi - k0 - 4 * hi : 1 << 30;
+            hide(s[0], (unsigned)now, lim, hi);
+            hide(s[1], (unsigned)(now >> 32), lim - 32, hi);
+        }
+        u32x4 fp[2][2];
+        soften<BF, 2, ND>(s, p.c, m, l, acc, fp);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int n = 0; n < ND; ++n) acc[n] = mfma<BF>(read_tr<DP>(tv, j * 32 + e * 16, n * 32, lane), fp[j][e], acc[n]);
+        if (t + 1 < te) store_tile(buf ^ 1);
         __syncthreads();
     }
-
-    const long long total = (long long)p.B * p.Nq * p.H;
-    if constexpr (WS) {
-        // the four waves' results of the same rows: maxima and sums first, then the accumulators through the tile memory (fp32 [wave][row][DP])
-        __shared__ float sm[4][32], sl[4][32];
-        static_assert(4 * 32 * DP * 4 <= (int)sizeof(sK) + (int)sizeof(sV), "merge buffer");
-        float* so = reinterpret_cast<float*>(&sK[0][0]);
-        float* so2 = reinterpret_cast<float*>(&sV[0][0]);             // waves 0, 1 use sK, waves 2, 3 use sV
-        float* mine = (wave < 2 ? so : so2) + (wave & 1) * 32 * DP;
-        if (hi == 0) {
-            sm[wave][l31] = m_run[0];
-            sl[wave][l31] = l_run[0];
+    const long long total = (long long)p.B * p.Nq * p.H, id = ((long long)row.b * p.Nq + row.qi) * p.H + row.h, part = w.part0 + at.split;
+    const float inv = l > 0.f ? 1.0f / l : 0.f;
+#pragma unroll
+    for (int n = 0; n < ND; ++n) {
+        if (!p.po) {
+            store_row<BF>(p.o + id * p.d, acc[n], inv, n, hi, p.d, row.on);
+        } else if (row.on) {
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const int c = n * 32 + 2 * r + 4 * hi;
+                if (c < p.d) *reinterpret_cast<f32x4*>(p.po + (part * total + id) * p.d + c) = f32x4{acc[n][r], acc[n][r + 1], acc[n][r + 2], acc[n][r + 3]};
+            }
         }
+    }
+    if (hi == 0 && row.on) {
+        if (p.po) *reinterpret_cast<f32x2*>(p.pml + (part * total + id) * 2) = f32x2{m, l};
+        else if (p.lse) p.lse[((long long)row.b * p.H + row.h) * p.Nq + row.qi] = (m + __builtin_amdgcn_logf(l)) * LN2;
+    }
+}
+
+// Few rows (at most 32 per key head): the keys are what has to be read, so every wave walks over its own runs of 32 of them with all rows as
+// columns, no barrier in the loop.  K goes from memory straight into A operands (a lane reads its key's row); V passes through a piece of LDS
+// that only this wave uses, for the transpose.  The next 32 keys are in flight while these are worked on; the four waves' results are merged at the end.
+template <bool BF, int DP> __device__ __forceinline__ void few_rows(const AttnArgs& p, const Deal& w, unsigned block, u16* lds) {
+    constexpr int SL = DP / 8, NV = 32 * SL / 64, ND = DP / 32;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, hi = lane >> 5;
+    u16* sV = lds + wave * 32 * DP;
+    const Place at = place_of(p, w, block);
+    const int rows = (int)at.rows;
+    const Row row = row_of(p, at.b, at.hk, l31, rows);
+    u32x4 fq[DP / 16];
+    load_q<DP>(p, row, hi, fq);
+    const int len = at.len;                                           // causal: the last row sees all of them
+    const int T0 = (w.np + 127) / 128, T1 = (len + 127) / 128;
+    const int tb = min(at.split * w.per_split, T0 + T1), te = w.splits == 1 ? T0 + T1 : min(tb + w.per_split, T0 + T1);
+    u32x4 rk[DP / 16], rv[NV];
+    const u16 *kown = p.k + at.b * p.k_b + at.hk * p.k_h, *vown = p.v + at.b * p.v_b + at.hk * p.v_h;
+    const unsigned char* mrow = p.mask ? p.mask + at.b * p.mask_b : nullptr;
+    // the tile's first key, number of keys in its segment and this lane's key; a tile's last runs may lie behind the segment
+    auto first = [&](int t) { return (t >= T0 ? t - T0 : t) * 128 + wave * 32; };
+    auto load_k = [&](int t) {
+        const bool own = t >= T0;
+        const int n = own ? len : w.np, kk = min(first(t) + l31, n - 1);
+        const u16* kb = (own ? kown : p.kp + at.hk * p.kp_h) + kk * (own ? p.k_n : p.kp_n);
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) {
+            const int c = s * 16 + hi * 8;
+            rk[s] = *reinterpret_cast<const u32x4*>(kb + (c < p.d ? c : 0));
+        }
+    };
+    auto load_v = [&](int t) {
+        const bool own = t >= T0;
+        const int n = own ? len : w.np, k0 = first(t);
+        const u16* vb = own ? vown : p.vp + at.hk * p.vp_h;
+        const long long vn = own ? p.v_n : p.vp_n;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int id = lane + 64 * i, c = id % SL * 8;
+            rv[i] = *reinterpret_cast<const u32x4*>(vb + min(k0 + id / SL, n - 1) * vn + (c < p.d ? c : 0));
+        }
+    };
+    auto exists = [&](int t) -> unsigned {
+        const bool own = t >= T0;
+        const int n = own ? len : w.np, key = first(t) + l31;
+        return (unsigned)__ballot(key < n && (!own || !mrow || mrow[min(key, n - 1)]));
+    };
+    f32x16 acc[ND];
+    float m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int n = 0; n < ND; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[n][r] = 0.f;
+    unsigned bits = 0;
+    if (tb < te) {
+        load_k(tb);
+        load_v(tb);
+        bits = exists(tb);
+    }
+    for (int t = tb; t < te; ++t) {
+        const unsigned now = bits;
+        const bool more = t + 1 < te;
+        if (more) bits = exists(t + 1);
+        // K of keys that do not exist and channels behind d are zero
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s)
+            if (s * 16 + hi * 8 >= p.d || !((now >> l31) & 1u)) rk[s] = u32x4{0u, 0u, 0u, 0u};
+        f32x16 s[1];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
+#pragma unroll
+        for (int e = 0; e < DP / 16; ++e) s[0] = mfma<BF>(rk[e], fq[e], s[0]);
+        if (more) load_k(t + 1);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int id = lane + 64 * i, r = id / SL, slot = id % SL;
+            if (slot * 8 >= p.d || !((now >> r) & 1u)) rv[i] = u32x4{0u, 0u, 0u, 0u};
+            *reinterpret_cast<u32x4*>(sV + slot_at<DP>(r, slot)) = rv[i];
+        }
+        if (more) load_v(t + 1);
+        const int k0 = first(t);
+        const bool edge = p.causal && t >= T0 && k0 + 32 > len - p.Nq + 1;
+        if (now != ~0u || edge) hide(s[0], now, edge ? len - p.Nq + row.qi - k0 - 4 * hi : 1 << 30, hi);
+        u32x4 fp[1][2];
+        soften<BF, 1, ND>(s, p.c, m, l, acc, fp);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");        // the other lanes' V rows are in place (a wave's LDS operations keep their order)
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int n = 0; n < ND; ++n) acc[n] = mfma<BF>(read_tr<DP>(sV, e * 16, n * 32, lane), fp[0][e], acc[n]);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");        // ... and read before the next ones replace them
+        __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+    // maxima and sums first, then the accumulators, fp32 [wave][row][DP + 4]; rows that do not exist are left out
+    float* sm = reinterpret_cast<float*>(lds);                        // [4][32] maxima, [4][32] sums
+    float* so = sm + 256;
+    constexpr int LD = DP + 4;
+    if (hi == 0) {
+        sm[wave * 32 + l31] = m;
+        sm[128 + wave * 32 + l31] = l;
+    }
+    if (l31 < rows)
 #pragma unroll
         for (int n = 0; n < ND; ++n)
 #pragma unroll
             for (int r = 0; r < 16; r += 4)
-                *reinterpret_cast<f32x4*>(mine + l31 * DP + n * 32 + 2 * r + 4 * hi) = f32x4{oacc[0][n][r], oacc[0][n][r + 1], oacc[0][n][r + 2], oacc[0][n][r + 3]};
-        __syncthreads();
-        const int rr = tid >> 3;
-        const Row x = row_of(p, b, hk, r0 + rr, rows);
-        if (x.on) {
-            float m = -INFINITY, l = 0.f, w[4];
+                *reinterpret_cast<f32x4*>(so + (wave * 32 + l31) * LD + n * 32 + 2 * r + 4 * hi) = f32x4{acc[n][r], acc[n][r + 1], acc[n][r + 2], acc[n][r + 3]};
+    __syncthreads();
+    const long long total = (long long)p.B * p.Nq * p.H, part = w.part0 + at.split;
+    const int rr = tid >> 3;
+    const Row x = row_of(p, at.b, at.hk, rr, rows);
+    if (!x.on) return;
+    float mm = -INFINITY, ll = 0.f, f[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) m = fmaxf(m, sm[i][rr]);
+    for (int i = 0; i < 4; ++i) mm = fmaxf(mm, sm[i * 32 + rr]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                w[i] = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm[i][rr] - m);
-                l += w[i] * sl[i][rr];
-            }
-            const long long id = ((long long)x.b * p.Nq + x.qi) * p.H + x.h;
-            const float inv = l > 0.f ? 1.0f / l : 0.f;
-            for (int c = (tid & 7) * 4; c < p.d; c += 32) {
-                f32x4 a = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < 4; ++i) {
+        f[i] = mm == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm[i * 32 + rr] - mm);
+        ll += f[i] * sm[128 + i * 32 + rr];
+    }
+    const long long id = ((long long)x.b * p.Nq + x.qi) * p.H + x.h;
+    const float inv = ll > 0.f ? 1.0f / ll : 0.f;
+    for (int c = (tid & 7) * 4; c < p.d; c += 32) {
+        f32x4 a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const f32x4 t = *reinterpret_cast<const f32x4*>((i < 2 ? so : so2) + (i & 1) * 32 * DP + rr * DP + c);
+        for (int i = 0; i < 4; ++i) {
+            const f32x4 t = *reinterpret_cast<const f32x4*>(so + (i * 32 + rr) * LD + c);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) a[e] += w[i] * t[e];
-                }
-                if (p.po) *reinterpret_cast<f32x4*>(p.po + ((p.split0 + split) * total + id) * p.d + c) = a;
-                else *reinterpret_cast<u32x2*>(p.o + id * p.d + c) = u32x2{pack2<BF>(a[0] * inv, a[1] * inv), pack2<BF>(a[2] * inv, a[3] * inv)};
-            }
-            if ((tid & 7) == 0) {
-                if (p.po) *reinterpret_cast<f32x2*>(p.pml + ((p.split0 + split) * total + id) * 2) = f32x2{m, l};
-                else if (p.lse) p.lse[((long long)x.b * p.H + x.h) * p.Nq + x.qi] = (m + __builtin_amdgcn_logf(l)) * LN2;
-            }
+            for (int e = 0; e < 4; ++e) a[e] += f[i] * t[e];
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < QB; ++i) {
-            if (!row[i].on) continue;
-            const long long id = ((long long)row[i].b * p.Nq + row[i].qi) * p.H + row[i].h;
-            const float inv = l_run[i] > 0.f ? 1.0f / l_run[i] : 0.f;
-#pragma unroll
-            for (int n = 0; n < ND; ++n)
-#pragma unroll
-                for (int r = 0; r < 16; r += 4) {
-                    const int c = n * 32 + 2 * r + 4 * hi;
-                    if (c >= p.d) continue;
-                    if (p.po)
-                        *reinterpret_cast<f32x4*>(p.po + ((p.split0 + split) * total + id) * p.d + c) = f32x4{oacc[i][n][r], oacc[i][n][r + 1], oacc[i][n][r + 2], oacc[i][n][r + 3]};
-                    else
-                        *reinterpret_cast<u32x2*>(p.o + id * p.d + c) = u32x2{pack2<BF>(oacc[i][n][r] * inv, oacc[i][n][r + 1] * inv), pack2<BF>(oacc[i][n][r + 2] * inv, oacc[i][n][r + 3] * inv)};
-                }
-            if (hi == 0) {
-                if (p.po) *reinterpret_cast<f32x2*>(p.pml + ((p.split0 + split) * total + id) * 2) = f32x2{m_run[i], l_run[i]};
-                else if (p.lse) p.lse[((long long)row[i].b * p.H + row[i].h) * p.Nq + row[i].qi] = (m_run[i] + __builtin_amdgcn_logf(l_run[i])) * LN2;
-            }
-        }
+        if (p.po) *reinterpret_cast<f32x4*>(p.po + (part * total + id) * p.d + c) = a;
+        else *reinterpret_cast<u32x2*>(p.o + id * p.d + c) = u32x2{pack2<BF>(a[0] * inv, a[1] * inv), pack2<BF>(a[2] * inv, a[3] * inv)};
+    }
+    if ((tid & 7) == 0) {
+        if (p.po) *reinterpret_cast<f32x2*>(p.pml + (part * total + id) * 2) = f32x2{mm, ll};
+        else if (p.lse) p.lse[((long long)x.b * p.H + x.h) * p.Nq + x.qi] = (mm + __builtin_amdgcn_logf(ll)) * LN2;
     }
 }
 
-// Joins the partial results of one row: sixteen lanes per row, eight channels each
-template <bool BF> __global__ void __launch_bounds__(256) k_ctx_join(const float* __restrict__ po, const float* __restrict__ pml, int splits, long long total, int d,
-                                                                   int Nq, int H, u16* __restrict__ o, float* __restrict__ lse) {
-    const long long id = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
-    const int c = (threadIdx.x & 15) * 8;
-    if (id >= total) return;
-    float m = -INFINITY, l = 0.f;
-    for (int s = 0; s < splits; ++s) m = fmaxf(m, pml[(s * total + id) * 2]);
-    float a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (m != -INFINITY)
-        for (int s = 0; s < splits; ++s) {
-            const f32x2 x = *reinterpret_cast<const f32x2*>(pml + (s * total + id) * 2);
-            if (x[0] == -INFINITY) continue;
-            const float w = __builtin_amdgcn_exp2f(x[0] - m);
-            l += w * x[1];
-            if (c < d) {
-                const f32x4 t0 = *reinterpret_cast<const f32x4*>(po + (s * total + id) * d + c), t1 = *reinterpret_cast<const f32x4*>(po + (s * total + id) * d + c + 4);
+constexpr int lds_many(int DP) { return 4 * 64 * DP; }                                             // in 16-bit units
+constexpr int lds_few(int DP) { return (256 + 128 * (DP + 4)) * 2; }
+constexpr int larger(int a, int b) { return a > b ? a : b; }
+
+// first: the stacked prefix rows (may be none), second: the samples' own rows
+enum { MANY, FEW, MIXED };                                                                         // MIXED: many stacked rows, few own rows
+template <bool BF, int DP, int MODE> __global__ void __launch_bounds__(256, 2) k_ctx_attn(AttnArgs p, Deal first, Deal second) {
+    __shared__ __attribute__((aligned(16))) u16 lds[MODE == MANY ? lds_many(DP) : MODE == FEW ? lds_few(DP) : larger(lds_many(DP), lds_few(DP))];
+    const bool one = (int)blockIdx.x < first.blocks;
+    const Deal& w = one ? first : second;
+    const unsigned block = one ? blockIdx.x : blockIdx.x - first.blocks;
+    if (MODE == MANY || (MODE == MIXED && one)) many_rows<BF, DP>(p, w, block, lds);
+    else few_rows<BF, DP>(p, w, block, lds);
+}
+
+// A context of at most 128 keys and many rows: the rows are what has to be read and written.  The block keeps every key of its key head in LDS and each wave
+// walks over tiles of 32 rows by itself, the next tile's queries in flight; all scores of a row are there at once, so nothing is rescaled.
+template <bool BF, int DP> __global__ void __launch_bounds__(256, DP == 64 ? 3 : 2) k_ctx_short(AttnArgs p, int chunks, int per_chunk) {
+    constexpr int SL = DP / 8, NST = 128 * SL / 256, ND = DP / 32;
+    __shared__ __attribute__((aligned(16))) u16 sK[128 * DP], sV[128 * DP];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, hi = lane >> 5;
+    int y, chunk;
+    block_of(chunks, y, chunk);
+    const int hk = y % p.Hk, b = y / p.Hk, rows = p.Nq * p.G;
+    const int t1 = min((chunk + 1) * per_chunk, (rows + 31) / 32);
+    int t = chunk * per_chunk + wave;
+    u32x4 next[DP / 16];
+    if (t < t1) load_q<DP>(p, row_of(p, b, hk, t * 32 + l31, rows), hi, next);
+    const int len = p.lens ? max(0, min(p.lens[b], p.Nk)) : p.Nk, NJ = (len + 31) / 32;
+    const u16 *kb = p.k + b * p.k_b + hk * p.k_h, *vb = p.v + b * p.v_b + hk * p.v_h;
+    const unsigned char* mk = p.mask ? p.mask + b * p.mask_b : nullptr;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    a[e] += w * t0[e];
-                    a[e + 4] += w * t1[e];
-                }
-            }
+    for (int i = 0; i < NST; ++i) {
+        const int id = tid + 256 * i, r = id / SL, slot = id % SL;
+        if (r >= NJ * 32) break;                                      // (r grows with i)
+        const bool ok = r < len && slot * 8 < p.d && (!mk || mk[r]);
+        const int kk = min(r, len - 1), c = slot * 8 < p.d ? slot * 8 : 0;
+        u32x4 rk = *reinterpret_cast<const u32x4*>(kb + kk * p.k_n + c), rv = *reinterpret_cast<const u32x4*>(vb + kk * p.v_n + c);
+        if (!ok) rk = rv = u32x4{0u, 0u, 0u, 0u};
+        *reinterpret_cast<u32x4*>(sK + slot_at<DP>(r, slot)) = rk;
+        *reinterpret_cast<u32x4*>(sV + slot_at<DP>(r, slot)) = rv;
+    }
+    unsigned bits[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int key = j * 32 + l31;
+        bits[j] = (unsigned)__ballot(key < len && (!mk || mk[key]));
+    }
+    __syncthreads();
+    for (; t < t1; t += 4) {
+        const Row row = row_of(p, b, hk, t * 32 + l31, rows);
+        u32x4 fq[DP / 16];
+#pragma unroll
+        for (int e = 0; e < DP / 16; ++e) fq[e] = next[e];
+        if (t + 4 < t1) load_q<DP>(p, row_of(p, b, hk, (t + 4) * 32 + l31, rows), hi, next);
+        f32x16 s[4];
+        float mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (j >= NJ) break;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[j][r] = 0.f;
+#pragma unroll
+            for (int e = 0; e < DP / 16; ++e) s[j] = mfma<BF>(read_row<DP>(sK, j * 32 + l31, e * 2 + hi), fq[e], s[j]);
+            if (bits[j] != ~0u) hide(s[j], bits[j], 1 << 30, hi);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[j][r]);
         }
+        const float m = half_max(mx) * p.c, ref = m == -INFINITY ? 0.f : m;
+        float l = 0.f;
+        f32x16 acc[ND];
+#pragma unroll
+        for (int n = 0; n < ND; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[n][r] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (j >= NJ) break;
+            u32x4 fp[2];
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) {
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[j][r], p.c, -ref)), p1 = __builtin_amdgcn_exp2f(fmaf(s[j][r + 1], p.c, -ref));
+                l += p0 + p1;
+                fp[r >> 3][(r >> 1) & 3] = pack2<BF>(p0, p1);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int n = 0; n < ND; ++n) acc[n] = mfma<BF>(read_tr<DP>(sV, j * 32 + e * 16, n * 32, lane), fp[e], acc[n]);
+        }
+        l = half_sum(l);
+        const float inv = l > 0.f ? 1.0f / l : 0.f;
+        const long long id = ((long long)b * p.Nq + row.qi) * p.H + row.h;
+#pragma unroll
+        for (int n = 0; n < ND; ++n) store_row<BF>(p.o + id * p.d, acc[n], inv, n, hi, p.d, row.on);
+        if (p.lse && hi == 0 && row.on) p.lse[((long long)b * p.H + row.h) * p.Nq + row.qi] = (m + __builtin_amdgcn_logf(l)) * LN2;
+    }
+}
+
+// Joins the partial results of one row, a wave each: four groups of sixteen lanes take every fourth part, a lane eight channels
+template <bool BF> __global__ void __launch_bounds__(256) k_ctx_join(const float* __restrict__ po, const float* __restrict__ pml, int parts, long long total, int d,
+                                                                   int Nq, int H, u16* __restrict__ o, float* __restrict__ lse) {
+    const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (id >= total) return;
+    const int lane = threadIdx.x & 63, grp = lane >> 4, c = (lane & 15) * 8;
+    float m = -INFINITY;
+    for (int s = lane; s < parts; s += 64) m = fmaxf(m, pml[(s * total + id) * 2]);
+    m = wave_max_f32(m);
+    const float ref = m == -INFINITY ? 0.f : m;
+    float l = 0.f, a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = grp; s < parts; s += 4) {
+        const f32x2 x = *reinterpret_cast<const f32x2*>(pml + (s * total + id) * 2);
+        const float f = __builtin_amdgcn_exp2f(x[0] - ref);          // a part without a key: exp2(-inf) = 0
+        const float* t = po + (s * total + id) * d + (c < d ? c : 0);
+        const f32x4 t0 = *reinterpret_cast<const f32x4*>(t), t1 = *reinterpret_cast<const f32x4*>(t + 4);
+        l += f * x[1];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            a[e] += f * t0[e];
+            a[e + 4] += f * t1[e];
+        }
+    }
+#pragma unroll
+    for (int w = 16; w < 64; w *= 2) {
+        l += __shfl_xor(l, w, 64);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) a[e] += __shfl_xor(a[e], w, 64);
+    }
+    if (grp) return;
     const float inv = l > 0.f ? 1.0f / l : 0.f;
     if (c < d)
         *reinterpret_cast<u32x4*>(o + id * d + c) = u32x4{pack2<BF>(a[0] * inv, a[1] * inv), pack2<BF>(a[2] * inv, a[3] * inv), pack2<BF>(a[4] * inv, a[5] * inv), pack2<BF>(a[6] * inv, a[7] * inv)};
@@ -367,55 +582,67 @@ template <bool BF> __global__ void __launch_bounds__(256) k_ctx_join(const float
 
 // How a call is laid out: which rows a block owns, how the keys are dealt out, which launches that takes
 struct Plan {
-    bool few;                  // own keys: at most 32 rows per key head, waves split the keys
-    bool stack;                // prefix: rows of all samples stacked (a row tile of one sample alone would be mostly empty)
-    bool stack_few;
-    int own_splits, own_per, pre_splits, pre_per;
+    bool one_pass;             // k_ctx_short
+    int mode, chunks, per_chunk;
+    Deal first, second;
     int parts;                 // partial results to join (0: the kernel writes the result)
 };
 Plan make_plan(int B, int Nq, int Np, int Nk, int H, int Hk) {
     Plan s{};
     const int G = H / Hk;
-    const long long rows = (long long)Nq * G;
-    s.few = rows <= 32;
-    s.stack = Np > 0 && rows < 128;
-    s.stack_few = s.stack && rows * B <= 32;
-    const int kt = s.few ? 128 : 64;
-    const long long blocks = (long long)B * Hk * (s.few ? 1 : (rows + 127) / 128);
-    const int tiles = (Nk + kt - 1) / kt + (s.stack ? 0 : (Np + kt - 1) / kt);
-    auto deal = [](long long blocks, int tiles, int least, int& splits, int& per) {      // about 512 blocks, at least `least` tiles each
-        const long long want = blocks >= 384 ? 1 : (512 + blocks - 1) / blocks;
-        per = (int)((tiles + want - 1) / want);
-        if (per < least) per = least;
-        splits = tiles > per ? (tiles + per - 1) / per : 1;
-        if (splits == 1) per = tiles > 0 ? tiles : 1;
-    };
-    deal(blocks, tiles, s.few ? 2 : 4, s.own_splits, s.own_per);
-    if (s.stack) {
-        const int pk = s.stack_few ? 128 : 64;
-        deal((long long)Hk * ((rows * B + 127) / 128), (Np + pk - 1) / pk, s.stack_few ? 2 : 4, s.pre_splits, s.pre_per);
+    const long long rows = (long long)Nq * G, heads = (long long)B * Hk;
+    if (Np == 0 && Nk <= 128 && rows >= 64) {
+        // about 1024 blocks (three or four a CU), at least two tiles a wave: the keys are staged once a block
+        const long long tiles = (rows + 31) / 32, want = heads >= 1024 ? 1 : (1024 + heads - 1) / heads;
+        const long long per = (tiles + want - 1) / want;
+        s.one_pass = true;
+        s.per_chunk = (int)(per < 8 ? 8 : (per + 3) / 4 * 4);
+        s.chunks = (int)((tiles + s.per_chunk - 1) / s.per_chunk);
+        return s;
     }
-    const int own = Nk > 0 || !s.stack ? s.own_splits : 0;
-    s.parts = own + (s.stack ? s.pre_splits : 0);
-    if (s.parts <= 1) s.parts = 0;
+    auto deal = [](Deal& w, long long tiles_heads, int key_tiles, int least) {      // about 512 blocks, at least `least` key tiles each
+        const long long want = tiles_heads >= 384 ? 1 : (512 + tiles_heads - 1) / tiles_heads;
+        long long per = (key_tiles + want - 1) / want;
+        if (per < least) per = least;
+        w.splits = key_tiles > per ? (int)((key_tiles + per - 1) / per) : 1;
+        w.per_split = (int)per;
+        w.blocks = (int)(tiles_heads * w.splits);
+    };
+    const bool few = rows <= 32, stack = Np > 0 && rows < 128;      // a row tile of one sample alone would be mostly empty
+    const bool stack_few = few && rows * B <= 32;
+    s.mode = !few ? MANY : (!stack || stack_few) ? FEW : MIXED;
+    if (stack) {
+        const int kt = stack_few ? 128 : 64;
+        s.first.stacked = 1;
+        s.first.np = Np;
+        s.first.xtiles = stack_few ? 1 : (int)((rows * B + 127) / 128);
+        deal(s.first, (long long)Hk * s.first.xtiles, (Np + kt - 1) / kt, stack_few ? 2 : 4);
+        s.parts = s.first.splits;
+    }
+    if (Nk > 0 || !stack) {
+        const int kt = few ? 128 : 64;
+        s.second.np = stack ? 0 : Np;
+        s.second.xtiles = few ? 1 : (int)((rows + 127) / 128);
+        s.second.part0 = s.parts;
+        deal(s.second, heads * s.second.xtiles, (Nk + kt - 1) / kt + (s.second.np + kt - 1) / kt, few ? 2 : 4);
+        s.parts += s.second.splits;
+    }
+    if (s.parts == 1) s.parts = 0;
     return s;
 }
 
-template <bool BF, int DP> void launch_one(const AttnArgs& p, bool ws, dim3 grid, hipStream_t st) {
-    if (ws) hipLaunchKernelGGL((k_ctx_attn<BF, DP, 1, true>), grid, dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((k_ctx_attn<BF, DP, 1, false>), grid, dim3(256), 0, st, p);
-}
-void launch_attn(AttnArgs p, int dtype, bool ws, long long tiles, long long heads, hipStream_t st) {
-    p.xtiles = (int)tiles;
-    const dim3 grid((unsigned)(tiles * heads * p.splits));
-    if (dtype == 2) {
-        if (p.d <= 64) launch_one<true, 64>(p, ws, grid, st);
-        else if (p.d <= 96) launch_one<true, 96>(p, ws, grid, st);
-        else launch_one<true, 128>(p, ws, grid, st);
-    } else {
-        if (p.d <= 64) launch_one<false, 64>(p, ws, grid, st);
-        else if (p.d <= 96) launch_one<false, 96>(p, ws, grid, st);
-        else launch_one<false, 128>(p, ws, grid, st);
+template <bool BF, int DP> void launch_fwd(const AttnArgs& p, const Plan& s, hipStream_t st) {
+    if (s.one_pass) {
+        hipLaunchKernelGGL((k_ctx_short<BF, DP>), dim3((unsigned)((long long)s.chunks * p.B * p.Hk)), dim3(256), 0, st, p, s.chunks, s.per_chunk);
+        return;
+    }
+    const dim3 grid((unsigned)(s.first.blocks + s.second.blocks));
+    if (s.mode == MANY) hipLaunchKernelGGL((k_ctx_attn<BF, DP, MANY>), grid, dim3(256), 0, st, p, s.first, s.second);
+    else if (s.mode == FEW) hipLaunchKernelGGL((k_ctx_attn<BF, DP, FEW>), grid, dim3(256), 0, st, p, s.first, s.second);
+    else hipLaunchKernelGGL((k_ctx_attn<BF, DP, MIXED>), grid, dim3(256), 0, st, p, s.first, s.second);
+    if (s.parts) {
+        const long long total = (long long)p.B * p.Nq * p.H;
+        hipLaunchKernelGGL((k_ctx_join<BF>), dim3((unsigned)((total + 3) / 4)), dim3(256), 0, st, p.po, p.pml, s.parts, total, p.d, p.Nq, p.H, p.o, p.lse);
     }
 }
 
@@ -576,14 +803,8 @@ template <bool BF, int DP> __global__ void __launch_bounds__(256, DP == 128 ? 1 
         if (t + 1 < T) store_tile(buf ^ 1);
         __syncthreads();
     }
-    if (!on) return;
 #pragma unroll
-    for (int n = 0; n < ND; ++n)
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-            const int c = n * 32 + 2 * e + 4 * hi;
-            if (c < p.d) *reinterpret_cast<u32x2*>(p.dq + id * p.d + c) = u32x2{pack2<BF>(acc[n][e] * back, acc[n][e + 1] * back), pack2<BF>(acc[n][e + 2] * back, acc[n][e + 3] * back)};
-        }
+    for (int n = 0; n < ND; ++n) store_row<BF>(p.dq + id * p.d, acc[n], back, n, hi, p.d, on);
 }
 
 // dk and dv: a wave owns 32 keys as accumulator columns (K, V in registers), the block 128, and walks over tiles of 64 rows; the rows of all samples
@@ -768,38 +989,31 @@ template <bool BF, int DP, bool FUSED> __global__ void __launch_bounds__(256, DP
                 for (int e = 0; e < 16; ++e) acc[e] = 0.f;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) acc = mfma<BF>(read_tr<DP>(sK, e * 16, n * 32, lane), read_tr<RT>(sS, e * 16, i * 32, lane), acc);
-                const int r = base + i * 32 + l31;
-                if (r < rows) {
-                    const long long id = ((long long)b * p.Nq + r / p.G) * p.H + hk * p.G + r % p.G;
-#pragma unroll
-                    for (int e = 0; e < 16; e += 4) {
-                        const int c = n * 32 + 2 * e + 4 * hi;
-                        if (c < p.d)
-                            *reinterpret_cast<u32x2*>(p.dq + id * p.d + c) = u32x2{pack2<BF>(acc[e] * back, acc[e + 1] * back), pack2<BF>(acc[e + 2] * back, acc[e + 3] * back)};
-                    }
-                }
+                const int r = base + i * 32 + l31, rr = min(r, rows - 1);
+                const long long id = ((long long)b * p.Nq + rr / p.G) * p.H + hk * p.G + rr % p.G;
+                store_row<BF>(p.dq + id * p.d, acc, back, n, hi, p.d, r < rows);
             }
             __syncthreads();                                                    // sS is written again in the next round
         }
     }
-    if (!in) return;
     const float bk_ = p.scale / run, bv_ = BF ? 1.f : 2.44140625e-4f;
-    const long long at = (((long long)bk * p.Nk + key) * p.Hk + hk) * p.d, plane = (long long)p.Bk * p.Nk * p.Hk * p.d;
+    const long long at = (((long long)bk * p.Nk + (in ? key : 0)) * p.Hk + hk) * p.d, plane = (long long)p.Bk * p.Nk * p.Hk * p.d;
 #pragma unroll
-    for (int n = 0; n < ND; ++n)
+    for (int n = 0; n < ND; ++n) {
+        if (!p.part) {
+            store_row<BF>(p.dk + at, ak[n], bk_, n, hi, p.d, in);
+            store_row<BF>(p.dv + at, av[n], bv_, n, hi, p.d, in);
+        } else if (in) {
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-            const int c = n * 32 + 2 * e + 4 * hi;
-            if (c >= p.d) continue;
-            if (p.part) {
+            for (int e = 0; e < 16; e += 4) {
+                const int c = n * 32 + 2 * e + 4 * hi;
+                if (c >= p.d) continue;
                 float* o = p.part + 2 * chunk * plane + at + c;
                 *reinterpret_cast<f32x4*>(o) = f32x4{ak[n][e] * bk_, ak[n][e + 1] * bk_, ak[n][e + 2] * bk_, ak[n][e + 3] * bk_};
                 *reinterpret_cast<f32x4*>(o + plane) = f32x4{av[n][e] * bv_, av[n][e + 1] * bv_, av[n][e + 2] * bv_, av[n][e + 3] * bv_};
-            } else {
-                *reinterpret_cast<u32x2*>(p.dk + at + c) = u32x2{pack2<BF>(ak[n][e] * bk_, ak[n][e + 1] * bk_), pack2<BF>(ak[n][e + 2] * bk_, ak[n][e + 3] * bk_)};
-                *reinterpret_cast<u32x2*>(p.dv + at + c) = u32x2{pack2<BF>(av[n][e] * bv_, av[n][e + 1] * bv_), pack2<BF>(av[n][e + 2] * bv_, av[n][e + 3] * bv_)};
             }
         }
+    }
 }
 
 // dk (y = 0) and dv (y = 1): the chunks' partial sums in their order
@@ -905,22 +1119,14 @@ int vidseg_context_attention_fwd(const void* q, long long q_b, long long q_n, lo
         p.po = (float*)scratch;
         p.pml = p.po + s.parts * total * d;
     }
-    const long long rows = (long long)Nq * p.G;
-    if (s.stack) {
-        AttnArgs a = p;
-        a.stacked = 1; a.splits = s.pre_splits; a.per_split = s.pre_per; a.split0 = 0; a.Nk = 0; a.causal = 0; a.lens = nullptr; a.mask = nullptr;
-        launch_attn(a, dtype, s.stack_few, s.stack_few ? 1 : (rows * B + 127) / 128, Hk, st);
-        p.Np = 0;
-        p.split0 = s.pre_splits;
-    }
-    if (Nk > 0 || !s.stack) {
-        p.splits = s.own_splits; p.per_split = s.own_per;
-        launch_attn(p, dtype, s.few, s.few ? 1 : (rows + 127) / 128, (long long)B * Hk, st);
-    }
-    if (s.parts) {
-        const unsigned blocks = (unsigned)((total + 15) / 16);
-        if (dtype == 2) hipLaunchKernelGGL((k_ctx_join<true>), dim3(blocks), dim3(256), 0, st, p.po, p.pml, s.parts, total, d, Nq, H, p.o, lse);
-        else hipLaunchKernelGGL((k_ctx_join<false>), dim3(blocks), dim3(256), 0, st, p.po, p.pml, s.parts, total, d, Nq, H, p.o, lse);
+    if (dtype == 2) {
+        if (d <= 64) launch_fwd<true, 64>(p, s, st);
+        else if (d <= 96) launch_fwd<true, 96>(p, s, st);
+        else launch_fwd<true, 128>(p, s, st);
+    } else {
+        if (d <= 64) launch_fwd<false, 64>(p, s, st);
+        else if (d <= 96) launch_fwd<false, 96>(p, s, st);
+        else launch_fwd<false, 128>(p, s, st);
     }
     VS_CHECK_LAUNCH("context_attention");
     return VS_OK;
