@@ -397,7 +397,7 @@ int vidseg_groupnorm_act_bwd(const void* dy, long long dy_batch_stride, long lon
 /* Attention over contexts (ATT:286-364 with other head widths, lengths and contexts; csrc/context_attn.hip; dtype 1 or 2): every query of sample b
  * attends, as one softmax, to Np prefix keys that all samples share and to the sample's own keys 0 .. lens[b] - 1 (lens NULL: all Nk) for which
  * mask[b * mask_b + key] != 0 (mask NULL: all); causal: query i sees own keys up to lens[b] - Nq + i (no mask then).  Heads of width d (8..128, d % 8
- * == 0), query head h on key head h * Hk / H; element strides per sample, row and head (multiples of 8; 0 shares one sample), 16-byte aligned.
+ * == 0), query head h on key head h * Hk / H; element strides per sample, row and head (multiples of 8, rows below 2^24; 0 shares one sample), 16-byte aligned.
  * out [B][Nq][H][d]; lse (opt) fp32 [B][H][Nq].  A query without a key: out 0, lse -inf.  Keys that do not exist are not read for their value.
  * scratch: vidseg_context_attention_scratch_kib(...) KiB (0: none; -1: sizes refused). */
 int vidseg_context_attention_scratch_kib(int B, int Nq, int Np, int Nk, int H, int Hk, int d);

@@ -152,13 +152,13 @@ def groupnorm_act(x, gamma, beta, *, groups=32, eps=1e-5, act=1):
 
 # ----------------------------------------------------------------------------- attention to contexts
 def _heads_of(t, d):
-    """[.., N, heads * d] or [.., N, heads, d] as (tensor, pointer, row stride, head stride): a copy only where the last dimension is not contiguous or
-    16-byte pieces are not aligned."""
+    """[.., N, heads * d] or [.., N, heads, d] as (tensor, pointer, first, row and head stride): a copy only where the last dimension is not contiguous,
+    16-byte pieces are not aligned or rows lie 2^24 elements and more apart."""
     while True:
         st = t.stride()
         n, h = (st[-2], d) if len(st) == 3 else (st[-3], st[-2])
         at = t.data_ptr()
-        if st[-1] == 1 and not (st[0] | n | h) & 7 and not at & 15:
+        if st[-1] == 1 and not (st[0] | n | h) & 7 and not at & 15 and n < 1 << 24:
             return t, at, st[0] if t.shape[0] > 1 else 0, n, h
         t = t.clone(memory_format=torch.contiguous_format)
 

@@ -22,6 +22,7 @@ typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) s16x4* lds4;
+template <int V> struct Const { static constexpr int value = V; };
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
@@ -33,6 +34,12 @@ template <bool BF> __device__ __forceinline__ unsigned pack2(float lo, float hi)
     if constexpr (BF) return __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{lo, hi}, b2));
     else return __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{lo, hi}, h2));
 }
+// acc + a.lo b.lo + a.hi b.hi
+template <bool BF> __device__ __forceinline__ float dot2(unsigned a, unsigned b, float acc) {
+    if constexpr (BF) return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, a), __builtin_bit_cast(b2, b), acc, false);
+    else return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, a), __builtin_bit_cast(h2, b), acc, false);
+}
+__device__ __forceinline__ f32x16 zero16() { return f32x16{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}; }
 // the same value in both lane halves: max / sum over lanes l and l + 32
 __device__ __forceinline__ float half_max(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -61,7 +68,87 @@ template <int DP> __device__ __forceinline__ u32x4 read_tr(const u16* t, int r0,
                                 __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(t + slot_at<DP>(r + 8, slot) + in))};
     return __builtin_bit_cast(u32x4, v);
 }
+// The same for all 32-column blocks of 16 rows at once.  Fetches into LDS may be under way into another buffer: the compiler would wait for them before every
+// transpose read it can see (it takes them for writes), so these are spelled out, with their own wait in the same statement.
+template <int DP> struct Turned {
+    unsigned at[2][DP / 32];                                          // byte addresses for rows 4 hi .. and 8 + 4 hi .. of a tile
+    __device__ __forceinline__ void init(const u16* t, int lane) {
+        const int r = 4 * (lane >> 5) + ((lane & 15) >> 2), in = (lane & 1) * 4;
+#pragma unroll
+        for (int n = 0; n < DP / 32; ++n) {
+            const int slot = n * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+            at[0][n] = (unsigned)(unsigned long long)(lds4)(t + slot_at<DP>(r, slot) + in);
+            at[1][n] = (unsigned)(unsigned long long)(lds4)(t + slot_at<DP>(r + 8, slot) + in);
+        }
+    }
+    // rows R0 .. R0 + 15
+    template <int R0> __device__ __forceinline__ void read(u32x4 (&f)[DP / 32]) const {
+#if defined(__HIP_DEVICE_COMPILE__)
+        constexpr int IMM = R0 * DP * 2;
+        u32x2 a[DP / 32], b[DP / 32];
+        if constexpr (DP == 64)
+            asm volatile("ds_read_b64_tr_b16 %0, %4 offset:%8\n\tds_read_b64_tr_b16 %1, %5 offset:%8\n\tds_read_b64_tr_b16 %2, %6 offset:%8\n\t"
+                         "ds_read_b64_tr_b16 %3, %7 offset:%8\n\ts_waitcnt lgkmcnt(0)"
+                         : "=&v"(a[0]), "=&v"(b[0]), "=&v"(a[1]), "=&v"(b[1])
+                         : "v"(at[0][0]), "v"(at[1][0]), "v"(at[0][1]), "v"(at[1][1]), "n"(IMM)
+                         : "memory");
+        else if constexpr (DP == 96)
+            asm volatile("ds_read_b64_tr_b16 %0, %6 offset:%12\n\tds_read_b64_tr_b16 %1, %7 offset:%12\n\tds_read_b64_tr_b16 %2, %8 offset:%12\n\t"
+                         "ds_read_b64_tr_b16 %3, %9 offset:%12\n\tds_read_b64_tr_b16 %4, %10 offset:%12\n\tds_read_b64_tr_b16 %5, %11 offset:%12\n\ts_waitcnt lgkmcnt(0)"
+                         : "=&v"(a[0]), "=&v"(b[0]), "=&v"(a[1]), "=&v"(b[1]), "=&v"(a[2]), "=&v"(b[2])
+                         : "v"(at[0][0]), "v"(at[1][0]), "v"(at[0][1]), "v"(at[1][1]), "v"(at[0][2]), "v"(at[1][2]), "n"(IMM)
+                         : "memory");
+        else
+            asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%16\n\tds_read_b64_tr_b16 %1, %9 offset:%16\n\tds_read_b64_tr_b16 %2, %10 offset:%16\n\t"
+                         "ds_read_b64_tr_b16 %3, %11 offset:%16\n\tds_read_b64_tr_b16 %4, %12 offset:%16\n\tds_read_b64_tr_b16 %5, %13 offset:%16\n\t"
+                         "ds_read_b64_tr_b16 %6, %14 offset:%16\n\tds_read_b64_tr_b16 %7, %15 offset:%16\n\ts_waitcnt lgkmcnt(0)"
+                         : "=&v"(a[0]), "=&v"(b[0]), "=&v"(a[1]), "=&v"(b[1]), "=&v"(a[2]), "=&v"(b[2]), "=&v"(a[3]), "=&v"(b[3])
+                         : "v"(at[0][0]), "v"(at[1][0]), "v"(at[0][1]), "v"(at[1][1]), "v"(at[0][2]), "v"(at[1][2]),
+                           "v"(at[0][3]), "v"(at[1][3]), "n"(IMM)
+                         : "memory");
+#pragma unroll
+        for (int n = 0; n < DP / 32; ++n) f[n] = u32x4{a[n][0], a[n][1], b[n][0], b[n][1]};
+#endif
+    }
+};
 template <int DP> __device__ __forceinline__ u32x4 read_row(const u16* t, int r, int slot) { return *reinterpret_cast<const u32x4*>(t + slot_at<DP>(r, slot)); }
+
+// Fetching of tiles of 64 rows straight into LDS (16 bytes a lane, four waves): lane i of piece w + 4 j fills 16-byte place (w + 4 j) 64 + i of the tile, so it
+// asks for the slot that belongs there.  What does not exist is asked for beyond the buffer's end and arrives as zeros.
+typedef __attribute__((address_space(3))) void* lds_ptr;
+constexpr unsigned BEYOND = 0xF0000000u;
+template <int DP> struct Fetch {
+    static constexpr int SL = DP / 8, N = 64 * SL / 256, M = 256 % SL ? N : 1;      // M = 1: a lane's places differ by whole rows that the swizzle does not see
+    unsigned off[M];
+    static __device__ __forceinline__ int row(int tid, int j) { return M == 1 ? tid / SL + j * (256 / SL) : (tid + 256 * j) / SL; }
+    __device__ __forceinline__ void init(int tid, long long step, int d) {           // step: elements from row to row (64 of them below 2^31 bytes)
+#pragma unroll
+        for (int j = 0; j < M; ++j) {
+            const int r = row(tid, j), c = (((tid + 256 * j) % SL) ^ swz<DP>(r)) * 8;
+            off[j] = c < d ? (unsigned)(r * (int)step + c) * 2u : BEYOND;
+        }
+    }
+    // the tile at `at`; rows of it that exist: live
+    __device__ __forceinline__ void tile(const u16* at, long long step, unsigned long long live, u16* lds, int tid, int wave) const {
+#if defined(__HIP_DEVICE_COMPILE__)                                    // (the host pass knows no 16-byte fetch)
+        const auto span = __builtin_amdgcn_make_buffer_rsrc(const_cast<u16*>(at), 0, (int)0xE0000000u, 0x00020000);
+        if (live == ~0ull) {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(span, (lds_ptr)(lds + (wave + 4 * j) * 512), 16, (int)off[M == 1 ? 0 : j], M == 1 ? j * (512 / SL) * (int)step : 0, 0, 0);
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(span, (lds_ptr)(lds + (wave + 4 * j) * 512), 16, (live >> row(tid, j)) & 1 ? (int)off[M == 1 ? 0 : j] : (int)BEYOND,
+                                                         M == 1 ? j * (512 / SL) * (int)step : 0, 0, 0);
+        }
+#endif
+    }
+};
+__device__ __forceinline__ void landed() {                             // this wave's fetches are in LDS; the barrier after it makes all of them visible
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
 
 struct AttnArgs {
     const u16 *q, *kp, *vp, *k, *v;
@@ -153,16 +240,30 @@ template <bool BF> __device__ __forceinline__ void store_row(u16* row, const f32
     }
 }
 
-// One step of the running softmax on NJ blocks of 32 scores: probabilities as B operands; m in log2 units, acc and l rescaled where it moved
-template <bool BF, int NJ, int ND> __device__ __forceinline__ void soften(const f32x16 (&s)[NJ], float c, float& m, float& l, f32x16 (&acc)[ND], u32x4 (&fp)[NJ][2]) {
-    float mx = s[0][0];
+// One step of the running softmax on a block of 32 scores: probabilities p = exp2(s c - m) as B operands, their sum of this lane half into l.  m (log2 units)
+// is moved only where it has to be: for a row's first key, and where a half's sum of 16 probabilities passes 2^12 (fp16 holds 2^16) -- the maximum,
+// the rescaling and the exchange between the lane halves are then done and the probabilities taken anew; otherwise the scores are touched once.
+template <bool BF, int ND> __device__ __forceinline__ void soften(const f32x16& s, float c, float& m, float& l, f32x16 (&acc)[ND], u32x4 (&fp)[2]) {
+    float sum;
+    auto take = [&](float ref) {
+        float a[2] = {0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
+        for (int r = 0; r < 16; r += 2) {
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[r], c, -ref)), p1 = __builtin_amdgcn_exp2f(fmaf(s[r + 1], c, -ref));
+            fp[r >> 3][(r >> 1) & 3] = pack2<BF>(p0, p1);             // the one rounding of the probabilities
+            a[0] += p0;
+            a[1] += p1;
+        }
+        sum = a[0] + a[1];
+    };
+    const bool none = m == -INFINITY;
+    take(none ? 0.f : m);
+    if (__builtin_expect(__any(none || !(sum <= 4096.f)), 0)) {
+        float mx = s[0];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[j][r]);
-    const float m_new = fmaxf(m, half_max(mx) * c);
-    const float ref = m_new == -INFINITY ? 0.f : m_new;               // a row without a key so far: every exp2 below gives 0
-    if (__any(m_new > m)) {
+        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+        const float m_new = fmaxf(m, half_max(mx) * c);
+        const float ref = m_new == -INFINITY ? 0.f : m_new;           // still no key: every exp2 gives 0
         const float alpha = __builtin_amdgcn_exp2f(m - ref);
         l *= alpha;
 #pragma unroll
@@ -170,17 +271,9 @@ template <bool BF, int NJ, int ND> __device__ __forceinline__ void soften(const 
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[n][r] *= alpha;
         m = m_new;
+        take(ref);
     }
-    float sum = 0.f;
-#pragma unroll
-    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-        for (int r = 0; r < 16; r += 2) {
-            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[j][r], c, -ref)), p1 = __builtin_amdgcn_exp2f(fmaf(s[j][r + 1], c, -ref));
-            sum += p0 + p1;
-            fp[j][r >> 3][(r >> 1) & 3] = pack2<BF>(p0, p1);          // p in (0, 1]: the one rounding of the probabilities
-        }
-    l += half_sum(sum);
+    l += sum;
 }
 
 // -inf into the scores of keys that do not exist (bits) or lie behind lim (in this lane's numbering)
@@ -193,95 +286,89 @@ __device__ __forceinline__ void hide(f32x16& s, unsigned bits, int lim, int hi) 
     }
 }
 
-// Many rows: the block's four waves own 32 rows each and share key tiles of 64 in LDS, staged through registers one tile ahead.
+// Many rows: the block's four waves own 32 rows each and share key tiles of 64 in LDS, fetched one tile ahead.
 template <bool BF, int DP> __device__ __forceinline__ void many_rows(const AttnArgs& p, const Deal& w, unsigned block, u16* lds) {
-    constexpr int KT = 64, SL = DP / 8, NST = KT * SL / 256, ND = DP / 32, TILE = KT * DP;
+    constexpr int KT = 64, ND = DP / 32, TILE = KT * DP, BR = 128;
     u16 *sK = lds, *sV = lds + 2 * TILE;                              // two buffers each
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, hi = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, hi = lane >> 5;
     const Place at = place_of(p, w, block);
-    const long long r0 = (long long)at.xt * 128;
+    const long long r0 = (long long)at.xt * BR;
     const Row row = row_of(p, at.b, at.hk, r0 + wave * 32 + l31, at.rows);
     u32x4 fq[DP / 16];
     load_q<DP>(p, row, hi, fq);
-    const long long last_r = (r0 + 128 < at.rows ? r0 + 128 : at.rows) - 1;
+    const long long last_r = (r0 + BR < at.rows ? r0 + BR : at.rows) - 1;
     const int seen = p.causal ? max(0, min(at.len, at.len - p.Nq + 1 + (int)(last_r / p.G))) : at.len;      // own keys that the block's last row sees
     const int all_see = p.causal ? at.len - p.Nq + 1 + (int)(r0 / p.G) : at.len;                             // own keys that every row sees
     const int T0 = (w.np + KT - 1) / KT, T1 = (seen + KT - 1) / KT;
     const int tb = min(at.split * w.per_split, T0 + T1), te = w.splits == 1 ? T0 + T1 : min(tb + w.per_split, T0 + T1);
 
-    u32x4 rk[NST], rv[NST];
-    unsigned long long live = 0;                                      // keys of the staged tile that exist
+    unsigned long long live = 0;                                      // keys of the fetched tile that exist
     const u16 *kown = p.k + at.b * p.k_b + at.hk * p.k_h, *vown = p.v + at.b * p.v_b + at.hk * p.v_h;
+    const u16 *kpre = p.kp + at.hk * p.kp_h, *vpre = p.vp + at.hk * p.vp_h;
     const unsigned char* mrow = p.mask ? p.mask + at.b * p.mask_b : nullptr;
-    auto load_tile = [&](int t) {
-        const bool own = t >= T0;
-        const int k0 = (own ? t - T0 : t) * KT, n = own ? seen : w.np;
-        const u16 *kb = own ? kown : p.kp + at.hk * p.kp_h, *vb = own ? vown : p.vp + at.hk * p.vp_h;
-        const long long kn = own ? p.k_n : p.kp_n, vn = own ? p.v_n : p.vp_n;
-        const unsigned char* mk = own ? mrow : nullptr;
-#pragma unroll
-        for (int i = 0; i < NST; ++i) {
-            const int id = tid + 256 * i, r = id / SL, slot = id % SL, key = k0 + r, kk = min(key, n - 1);
-            const bool ok = key < n && slot * 8 < p.d && (!mk || mk[kk]);
-            const int c = slot * 8 < p.d ? slot * 8 : 0;
-            rk[i] = *reinterpret_cast<const u32x4*>(kb + kk * kn + c);
-            rv[i] = *reinterpret_cast<const u32x4*>(vb + kk * vn + c);
-            if (!ok) rk[i] = rv[i] = u32x4{0u, 0u, 0u, 0u};
+    Turned<DP> turned;
+    turned.init(sV, lane);
+    Fetch<DP> fk, fv;
+    bool prefix = tb < T0;
+    fk.init(tid, prefix ? p.kp_n : p.k_n, p.d);
+    fv.init(tid, prefix ? p.vp_n : p.v_n, p.d);
+    auto fetch = [&](int t, int buf) {
+        if (prefix && t >= T0) {
+            prefix = false;
+            fk.init(tid, p.k_n, p.d);
+            fv.init(tid, p.v_n, p.d);
         }
-        const int key = k0 + lane;
-        live = __ballot(key < n && (!mk || mk[min(key, n - 1)]));
-    };
-    auto store_tile = [&](int buf) {
-#pragma unroll
-        for (int i = 0; i < NST; ++i) {
-            const int id = tid + 256 * i, r = id / SL, slot = id % SL;
-            *reinterpret_cast<u32x4*>(sK + buf * TILE + slot_at<DP>(r, slot)) = rk[i];
-            *reinterpret_cast<u32x4*>(sV + buf * TILE + slot_at<DP>(r, slot)) = rv[i];
-        }
+        const int k0 = (prefix ? t : t - T0) * KT, n = (prefix ? w.np : seen) - k0;
+        const long long kn = prefix ? p.kp_n : p.k_n, vn = prefix ? p.vp_n : p.v_n;
+        live = n >= KT ? ~0ull : (1ull << n) - 1;
+        if (!prefix && mrow) live = __ballot(lane < n && mrow[k0 + min(lane, n - 1)]);
+        fk.tile((prefix ? kpre : kown) + k0 * kn, kn, live, sK + buf * TILE, tid, wave);
+        fv.tile((prefix ? vpre : vown) + k0 * vn, vn, live, sV + buf * TILE, tid, wave);
     };
     f32x16 acc[ND];
     float m = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int n = 0; n < ND; ++n)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[n][r] = 0.f;
-    if (tb < te) {
-        load_tile(tb);
-        store_tile(0);
-    }
-    __syncthreads();
-    for (int t = tb; t < te; ++t) {
-        const int buf = (t - tb) & 1;
-        const u16 *tk = sK + buf * TILE, *tv = sV + buf * TILE;
+    for (int n = 0; n < ND; ++n) acc[n] = zero16();
+    if (tb < te) fetch(tb, 0);
+    landed();
+    auto work = [&](auto which, int t) {                              // the buffer is a constant of the code: every LDS address is one register and an immediate
+        constexpr int buf = decltype(which)::value;
+        const u16* tk = sK + buf * TILE;
         const unsigned long long now = live;
-        if (t + 1 < te) load_tile(t + 1);
+        if (t + 1 < te) fetch(t + 1, buf ^ 1);
         const int k0 = (t >= T0 ? t - T0 : t) * KT;
         const bool edge = p.causal && t >= T0 && k0 + KT > all_see;
+        // both halves' scores first: the matrix pipe works on the second while the first becomes probabilities
         f32x16 s[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[j][r] = 0.f;
-#pragma unroll
-            for (int e = 0; e < DP / 16; ++e) s[j] = mfma<BF>(read_row<DP>(tk, j * 32 + l31, e * 2 + hi), fq[e], s[j]);
-        }
-        if (now != ~0ull || edge) {
-            const int lim = edge ? at.len - p.Nq + row.qi - k0 - 4 * hi : 1 << 30;
-            hide(s[0], (unsigned)now, lim, hi);
-            hide(s[1], (unsigned)(now >> 32), lim - 32, hi);
-        }
-        u32x4 fp[2][2];
-        soften<BF, 2, ND>(s, p.c, m, l, acc, fp);
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
+            for (int e = 0; e < DP / 16; ++e) s[j] = mfma<BF>(read_row<DP>(tk, j * 32 + l31, e * 2 + hi), fq[e], e ? s[j] : zero16());
+        if (now != ~0ull || edge)
 #pragma unroll
-                for (int n = 0; n < ND; ++n) acc[n] = mfma<BF>(read_tr<DP>(tv, j * 32 + e * 16, n * 32, lane), fp[j][e], acc[n]);
-        if (t + 1 < te) store_tile(buf ^ 1);
-        __syncthreads();
+            for (int j = 0; j < 2; ++j) hide(s[j], (unsigned)(now >> (32 * j)), edge ? at.len - p.Nq + row.qi - k0 - 32 * j - 4 * hi : 1 << 30, hi);
+        auto half = [&](auto which_half) {
+            constexpr int j = decltype(which_half)::value;
+            u32x4 fp[2], fv[ND];
+            soften<BF, ND>(s[j], p.c, m, l, acc, fp);
+            turned.template read<buf * KT + j * 32>(fv);
+#pragma unroll
+            for (int n = 0; n < ND; ++n) acc[n] = mfma<BF>(fv[n], fp[0], acc[n]);
+            turned.template read<buf * KT + j * 32 + 16>(fv);
+#pragma unroll
+            for (int n = 0; n < ND; ++n) acc[n] = mfma<BF>(fv[n], fp[1], acc[n]);
+        };
+        half(Const<0>{});
+        half(Const<1>{});
+        landed();
+    };
+    for (int t = tb; t < te; t += 2) {
+        work(Const<0>{}, t);
+        if (t + 1 < te) work(Const<1>{}, t + 1);
     }
-    const long long total = (long long)p.B * p.Nq * p.H, id = ((long long)row.b * p.Nq + row.qi) * p.H + row.h, part = w.part0 + at.split;
+    const long long total = (long long)p.B * p.Nq * p.H, part = w.part0 + at.split;
+    l = half_sum(l);
+    const long long id = ((long long)row.b * p.Nq + row.qi) * p.H + row.h;
     const float inv = l > 0.f ? 1.0f / l : 0.f;
 #pragma unroll
     for (int n = 0; n < ND; ++n) {
@@ -367,11 +454,11 @@ template <bool BF, int DP> __device__ __forceinline__ void few_rows(const AttnAr
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s)
             if (s * 16 + hi * 8 >= p.d || !((now >> l31) & 1u)) rk[s] = u32x4{0u, 0u, 0u, 0u};
-        f32x16 s[1];
+        f32x16 s;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
+        for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
-        for (int e = 0; e < DP / 16; ++e) s[0] = mfma<BF>(rk[e], fq[e], s[0]);
+        for (int e = 0; e < DP / 16; ++e) s = mfma<BF>(rk[e], fq[e], s);
         if (more) load_k(t + 1);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -382,15 +469,15 @@ template <bool BF, int DP> __device__ __forceinline__ void few_rows(const AttnAr
         if (more) load_v(t + 1);
         const int k0 = first(t);
         const bool edge = p.causal && t >= T0 && k0 + 32 > len - p.Nq + 1;
-        if (now != ~0u || edge) hide(s[0], now, edge ? len - p.Nq + row.qi - k0 - 4 * hi : 1 << 30, hi);
-        u32x4 fp[1][2];
-        soften<BF, 1, ND>(s, p.c, m, l, acc, fp);
+        if (now != ~0u || edge) hide(s, now, edge ? len - p.Nq + row.qi - k0 - 4 * hi : 1 << 30, hi);
+        u32x4 fp[2];
+        soften<BF, ND>(s, p.c, m, l, acc, fp);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");        // the other lanes' V rows are in place (a wave's LDS operations keep their order)
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int e = 0; e < 2; ++e)
 #pragma unroll
-            for (int n = 0; n < ND; ++n) acc[n] = mfma<BF>(read_tr<DP>(sV, e * 16, n * 32, lane), fp[0][e], acc[n]);
+            for (int n = 0; n < ND; ++n) acc[n] = mfma<BF>(read_tr<DP>(sV, e * 16, n * 32, lane), fp[e], acc[n]);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");        // ... and read before the next ones replace them
         __builtin_amdgcn_wave_barrier();
     }
@@ -399,6 +486,7 @@ template <bool BF, int DP> __device__ __forceinline__ void few_rows(const AttnAr
     float* sm = reinterpret_cast<float*>(lds);                        // [4][32] maxima, [4][32] sums
     float* so = sm + 256;
     constexpr int LD = DP + 4;
+    l = half_sum(l);
     if (hi == 0) {
         sm[wave * 32 + l31] = m;
         sm[128 + wave * 32 + l31] = l;
@@ -447,7 +535,7 @@ constexpr int larger(int a, int b) { return a > b ? a : b; }
 
 // first: the stacked prefix rows (may be none), second: the samples' own rows
 enum { MANY, FEW, MIXED };                                                                         // MIXED: many stacked rows, few own rows
-template <bool BF, int DP, int MODE> __global__ void __launch_bounds__(256, 2) k_ctx_attn(AttnArgs p, Deal first, Deal second) {
+template <bool BF, int DP, int MODE> __global__ void __launch_bounds__(256, MODE == MANY && DP == 64 ? 4 : 2) k_ctx_attn(AttnArgs p, Deal first, Deal second) {
     __shared__ __attribute__((aligned(16))) u16 lds[MODE == MANY ? lds_many(DP) : MODE == FEW ? lds_few(DP) : larger(lds_many(DP), lds_few(DP))];
     const bool one = (int)blockIdx.x < first.blocks;
     const Deal& w = one ? first : second;
@@ -667,10 +755,6 @@ struct BwdArgs {
     int xtiles, chunks, per_chunk;
 };
 
-template <bool BF> __device__ __forceinline__ float dot2(unsigned a, unsigned b, float acc) {
-    if constexpr (BF) return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, a), __builtin_bit_cast(b2, b), acc, false);
-    else return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, a), __builtin_bit_cast(h2, b), acc, false);
-}
 __device__ __forceinline__ unsigned max_abs2(unsigned m, unsigned w) {          // the larger magnitude of each half (fp16 bits order like integers)
     typedef unsigned short us2 __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(us2, m), __builtin_bit_cast(us2, w & 0x7fff7fffu)));
@@ -1069,7 +1153,10 @@ template <bool BF, int DP> void launch_bwd(BwdArgs p, const BwdPlan& s, bool wan
     }
 }
 
-bool row_strides_ok(const void* p, long long a, long long b, long long c) { return ((uintptr_t)p % 16) == 0 && a % 8 == 0 && b % 8 == 0 && c % 8 == 0; }
+// (sample, row, head) strides; a tile of 64 rows has to lie within 2^31 bytes
+bool row_strides_ok(const void* p, long long a, long long b, long long c) {
+    return ((uintptr_t)p % 16) == 0 && a % 8 == 0 && b % 8 == 0 && c % 8 == 0 && b >= 0 && b < (1ll << 24);
+}
 
 int check_sizes(const char* name, int dtype, int B, int Nq, int Np, int Nk, int H, int Hk, int d, float scale) {
     VS_REQUIRE(dtype == 1 || dtype == 2, "%s: dtype %d (1 fp16, 2 bf16)", name, dtype);
@@ -1103,7 +1190,7 @@ int vidseg_context_attention_fwd(const void* q, long long q_b, long long q_n, lo
     VS_REQUIRE(q && out && (Nk == 0 || (k && v)) && (Np == 0 || (k_prefix && v_prefix)), "context_attention: null operand");
     VS_REQUIRE(row_strides_ok(q, q_b, q_n, q_h) && row_strides_ok(out, 0, 0, 0) && (Nk == 0 || (row_strides_ok(k, k_b, k_n, k_h) && row_strides_ok(v, v_b, v_n, v_h))) &&
                    (Np == 0 || (row_strides_ok(k_prefix, 0, kp_n, kp_h) && row_strides_ok(v_prefix, 0, vp_n, vp_h))),
-               "context_attention: operands must be 16-byte aligned with strides that are multiples of 8 elements");
+               "context_attention: operands must be 16-byte aligned with strides that are multiples of 8 elements (rows below 2^24 apart)");
     VS_REQUIRE(!(causal && mask), "context_attention: a causal call takes no key mask");
     const Plan s = make_plan(B, Nq, Np, Nk, H, Hk);
     const long long total = (long long)B * Nq * H;
@@ -1149,7 +1236,7 @@ int vidseg_context_attention_bwd(const void* dout, long long g_b, long long g_n,
     VS_REQUIRE(dout && q && k && v && out && lse && dq && (!dk == !dv), "context_attention_bwd: null operand");
     VS_REQUIRE(row_strides_ok(dout, g_b, g_n, g_h) && row_strides_ok(q, q_b, q_n, q_h) && row_strides_ok(k, k_b, k_n, k_h) && row_strides_ok(v, v_b, v_n, v_h) &&
                    row_strides_ok(out, 0, 0, 0) && row_strides_ok(dq, 0, 0, 0) && row_strides_ok(dk, 0, 0, 0) && row_strides_ok(dv, 0, 0, 0),
-               "context_attention_bwd: operands must be 16-byte aligned with strides that are multiples of 8 elements");
+               "context_attention_bwd: operands must be 16-byte aligned with strides that are multiples of 8 elements (rows below 2^24 apart)");
     const BwdPlan s = make_bwd_plan(B, Bk, Nq, Nk, H, Hk, d);
     VS_REQUIRE((long long)s.ktiles * s.chunks * Bk * Hk < (1ll << 24), "context_attention_bwd: Nk=%d, Hk=%d are too many blocks", Nk, Hk);
     VS_REQUIRE(dk || !s.fused, "context_attention_bwd: up to 128 keys all three gradients come out of one pass");
