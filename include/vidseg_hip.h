@@ -398,22 +398,22 @@ int vidseg_groupnorm_act_bwd(const void* dy, long long dy_batch_stride, long lon
  * attends, as one softmax, to Np prefix keys that all samples share and to the sample's own keys 0 .. lens[b] - 1 (lens NULL: all Nk) for which
  * mask[b * mask_b + key] != 0 (mask NULL: all); causal: query i sees own keys up to lens[b] - Nq + i (no mask then).  Heads of width d (8..128, d % 8
  * == 0), query head h on key head h * Hk / H; element strides per sample, row and head (multiples of 8, rows below 2^24; 0 shares one sample), 16-byte aligned.
- * out [B][Nq][H][d]; lse (opt) fp32 [B][H][Nq].  A query without a key: out 0, lse -inf.  Keys that do not exist are not read for their value.
+ * out [B][Nq][H][d]; out_lo (opt): what the rounding of out left, same type; lse (opt) fp32 [B][H][Nq].  A query without a key: out 0, lse -inf.  Keys that do not exist are not read for their value.
  * scratch: vidseg_context_attention_scratch_kib(...) KiB (0: none; -1: sizes refused). */
 int vidseg_context_attention_scratch_kib(int B, int Nq, int Np, int Nk, int H, int Hk, int d);
 int vidseg_context_attention_fwd(const void* q, long long q_b, long long q_n, long long q_h, const void* k_prefix, long long kp_n, long long kp_h,
                                  const void* v_prefix, long long vp_n, long long vp_h, const void* k, long long k_b, long long k_n, long long k_h,
                                  const void* v, long long v_b, long long v_n, long long v_h, const int* lens, const void* mask, long long mask_b,
-                                 void* out, float* lse, int dtype, int B, int Nq, int Np, int Nk, int H, int Hk, int d, float scale, int causal,
+                                 void* out, void* out_lo, float* lse, int dtype, int B, int Nq, int Np, int Nk, int H, int Hk, int d, float scale, int causal,
                                  void* scratch, long long scratch_kib, vidseg_stream_t stream);
-/* its gradients (no prefix, not causal): out and lse as the forward call wrote them, dq [B][Nq][H][d], dk / dv [Bk][Nk][Hk][d] contiguous.  Bk = 1 < B: one sample of
+/* its gradients (no prefix, not causal): lse and, over 128 keys, out and out_lo as the forward call wrote them (NULL otherwise); dq [B][Nq][H][d], dk / dv [Bk][Nk][Hk][d] contiguous.  Bk = 1 < B: one sample of
  * k / v serves all (k_b = v_b = 0) and its gradients are summed over the batch.  dk = dv = NULL: dq alone (more than 128 keys only).  Sums in a fixed order, no atomics.
- * fp16: exact powers of two keep the intermediate gradients in range for |v| below 500.
+ * fp16: exact powers of two keep the intermediate gradients in range.
  * scratch: vidseg_context_attention_bwd_scratch_kib(...) KiB (-1: sizes refused). */
 int vidseg_context_attention_bwd_scratch_kib(int B, int Bk, int Nq, int Nk, int H, int Hk, int d);
 int vidseg_context_attention_bwd(const void* dout, long long g_b, long long g_n, long long g_h, const void* q, long long q_b, long long q_n, long long q_h,
                                  const void* k, long long k_b, long long k_n, long long k_h, const void* v, long long v_b, long long v_n,
-                                 long long v_h, const int* lens, const void* mask, long long mask_b, const void* out, const float* lse, void* dq, void* dk,
+                                 long long v_h, const int* lens, const void* mask, long long mask_b, const void* out, const void* out_lo, const float* lse, void* dq, void* dk,
                                  void* dv, int dtype, int B, int Bk, int Nq, int Nk, int H, int Hk, int d, float scale, void* scratch,
                                  long long scratch_kib, vidseg_stream_t stream);
 

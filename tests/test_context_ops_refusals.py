@@ -103,7 +103,7 @@ def test_context_attention_c_entry_refuses():
 
     def fwd(**k):
         a = dict(q=p, qb=192, qn=64, qh=64, kp=None, kpn=0, kph=0, vp=None, vpn=0, vph=0, k=p, kb=320, kn=64, kh=64, v=p, vb=320, vn=64, vh=64, lens=None,
-                 mask=None, mb=0, out=p, lse=None, dtype=1, B=1, Nq=3, Np=0, Nk=5, H=1, Hk=1, d=64, scale=0.125, causal=0, scratch=None, kib=0)
+                 mask=None, mb=0, out=p, lo=None, lse=None, dtype=1, B=1, Nq=3, Np=0, Nk=5, H=1, Hk=1, d=64, scale=0.125, causal=0, scratch=None, kib=0)
         a.update(k)
         return _lib.lib().vidseg_context_attention_fwd(*a.values(), None)
     for k in (dict(q=None), dict(out=None), dict(k=None), dict(Np=4), dict(dtype=0), dict(dtype=3), dict(B=0), dict(Nq=0), dict(Nk=-1), dict(H=3, Hk=2), dict(d=12), dict(d=136),

@@ -24,9 +24,9 @@ _P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
 _lib.register({
     "vidseg_groupnorm_act_fwd": [_P, _L, _L, _I, _I, _L, _I, _I, _P, _P, _F, _I, _I, _P, _P, _P, _P, _L, _P],
     "vidseg_context_attention_scratch_kib": [_I, _I, _I, _I, _I, _I, _I],
-    "vidseg_context_attention_fwd": [_P, _L, _L, _L] + [_P, _L, _L] * 2 + [_P, _L, _L, _L] * 2 + [_P, _P, _L, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _L, _P],
+    "vidseg_context_attention_fwd": [_P, _L, _L, _L] + [_P, _L, _L] * 2 + [_P, _L, _L, _L] * 2 + [_P, _P, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _L, _P],
     "vidseg_context_attention_bwd_scratch_kib": [_I, _I, _I, _I, _I, _I, _I],
-    "vidseg_context_attention_bwd": [_P, _L, _L, _L] * 4 + [_P, _P, _L, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _P, _L, _P],
+    "vidseg_context_attention_bwd": [_P, _L, _L, _L] * 4 + [_P, _P, _L, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _P, _L, _P],
     "vidseg_groupnorm_act_bwd": [_P, _L, _L, _P, _L, _L, _I, _I, _L, _I, _I, _P, _P, _P, _P, _I, _I, _P, _P, _P, _P, _L, _P],
 })
 
@@ -195,7 +195,7 @@ def _mask(key_mask):
     return key_mask.data_ptr(), key_mask.stride(0) if key_mask.shape[0] > 1 else 0
 
 
-def _context_attention(q, k_prefix, v_prefix, k, v, heads, kv_heads, d, k_lens, key_mask, scale, causal, want_lse):
+def _context_attention(q, k_prefix, v_prefix, k, v, heads, kv_heads, d, k_lens, key_mask, scale, causal, want_lse, out_lo=None):
     B, Nq = q.shape[:2]
     device = q.device
     out = torch.empty(q.shape, dtype=q.dtype, device=device)
@@ -216,7 +216,7 @@ def _context_attention(q, k_prefix, v_prefix, k, v, heads, kv_heads, d, k_lens, 
         own = (*ks, *vs)
     kib = _lib.lib().vidseg_context_attention_scratch_kib(B, Nq, Np, Nk, heads, kv_heads, d)
     scratch = torch.empty(kib * 256, dtype=F32, device=device) if kib > 0 else None
-    _launch(device, "vidseg_context_attention_fwd", qp, qb, qn, qh, *pre, *own, ptr(k_lens), *_mask(key_mask), out.data_ptr(), ptr(lse),
+    _launch(device, "vidseg_context_attention_fwd", qp, qb, qn, qh, *pre, *own, ptr(k_lens), *_mask(key_mask), out.data_ptr(), ptr(out_lo), ptr(lse),
             _DTYPE[q.dtype], B, Nq, Np, Nk, heads, kv_heads, d, scale, causal, ptr(scratch), max(kib, 0))
     return out, lse
 
@@ -224,8 +224,10 @@ def _context_attention(q, k_prefix, v_prefix, k, v, heads, kv_heads, d, k_lens, 
 class _CrossAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, heads, kv_heads, d, k_lens, key_mask, scale):
-        out, lse = _context_attention(q, None, None, k, v, heads, kv_heads, d, k_lens, key_mask, scale, 0, True)
-        ctx.save_for_backward(q, k, v, k_lens, key_mask, out, lse)
+        # over 128 keys the backward pass takes sum(do * o) from the saved result, to more bits than its type has; below, it has no use for it
+        left = torch.empty(q.shape, dtype=q.dtype, device=q.device) if k.shape[1] > 128 else None
+        out, lse = _context_attention(q, None, None, k, v, heads, kv_heads, d, k_lens, key_mask, scale, 0, True, left)
+        ctx.save_for_backward(q, k, v, k_lens, key_mask, None if left is None else out, left, lse)
         ctx.how = heads, kv_heads, d, scale
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
@@ -236,7 +238,7 @@ class _CrossAttention(torch.autograd.Function):
     def backward(ctx, dout, _):
         if dout is None:
             return (None,) * 9
-        q, k, v, k_lens, key_mask, out, lse = ctx.saved_tensors
+        q, k, v, k_lens, key_mask, out, left, lse = ctx.saved_tensors
         heads, kv_heads, d, scale = ctx.how
         device, dtype = q.device, q.dtype
         (B, Nq), (Bk, Nk) = q.shape[:2], k.shape[:2]
@@ -253,7 +255,7 @@ class _CrossAttention(torch.autograd.Function):
         v, *vs = _heads_of(v, d)
         kib = _lib.lib().vidseg_context_attention_bwd_scratch_kib(B, Bk, Nq, Nk, heads, kv_heads, d)
         scratch = torch.empty(kib * 256, dtype=F32, device=device) if kib > 0 else None
-        _launch(device, "vidseg_context_attention_bwd", *gs, *qs, *ks, *vs, ptr(k_lens), *_mask(key_mask), out.data_ptr(), lse.data_ptr(), dq.data_ptr(),
+        _launch(device, "vidseg_context_attention_bwd", *gs, *qs, *ks, *vs, ptr(k_lens), *_mask(key_mask), ptr(out), ptr(left), lse.data_ptr(), dq.data_ptr(),
                 ptr(dk), ptr(dv), _DTYPE[dtype], B, Bk, Nq, Nk, heads, kv_heads, d, scale, ptr(scratch), max(kib, 0))
         return dq, dk, dv, None, None, None, None, None, None
 
@@ -264,7 +266,7 @@ def cross_attention(q, k, v, heads, *, kv_heads=None, k_lens=None, key_mask=None
     Query head h reads key head h * kv_heads // heads.  One sample of k / v serves the whole batch.  A key exists if it lies below k_lens[b] (int32 [B] on the device)
     and key_mask[b or 0, key] (bool) is true; what k / v hold elsewhere, NaN included, reaches nothing, and a query without any key gets zeros.
     return_lse: also log(sum exp) of the scores, fp32 [B, heads, Nq] (-inf without a key).  Differentiable (once) in q, k and v, not through the
-    log-sum-exp; in fp16 the gradients hold for |v| below 500.  Gradients of one shared k / v are summed over the batch  (attention.py:286-364)."""
+    log-sum-exp.  Gradients of one shared k / v are summed over the batch  (attention.py:286-364)."""
     name = "cross_attention"
     d, kv_heads = _attention_shapes(name, q, heads, kv_heads, (("k", k, 1), ("v", v, 1)))
     B, sk = q.shape[0], k.shape

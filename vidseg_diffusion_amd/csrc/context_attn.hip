@@ -68,55 +68,28 @@ template <int DP> __device__ __forceinline__ u32x4 read_tr(const u16* t, int r0,
                                 __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(t + slot_at<DP>(r + 8, slot) + in))};
     return __builtin_bit_cast(u32x4, v);
 }
-// The same for all 32-column blocks of 16 rows at once.  Fetches into LDS may be under way into another buffer: the compiler would wait for them before every
-// transpose read it can see (it takes them for writes), so these are spelled out, with their own wait in the same statement.
-template <int DP> struct Turned {
-    unsigned at[2][DP / 32];                                          // byte addresses for rows 4 hi .. and 8 + 4 hi .. of a tile
-    __device__ __forceinline__ void init(const u16* t, int lane) {
-        const int r = 4 * (lane >> 5) + ((lane & 15) >> 2), in = (lane & 1) * 4;
-#pragma unroll
-        for (int n = 0; n < DP / 32; ++n) {
-            const int slot = n * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
-            at[0][n] = (unsigned)(unsigned long long)(lds4)(t + slot_at<DP>(r, slot) + in);
-            at[1][n] = (unsigned)(unsigned long long)(lds4)(t + slot_at<DP>(r + 8, slot) + in);
-        }
-    }
-    // rows R0 .. R0 + 15
-    template <int R0> __device__ __forceinline__ void read(u32x4 (&f)[DP / 32]) const {
-#if defined(__HIP_DEVICE_COMPILE__)
-        constexpr int IMM = R0 * DP * 2;
-        u32x2 a[DP / 32], b[DP / 32];
-        if constexpr (DP == 64)
-            asm volatile("ds_read_b64_tr_b16 %0, %4 offset:%8\n\tds_read_b64_tr_b16 %1, %5 offset:%8\n\tds_read_b64_tr_b16 %2, %6 offset:%8\n\t"
-                         "ds_read_b64_tr_b16 %3, %7 offset:%8\n\ts_waitcnt lgkmcnt(0)"
-                         : "=&v"(a[0]), "=&v"(b[0]), "=&v"(a[1]), "=&v"(b[1])
-                         : "v"(at[0][0]), "v"(at[1][0]), "v"(at[0][1]), "v"(at[1][1]), "n"(IMM)
-                         : "memory");
-        else if constexpr (DP == 96)
-            asm volatile("ds_read_b64_tr_b16 %0, %6 offset:%12\n\tds_read_b64_tr_b16 %1, %7 offset:%12\n\tds_read_b64_tr_b16 %2, %8 offset:%12\n\t"
-                         "ds_read_b64_tr_b16 %3, %9 offset:%12\n\tds_read_b64_tr_b16 %4, %10 offset:%12\n\tds_read_b64_tr_b16 %5, %11 offset:%12\n\ts_waitcnt lgkmcnt(0)"
-                         : "=&v"(a[0]), "=&v"(b[0]), "=&v"(a[1]), "=&v"(b[1]), "=&v"(a[2]), "=&v"(b[2])
-                         : "v"(at[0][0]), "v"(at[1][0]), "v"(at[0][1]), "v"(at[1][1]), "v"(at[0][2]), "v"(at[1][2]), "n"(IMM)
-                         : "memory");
-        else
-            asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%16\n\tds_read_b64_tr_b16 %1, %9 offset:%16\n\tds_read_b64_tr_b16 %2, %10 offset:%16\n\t"
-                         "ds_read_b64_tr_b16 %3, %11 offset:%16\n\tds_read_b64_tr_b16 %4, %12 offset:%16\n\tds_read_b64_tr_b16 %5, %13 offset:%16\n\t"
-                         "ds_read_b64_tr_b16 %6, %14 offset:%16\n\tds_read_b64_tr_b16 %7, %15 offset:%16\n\ts_waitcnt lgkmcnt(0)"
-                         : "=&v"(a[0]), "=&v"(b[0]), "=&v"(a[1]), "=&v"(b[1]), "=&v"(a[2]), "=&v"(b[2]), "=&v"(a[3]), "=&v"(b[3])
-                         : "v"(at[0][0]), "v"(at[1][0]), "v"(at[0][1]), "v"(at[1][1]), "v"(at[0][2]), "v"(at[1][2]),
-                           "v"(at[0][3]), "v"(at[1][3]), "n"(IMM)
-                         : "memory");
-#pragma unroll
-        for (int n = 0; n < DP / 32; ++n) f[n] = u32x4{a[n][0], a[n][1], b[n][0], b[n][1]};
-#endif
-    }
-};
 template <int DP> __device__ __forceinline__ u32x4 read_row(const u16* t, int r, int slot) { return *reinterpret_cast<const u32x4*>(t + slot_at<DP>(r, slot)); }
 
 // Fetching of tiles of 64 rows straight into LDS (16 bytes a lane, four waves): lane i of piece w + 4 j fills 16-byte place (w + 4 j) 64 + i of the tile, so it
 // asks for the slot that belongs there.  What does not exist is asked for beyond the buffer's end and arrives as zeros.
-typedef __attribute__((address_space(3))) void* lds_ptr;
+//
+// The fetch is spelled out: of one that it can see the compiler assumes that any LDS read might want its data and waits for it, the next tile's
+// fetches too.  It has no register result; landed() waits for it.  (s_nop 4: an SGPR that a vector instruction has just written, and M0, are settled;
+// nothing else in this file keeps a value in M0.)
 constexpr unsigned BEYOND = 0xF0000000u;
+struct Span {
+    u32x4 r;                   // buffer resource: address, no stride, 0xE0000000 bytes
+    __device__ __forceinline__ explicit Span(const u16* at) {
+        const unsigned long long a = (unsigned long long)at;
+        r = u32x4{(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)a), (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(a >> 32)) & 0xffffu, 0xE0000000u, 0x00020000u};
+    }
+    __device__ __forceinline__ void fetch(u16* lds, unsigned off, int step) const {
+#if defined(__HIP_DEVICE_COMPILE__)
+        const int m0 = __builtin_amdgcn_readfirstlane((int)(unsigned)(unsigned long long)lds);     // the low half of a generic LDS address is its offset
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(m0), "v"(off), "s"(r), "s"(step));
+#endif
+    }
+};
 template <int DP> struct Fetch {
     static constexpr int SL = DP / 8, N = 64 * SL / 256, M = 256 % SL ? N : 1;      // M = 1: a lane's places differ by whole rows that the swizzle does not see
     unsigned off[M];
@@ -130,25 +103,16 @@ template <int DP> struct Fetch {
     }
     // the tile at `at`; rows of it that exist: live
     __device__ __forceinline__ void tile(const u16* at, long long step, unsigned long long live, u16* lds, int tid, int wave) const {
-#if defined(__HIP_DEVICE_COMPILE__)                                    // (the host pass knows no 16-byte fetch)
-        const auto span = __builtin_amdgcn_make_buffer_rsrc(const_cast<u16*>(at), 0, (int)0xE0000000u, 0x00020000);
-        if (live == ~0ull) {
+        const Span span(at);
 #pragma unroll
-            for (int j = 0; j < N; ++j)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(span, (lds_ptr)(lds + (wave + 4 * j) * 512), 16, (int)off[M == 1 ? 0 : j], M == 1 ? j * (512 / SL) * (int)step : 0, 0, 0);
-        } else {
-#pragma unroll
-            for (int j = 0; j < N; ++j)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(span, (lds_ptr)(lds + (wave + 4 * j) * 512), 16, (live >> row(tid, j)) & 1 ? (int)off[M == 1 ? 0 : j] : (int)BEYOND,
-                                                         M == 1 ? j * (512 / SL) * (int)step : 0, 0, 0);
+        for (int j = 0; j < N; ++j) {
+            const unsigned o = off[M == 1 ? 0 : j];
+            span.fetch(lds + (wave + 4 * j) * 512, live == ~0ull || ((live >> row(tid, j)) & 1) ? o : BEYOND, M == 1 ? j * (512 / SL) * (int)step : 0);
         }
-#endif
     }
 };
-__device__ __forceinline__ void landed() {                             // this wave's fetches are in LDS; the barrier after it makes all of them visible
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-}
+// this wave's fetches and writes are in LDS; the barrier makes all of them visible
+__device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 struct AttnArgs {
     const u16 *q, *kp, *vp, *k, *v;
@@ -156,7 +120,7 @@ struct AttnArgs {
     const int* lens;
     const unsigned char* mask;
     long long mask_b;
-    u16* o;                    // [B][Nq][H][d]
+    u16 *o, *o_lo;             // [B][Nq][H][d]; o_lo (or null): what the rounding of o left, for the backward pass
     float* lse;                // [B][H][Nq] or null
     float *po, *pml;           // partial results: [part][B * Nq * H][d], [..][2] = (maximum in log2 units, sum)
     int B, Nq, Np, Nk, H, Hk, G, d, causal;
@@ -229,12 +193,21 @@ template <int DP> __device__ __forceinline__ void load_q(const AttnArgs& p, cons
 }
 
 // 32 columns n * 32 .. of one row out of its accumulator, times f, as 16-byte pieces: the lane halves hold the rows 4 hi .. of every
-// 8 channels, one exchange of two registers gives each half 8 neighbouring channels.  All lanes call it.
-template <bool BF> __device__ __forceinline__ void store_row(u16* row, const f32x16& a, float f, int n, int hi, int d, bool on) {
+// 8 channels, one exchange of two registers gives each half 8 neighbouring channels.  lo: what the rounding left.  All lanes call it.
+template <bool BF> __device__ __forceinline__ float value_of(unsigned x, int half) {
+    const unsigned short w = half ? x >> 16 : x & 0xffffu;
+    return BF ? __uint_as_float((unsigned)w << 16) : (float)__builtin_bit_cast(_Float16, w);
+}
+template <bool BF> __device__ __forceinline__ unsigned left2(float a, float b) {
+    const unsigned x = pack2<BF>(a, b);
+    return pack2<BF>(a - value_of<BF>(x, 0), b - value_of<BF>(x, 1));
+}
+template <bool BF, bool LEFT = false> __device__ __forceinline__ void store_row(u16* row, const f32x16& a, float f, int n, int hi, int d, bool on) {
+    auto two = [&](int r) __attribute__((always_inline)) { return LEFT ? left2<BF>(a[r] * f, a[r + 1] * f) : pack2<BF>(a[r] * f, a[r + 1] * f); };
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
-        const auto x = __builtin_amdgcn_permlane32_swap(pack2<BF>(a[8 * g] * f, a[8 * g + 1] * f), pack2<BF>(a[8 * g + 4] * f, a[8 * g + 5] * f), false, false);
-        const auto y = __builtin_amdgcn_permlane32_swap(pack2<BF>(a[8 * g + 2] * f, a[8 * g + 3] * f), pack2<BF>(a[8 * g + 6] * f, a[8 * g + 7] * f), false, false);
+        const auto x = __builtin_amdgcn_permlane32_swap(two(8 * g), two(8 * g + 4), false, false);
+        const auto y = __builtin_amdgcn_permlane32_swap(two(8 * g + 2), two(8 * g + 6), false, false);
         const int c = n * 32 + 16 * g + 8 * hi;
         if (on && c < d) *reinterpret_cast<u32x4*>(row + c) = u32x4{x[0], y[0], x[1], y[1]};
     }
@@ -245,7 +218,7 @@ template <bool BF> __device__ __forceinline__ void store_row(u16* row, const f32
 // the rescaling and the exchange between the lane halves are then done and the probabilities taken anew; otherwise the scores are touched once.
 template <bool BF, int ND> __device__ __forceinline__ void soften(const f32x16& s, float c, float& m, float& l, f32x16 (&acc)[ND], u32x4 (&fp)[2]) {
     float sum;
-    auto take = [&](float ref) {
+    auto take = [&](float ref) __attribute__((always_inline)) {
         float a[2] = {0.f, 0.f};
 #pragma unroll
         for (int r = 0; r < 16; r += 2) {
@@ -306,13 +279,11 @@ template <bool BF, int DP> __device__ __forceinline__ void many_rows(const AttnA
     const u16 *kown = p.k + at.b * p.k_b + at.hk * p.k_h, *vown = p.v + at.b * p.v_b + at.hk * p.v_h;
     const u16 *kpre = p.kp + at.hk * p.kp_h, *vpre = p.vp + at.hk * p.vp_h;
     const unsigned char* mrow = p.mask ? p.mask + at.b * p.mask_b : nullptr;
-    Turned<DP> turned;
-    turned.init(sV, lane);
     Fetch<DP> fk, fv;
     bool prefix = tb < T0;
     fk.init(tid, prefix ? p.kp_n : p.k_n, p.d);
     fv.init(tid, prefix ? p.vp_n : p.v_n, p.d);
-    auto fetch = [&](int t, int buf) {
+    auto fetch = [&](int t, int buf) __attribute__((always_inline)) {
         if (prefix && t >= T0) {
             prefix = false;
             fk.init(tid, p.k_n, p.d);
@@ -331,7 +302,7 @@ template <bool BF, int DP> __device__ __forceinline__ void many_rows(const AttnA
     for (int n = 0; n < ND; ++n) acc[n] = zero16();
     if (tb < te) fetch(tb, 0);
     landed();
-    auto work = [&](auto which, int t) {                              // the buffer is a constant of the code: every LDS address is one register and an immediate
+    auto work = [&](auto which, int t) __attribute__((always_inline)) {                              // the buffer is a constant of the code: every LDS address is one register and an immediate
         constexpr int buf = decltype(which)::value;
         const u16* tk = sK + buf * TILE;
         const unsigned long long now = live;
@@ -347,16 +318,14 @@ template <bool BF, int DP> __device__ __forceinline__ void many_rows(const AttnA
         if (now != ~0ull || edge)
 #pragma unroll
             for (int j = 0; j < 2; ++j) hide(s[j], (unsigned)(now >> (32 * j)), edge ? at.len - p.Nq + row.qi - k0 - 32 * j - 4 * hi : 1 << 30, hi);
-        auto half = [&](auto which_half) {
+        auto half = [&](auto which_half) __attribute__((always_inline)) {
             constexpr int j = decltype(which_half)::value;
-            u32x4 fp[2], fv[ND];
+            u32x4 fp[2];
             soften<BF, ND>(s[j], p.c, m, l, acc, fp);
-            turned.template read<buf * KT + j * 32>(fv);
 #pragma unroll
-            for (int n = 0; n < ND; ++n) acc[n] = mfma<BF>(fv[n], fp[0], acc[n]);
-            turned.template read<buf * KT + j * 32 + 16>(fv);
+            for (int e = 0; e < 2; ++e)
 #pragma unroll
-            for (int n = 0; n < ND; ++n) acc[n] = mfma<BF>(fv[n], fp[1], acc[n]);
+                for (int n = 0; n < ND; ++n) acc[n] = mfma<BF>(read_tr<DP>(sV + buf * TILE, j * 32 + e * 16, n * 32, lane), fp[e], acc[n]);
         };
         half(Const<0>{});
         half(Const<1>{});
@@ -374,6 +343,7 @@ template <bool BF, int DP> __device__ __forceinline__ void many_rows(const AttnA
     for (int n = 0; n < ND; ++n) {
         if (!p.po) {
             store_row<BF>(p.o + id * p.d, acc[n], inv, n, hi, p.d, row.on);
+            if (p.o_lo) store_row<BF, true>(p.o_lo + id * p.d, acc[n], inv, n, hi, p.d, row.on);
         } else if (row.on) {
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
@@ -407,8 +377,8 @@ template <bool BF, int DP> __device__ __forceinline__ void few_rows(const AttnAr
     const u16 *kown = p.k + at.b * p.k_b + at.hk * p.k_h, *vown = p.v + at.b * p.v_b + at.hk * p.v_h;
     const unsigned char* mrow = p.mask ? p.mask + at.b * p.mask_b : nullptr;
     // the tile's first key, number of keys in its segment and this lane's key; a tile's last runs may lie behind the segment
-    auto first = [&](int t) { return (t >= T0 ? t - T0 : t) * 128 + wave * 32; };
-    auto load_k = [&](int t) {
+    auto first = [&](int t) __attribute__((always_inline)) { return (t >= T0 ? t - T0 : t) * 128 + wave * 32; };
+    auto load_k = [&](int t) __attribute__((always_inline)) {
         const bool own = t >= T0;
         const int n = own ? len : w.np, kk = min(first(t) + l31, n - 1);
         const u16* kb = (own ? kown : p.kp + at.hk * p.kp_h) + kk * (own ? p.k_n : p.kp_n);
@@ -418,7 +388,7 @@ template <bool BF, int DP> __device__ __forceinline__ void few_rows(const AttnAr
             rk[s] = *reinterpret_cast<const u32x4*>(kb + (c < p.d ? c : 0));
         }
     };
-    auto load_v = [&](int t) {
+    auto load_v = [&](int t) __attribute__((always_inline)) {
         const bool own = t >= T0;
         const int n = own ? len : w.np, k0 = first(t);
         const u16* vb = own ? vown : p.vp + at.hk * p.vp_h;
@@ -521,7 +491,10 @@ template <bool BF, int DP> __device__ __forceinline__ void few_rows(const AttnAr
             for (int e = 0; e < 4; ++e) a[e] += f[i] * t[e];
         }
         if (p.po) *reinterpret_cast<f32x4*>(p.po + (part * total + id) * p.d + c) = a;
-        else *reinterpret_cast<u32x2*>(p.o + id * p.d + c) = u32x2{pack2<BF>(a[0] * inv, a[1] * inv), pack2<BF>(a[2] * inv, a[3] * inv)};
+        else {
+            *reinterpret_cast<u32x2*>(p.o + id * p.d + c) = u32x2{pack2<BF>(a[0] * inv, a[1] * inv), pack2<BF>(a[2] * inv, a[3] * inv)};
+            if (p.o_lo) *reinterpret_cast<u32x2*>(p.o_lo + id * p.d + c) = u32x2{left2<BF>(a[0] * inv, a[1] * inv), left2<BF>(a[2] * inv, a[3] * inv)};
+        }
     }
     if ((tid & 7) == 0) {
         if (p.po) *reinterpret_cast<f32x2*>(p.pml + (part * total + id) * 2) = f32x2{mm, ll};
@@ -535,7 +508,7 @@ constexpr int larger(int a, int b) { return a > b ? a : b; }
 
 // first: the stacked prefix rows (may be none), second: the samples' own rows
 enum { MANY, FEW, MIXED };                                                                         // MIXED: many stacked rows, few own rows
-template <bool BF, int DP, int MODE> __global__ void __launch_bounds__(256, MODE == MANY && DP == 64 ? 4 : 2) k_ctx_attn(AttnArgs p, Deal first, Deal second) {
+template <bool BF, int DP, int MODE> __global__ void __launch_bounds__(256, MODE == MANY && DP == 64 ? 3 : 2) k_ctx_attn(AttnArgs p, Deal first, Deal second) {
     __shared__ __attribute__((aligned(16))) u16 lds[MODE == MANY ? lds_many(DP) : MODE == FEW ? lds_few(DP) : larger(lds_many(DP), lds_few(DP))];
     const bool one = (int)blockIdx.x < first.blocks;
     const Deal& w = one ? first : second;
@@ -630,7 +603,7 @@ template <bool BF, int DP> __global__ void __launch_bounds__(256, DP == 64 ? 3 :
 
 // Joins the partial results of one row, a wave each: four groups of sixteen lanes take every fourth part, a lane eight channels
 template <bool BF> __global__ void __launch_bounds__(256) k_ctx_join(const float* __restrict__ po, const float* __restrict__ pml, int parts, long long total, int d,
-                                                                   int Nq, int H, u16* __restrict__ o, float* __restrict__ lse) {
+                                                                   int Nq, int H, u16* __restrict__ o, u16* __restrict__ o_lo, float* __restrict__ lse) {
     const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (id >= total) return;
     const int lane = threadIdx.x & 63, grp = lane >> 4, c = (lane & 15) * 8;
@@ -660,8 +633,12 @@ template <bool BF> __global__ void __launch_bounds__(256) k_ctx_join(const float
     }
     if (grp) return;
     const float inv = l > 0.f ? 1.0f / l : 0.f;
-    if (c < d)
-        *reinterpret_cast<u32x4*>(o + id * d + c) = u32x4{pack2<BF>(a[0] * inv, a[1] * inv), pack2<BF>(a[2] * inv, a[3] * inv), pack2<BF>(a[4] * inv, a[5] * inv), pack2<BF>(a[6] * inv, a[7] * inv)};
+    if (c < d) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) a[e] *= inv;
+        *reinterpret_cast<u32x4*>(o + id * d + c) = u32x4{pack2<BF>(a[0], a[1]), pack2<BF>(a[2], a[3]), pack2<BF>(a[4], a[5]), pack2<BF>(a[6], a[7])};
+        if (o_lo) *reinterpret_cast<u32x4*>(o_lo + id * d + c) = u32x4{left2<BF>(a[0], a[1]), left2<BF>(a[2], a[3]), left2<BF>(a[4], a[5]), left2<BF>(a[6], a[7])};
+    }
     if (lse && c == 0) {
         const long long bq = id / H;
         lse[((bq / Nq) * H + id % H) * Nq + bq % Nq] = (m + __builtin_amdgcn_logf(l)) * LN2;
@@ -730,18 +707,18 @@ template <bool BF, int DP> void launch_fwd(const AttnArgs& p, const Plan& s, hip
     else hipLaunchKernelGGL((k_ctx_attn<BF, DP, MIXED>), grid, dim3(256), 0, st, p, s.first, s.second);
     if (s.parts) {
         const long long total = (long long)p.B * p.Nq * p.H;
-        hipLaunchKernelGGL((k_ctx_join<BF>), dim3((unsigned)((total + 3) / 4)), dim3(256), 0, st, p.po, p.pml, s.parts, total, p.d, p.Nq, p.H, p.o, p.lse);
+        hipLaunchKernelGGL((k_ctx_join<BF>), dim3((unsigned)((total + 3) / 4)), dim3(256), 0, st, p.po, p.pml, s.parts, total, p.d, p.Nq, p.H, p.o, p.o_lo, p.lse);
     }
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------------
-// Backward.  With L = lse log2 e and D = sum_d do o of a row:  p = exp2(s c - L),  dp = do v^T,  ds = p (dp - D),
+// Backward.  With L = lse log2 e and D = sum_keys p dp of a row:  p = exp2(s c - L),  dp = do v^T,  ds = p (dp - D),
 //   dv = p^T do,   dk = scale ds^T q,   dq = scale ds k.
 // p and ds are rounded once to the storage type before they enter a product.  fp16 needs both kept away from its subnormals (p of a row over
-// 4096 keys is 2^-12, its ds smaller still): p is carried as 2^12 p, ds with a power of two that brings the largest |do| in sight to [1, 2) --
-// exact factors that leave in fp32 at the end.  |ds| 2^k <= d max|v| then, inside fp16 for |v| below 500.
+// 4096 keys is 2^-12, its ds smaller still): p is carried as 2^12 p, ds with a power of two that brings the largest |dp - D| in sight to about 1 --
+// exact factors that leave in fp32 at the end; accumulators are rescaled where the power changes.
 struct BwdArgs {
-    const u16 *q, *k, *v, *o, *go;
+    const u16 *q, *k, *v, *o, *o_lo, *go;
     long long q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h, g_b, g_n, g_h;
     const float* lse;
     float* delta;              // [B][H][Nq]: D, written by the dq kernel for the dk / dv kernel
@@ -755,49 +732,51 @@ struct BwdArgs {
     int xtiles, chunks, per_chunk;
 };
 
-__device__ __forceinline__ unsigned max_abs2(unsigned m, unsigned w) {          // the larger magnitude of each half (fp16 bits order like integers)
-    typedef unsigned short us2 __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(us2, m), __builtin_bit_cast(us2, w & 0x7fff7fffu)));
-}
-// 2^-floor(log2 a) of the larger half, 1 for zero
-__device__ __forceinline__ float scale_of(unsigned m) {
-    const unsigned h = max(m & 0xffffu, m >> 16);
-    const float a = (float)__builtin_bit_cast(_Float16, (unsigned short)h);
-    const unsigned e = __float_as_uint(a) >> 23;
-    return h ? __uint_as_float((254u - min(e, 253u)) << 23) : 1.0f;
-}
+constexpr float P_LOG2 = 12.f, P_BACK = 2.44140625e-4f;                         // fp16: p as 2^12 p
+// 2^-floor(log2 m), at most 2^60
+__device__ __forceinline__ float power_for(float m) { return __uint_as_float((254u - max(67u, min(__float_as_uint(m) >> 23, 253u))) << 23); }
 
-constexpr float P_LOG2 = 12.f;                                                   // fp16: p as 2^12 p
-
-// dq: a wave owns 32 rows as accumulator columns, the block's waves share key tiles of 64 (the forward kernel's arrangement)
-template <bool BF, int DP> __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) k_ctx_bwd_q(BwdArgs p) {
-    constexpr int KT = 64, SL = DP / 8, NST = KT * SL / 256, ND = DP / 32;
-    __shared__ __attribute__((aligned(16))) u16 sK[2][KT * DP], sV[2][KT * DP];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, hi = lane >> 5;
+// dq: a wave owns 32 rows as accumulator columns, the block's waves share key tiles of 64 (the forward kernel's arrangement); K serves as rows (scores)
+// and transposed (ds k).  D comes out of the saved result: o was rounded, o_lo holds what the rounding left.
+template <bool BF, int DP> __global__ void __launch_bounds__(256, DP == 64 ? 3 : 2) k_ctx_bwd_q(BwdArgs p) {
+    constexpr int KT = 64, ND = DP / 32, TILE = KT * DP;
+    __shared__ __attribute__((aligned(16))) u16 sK[2 * TILE], sV[2 * TILE];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, hi = lane >> 5;
     int y, xt;
     block_of(p.xtiles, y, xt);
     const int hk = y % p.Hk, b = y / p.Hk, rows = p.Nq * p.G;
+    const int len = p.lens ? max(0, min(p.lens[b], p.Nk)) : p.Nk, T = (len + KT - 1) / KT;
+    const u16 *kb = p.k + b * p.k_b + hk * p.k_h, *vb = p.v + b * p.v_b + hk * p.v_h;
+    const unsigned char* mk = p.mask ? p.mask + b * p.mask_b : nullptr;
+    Fetch<DP> fk, fv;
+    fk.init(tid, p.k_n, p.d);
+    fv.init(tid, p.v_n, p.d);
+    unsigned long long live = 0;
+    auto fetch = [&](int t, int buf) __attribute__((always_inline)) {
+        const int k0 = t * KT, n = len - k0;
+        live = n >= KT ? ~0ull : (1ull << n) - 1;
+        if (mk) live = __ballot(lane < n && mk[k0 + min(lane, n - 1)]);
+        fk.tile(kb + k0 * p.k_n, p.k_n, live, sK + buf * TILE, tid, wave);
+        fv.tile(vb + k0 * p.v_n, p.v_n, live, sV + buf * TILE, tid, wave);
+    };
+    if (T > 0) fetch(0, 0);
     const int r = xt * 128 + wave * 32 + l31;
     const bool on = r < rows;
     const int rr = min(r, rows - 1), qi = rr / p.G, h = hk * p.G + rr % p.G;
     const long long id = ((long long)b * p.Nq + qi) * p.H + h;
     u32x4 fq[DP / 16], fg[DP / 16];
     float D = 0.f;
-    unsigned amax = 0;
     {
-        const u16 *qp = p.q + b * p.q_b + qi * p.q_n + h * p.q_h, *gp = p.go + b * p.g_b + qi * p.g_n + h * p.g_h, *op = p.o + id * p.d;
+        const u16 *qp = p.q + b * p.q_b + qi * p.q_n + h * p.q_h, *gp = p.go + b * p.g_b + qi * p.g_n + h * p.g_h;
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s) {
             const int at = s * 16 + hi * 8, a = at < p.d ? at : 0;
             fq[s] = *reinterpret_cast<const u32x4*>(qp + a);
             fg[s] = *reinterpret_cast<const u32x4*>(gp + a);
-            const u32x4 fo = *reinterpret_cast<const u32x4*>(op + a);
+            const u32x4 fo = *reinterpret_cast<const u32x4*>(p.o + id * p.d + a), fl = *reinterpret_cast<const u32x4*>(p.o_lo + id * p.d + a);
             if (at >= p.d) fq[s] = fg[s] = u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                D = dot2<BF>(fg[s][e], fo[e], D);
-                if (!BF) amax = max_abs2(amax, fg[s][e]);
-            }
+            for (int e = 0; e < 4; ++e) D = dot2<BF>(fg[s][e], fl[e], dot2<BF>(fg[s][e], fo[e], D));
         }
     }
     D = half_sum(D);
@@ -805,120 +784,158 @@ template <bool BF, int DP> __global__ void __launch_bounds__(256, DP == 128 ? 1 
     const float lse = p.lse[bhq];
     const float L = lse == -INFINITY ? INFINITY : lse * LOG2E;                  // a row without a key: p = 0
     if (on && hi == 0) p.delta[bhq] = D;
-    float fs = 1.f, back = p.scale;
-    if (!BF) {
-        const auto t = __builtin_amdgcn_permlane32_swap(amax, amax, false, false);
-        fs = scale_of(max_abs2(t[0], t[1]));
-        back = p.scale / fs;
-    }
-    const int len = p.lens ? max(0, min(p.lens[b], p.Nk)) : p.Nk, T = (len + KT - 1) / KT;
-    const u16 *kb = p.k + b * p.k_b + hk * p.k_h, *vb = p.v + b * p.v_b + hk * p.v_h;
-    const unsigned char* mk = p.mask ? p.mask + b * p.mask_b : nullptr;
-    u32x4 rk[NST], rv[NST];
-    unsigned long long live = 0;
-    auto load_tile = [&](int t) {
-#pragma unroll
-        for (int i = 0; i < NST; ++i) {
-            const int id = tid + 256 * i, row = id / SL, slot = id % SL, key = t * KT + row, kk = min(key, len - 1);
-            const bool ok = key < len && slot * 8 < p.d && (!mk || mk[kk]);
-            const int at = slot * 8 < p.d ? slot * 8 : 0;
-            rk[i] = *reinterpret_cast<const u32x4*>(kb + kk * p.k_n + at);
-            rv[i] = *reinterpret_cast<const u32x4*>(vb + kk * p.v_n + at);
-            if (!ok) rk[i] = rv[i] = u32x4{0u, 0u, 0u, 0u};
-        }
-        const int key = t * KT + lane;
-        live = __ballot(key < len && (!mk || mk[min(key, len - 1)]));
-    };
-    auto store_tile = [&](int buf) {
-#pragma unroll
-        for (int i = 0; i < NST; ++i) {
-            const int id = tid + 256 * i;
-            *reinterpret_cast<u32x4*>(&sK[buf][slot_at<DP>(id / SL, id % SL)]) = rk[i];
-            *reinterpret_cast<u32x4*>(&sV[buf][slot_at<DP>(id / SL, id % SL)]) = rv[i];
-        }
-    };
+    float power = BF ? 1.f : 1.152921504606846976e18f;                          // this row's factor of ds
     f32x16 acc[ND];
 #pragma unroll
-    for (int n = 0; n < ND; ++n)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[n][e] = 0.f;
-    if (T > 0) {
-        load_tile(0);
-        store_tile(0);
-    }
-    __syncthreads();
-    for (int t = 0; t < T; ++t) {
-        const int buf = t & 1;
+    for (int n = 0; n < ND; ++n) acc[n] = zero16();
+    landed();
+    auto work = [&](auto which, int t) __attribute__((always_inline)) {
+        constexpr int buf = decltype(which)::value;
         const unsigned long long now = live;
-        if (t + 1 < T) load_tile(t + 1);
+        if (t + 1 < T) fetch(t + 1, buf ^ 1);
+        auto half = [&](auto which_half) __attribute__((always_inline)) {
+            constexpr int j = decltype(which_half)::value;
+            f32x16 s, z;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const unsigned keys = (unsigned)(now >> (32 * j));
-            if (keys == 0) continue;
-            f32x16 s, dp;
+            for (int e = 0; e < DP / 16; ++e) s = mfma<BF>(read_row<DP>(sK + buf * TILE, j * 32 + l31, e * 2 + hi), fq[e], e ? s : zero16());
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
+            for (int e = 0; e < DP / 16; ++e) z = mfma<BF>(read_row<DP>(sV + buf * TILE, j * 32 + l31, e * 2 + hi), fg[e], e ? z : zero16());
+            if (now != ~0ull) hide(s, (unsigned)(now >> (32 * j)), 1 << 30, hi);
 #pragma unroll
-            for (int e = 0; e < DP / 16; ++e) {
-                s = mfma<BF>(read_row<DP>(sK[buf], j * 32 + l31, e * 2 + hi), fq[e], s);
-                dp = mfma<BF>(read_row<DP>(sV[buf], j * 32 + l31, e * 2 + hi), fg[e], dp);
-            }
-            if (keys != ~0u) {
-                const unsigned bits = keys >> (4 * hi);
+            for (int e = 0; e < 16; ++e) z[e] -= D;
+            if (!BF) {
+                float m = fabsf(z[0]);
 #pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    if (!((bits >> ((e & 3) + 8 * (e >> 2))) & 1u)) s[e] = -INFINITY;
+                for (int e = 1; e < 16; ++e) m = fmaxf(m, fabsf(z[e]));
+                if (__builtin_expect(__any(m * power > 16384.f), 0)) {
+                    const float f = fminf(power, power_for(half_max(m)));      // both lane halves hold the same row
+#pragma unroll
+                    for (int n = 0; n < ND; ++n)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) acc[n][e] *= f / power;
+                    power = f;
+                }
             }
             u32x4 fd[2];
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
-                float a = __builtin_amdgcn_exp2f(fmaf(s[e], p.c, -L)) * (dp[e] - D), d = __builtin_amdgcn_exp2f(fmaf(s[e + 1], p.c, -L)) * (dp[e + 1] - D);
+                float x = __builtin_amdgcn_exp2f(fmaf(s[e], p.c, -L)) * z[e], w = __builtin_amdgcn_exp2f(fmaf(s[e + 1], p.c, -L)) * z[e + 1];
                 if (!BF) {
-                    a *= fs;
-                    d *= fs;
+                    x *= power;
+                    w *= power;
                 }
-                fd[e >> 3][(e >> 1) & 3] = pack2<BF>(a, d);
+                fd[e >> 3][(e >> 1) & 3] = pack2<BF>(x, w);
             }
 #pragma unroll
             for (int e = 0; e < 2; ++e)
 #pragma unroll
-                for (int n = 0; n < ND; ++n) acc[n] = mfma<BF>(read_tr<DP>(sK[buf], j * 32 + e * 16, n * 32, lane), fd[e], acc[n]);
-        }
-        if (t + 1 < T) store_tile(buf ^ 1);
-        __syncthreads();
+                for (int n = 0; n < ND; ++n) acc[n] = mfma<BF>(read_tr<DP>(sK + buf * TILE, j * 32 + e * 16, n * 32, lane), fd[e], acc[n]);
+        };
+        half(Const<0>{});
+        half(Const<1>{});
+        landed();
+    };
+    for (int t = 0; t < T; t += 2) {
+        work(Const<0>{}, t);
+        if (t + 1 < T) work(Const<1>{}, t + 1);
     }
+    const float back = p.scale / power;
 #pragma unroll
     for (int n = 0; n < ND; ++n) store_row<BF>(p.dq + id * p.d, acc[n], back, n, hi, p.d, on);
 }
 
-// dk and dv: a wave owns 32 keys as accumulator columns (K, V in registers), the block 128, and walks over tiles of 64 rows; the rows of all samples
-// where they share one context.  FUSED (at most 128 keys): the block holds every key of its rows, so dq comes out of the same pass -- ds goes
-// through LDS once more, each wave takes its share of the [64][d] tile of ds k -- and q, o and do are read once in all.
+// The 32 lanes of a half hold 32 keys of 16 rows (registers): the rows' sums over the lanes.  Registers are folded pairwise across 16-lane groups first, then
+// summed within them; lane i < 8 of a group ends with the sum of row register 2 i (+ 1 in the upper group).
+__device__ __forceinline__ float rows_sum(const f32x16& x, int lane) {
+    float a[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const auto w = __builtin_amdgcn_permlane16_swap(__float_as_uint(x[2 * i]), __float_as_uint(x[2 * i + 1]), false, false);
+        a[i] = __uint_as_float(w[0]) + __uint_as_float(w[1]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        a[i] += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(a[i]), 0x128, 0xf, 0xf, true));     // row_ror:8
+        a[i] += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(a[i]), 0x124, 0xf, 0xf, true));     // row_ror:4
+        a[i] += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(a[i]), 0x122, 0xf, 0xf, true));     // row_ror:2
+        a[i] += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(a[i]), 0x121, 0xf, 0xf, true));     // row_ror:1
+    }
+    float v = a[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) v = (lane & 7) == i ? a[i] : v;
+    return v;
+}
+
+// dk and dv: a wave owns 32 keys as accumulator columns (K, V in registers), the block 128, and walks over tiles of 64 queries of one head: the heads of the
+// group, and the samples where they share one context, one after the other.  FUSED (at most 128 keys): the block holds every key of its rows, so D is summed
+// here from the unrounded p dp (four partial sums a row through LDS) and dq comes out of the same pass -- ds goes through LDS once more, each wave takes
+// its share of the [64][d] tile of ds k -- and q and do are all that is read per row.
 template <bool BF, int DP, bool FUSED> __global__ void __launch_bounds__(256, DP == 64 ? 2 : 1) k_ctx_bwd_kv(BwdArgs p) {
-    constexpr int RT = 64, SLP = DP == 64 ? 8 : 16, NST = RT * SLP / 256, ND = DP / 32;
-    __shared__ __attribute__((aligned(16))) u16 sQ[2][RT * DP], sG[2][RT * DP], sK[FUSED ? 128 * DP : 8], sS[FUSED ? 128 * RT : 8];
-    __shared__ __attribute__((aligned(16))) float sL[2][RT], sD[2][RT];
-    __shared__ unsigned sM[2][4];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, hi = lane >> 5;
+    constexpr int RT = 64, ND = DP / 32, TILE = RT * DP;
+    __shared__ __attribute__((aligned(16))) u16 sQ[2 * TILE], sG[2 * TILE], sK[FUSED ? 128 * DP : 8], sS[FUSED ? 128 * RT : 8];
+    __shared__ __attribute__((aligned(16))) float sL[2][RT], sD[FUSED ? 4 : 2][RT], sM[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, hi = lane >> 5;
     int y, kt;
     block_of(p.xtiles, y, kt);
     const int chunk = y % p.chunks;
     y /= p.chunks;
     const int hk = y % p.Hk, bk = y / p.Hk;                                      // bk: sample of k and v
     const bool shared = p.Bk < p.B;
-    const int rows = p.Nq * p.G, tiles = (rows + RT - 1) / RT;
-    const long long all = (long long)tiles * (shared ? p.B : 1);
-    const long long t0 = (long long)chunk * p.per_chunk, t1 = t0 + p.per_chunk < all ? t0 + p.per_chunk : all;
+    const int tiles = (p.Nq + RT - 1) / RT;                                      // of one head
+    const long long all = (long long)tiles * p.G * (shared ? p.B : 1), t0 = (long long)chunk * p.per_chunk;
+    int count = (int)((t0 + p.per_chunk < all ? t0 + p.per_chunk : all) - t0);
     const int key = kt * 128 + wave * 32 + l31;
     const bool in = key < p.Nk;
     // a key that no sample of this block has is taken as zero, so nothing that lies there reaches a product
-    auto lives = [&](int b) { return in && (!p.lens || key < p.lens[b]) && (!p.mask || p.mask[b * p.mask_b + key]); };
+    auto lives = [&](int b) __attribute__((always_inline)) { return in && (!p.lens || key < p.lens[b]) && (!p.mask || p.mask[b * p.mask_b + key]); };
     bool any = false;
     if (shared) {
-        for (int b = 0; b < p.B; ++b) any |= lives(b);
+        for (int i = 0; i < p.B; ++i) any |= lives(i);
     } else {
         any = lives(bk);
     }
+    if (!FUSED && !__syncthreads_or(any)) count = 0;                             // all 128 keys are dead: their gradients are zero
+    struct At {                                                                  // a tile: sample, head of the group, first query
+        int b, g, i;
+    };
+    auto step = [&](At& x) __attribute__((always_inline)) {
+        if (++x.i == tiles) {
+            x.i = 0;
+            if (++x.g == p.G) {
+                x.g = 0;
+                ++x.b;
+            }
+        }
+    };
+    At now;
+    now.i = (int)(t0 % tiles);
+    now.g = (int)(t0 / tiles % p.G);
+    now.b = shared ? (int)(t0 / tiles / p.G) : bk;
+    At next = now;                                                               // the tile to be fetched next
+    Fetch<DP> fq, fg;
+    fq.init(tid, p.q_n, p.d);
+    fg.init(tid, p.g_n, p.d);
+    float rL = INFINITY, rD = 0.f;
+    auto fetch = [&](int buf) __attribute__((always_inline)) {
+        const int q0 = next.i * RT, n = p.Nq - q0, h = hk * p.G + next.g;
+        const unsigned long long live = n >= RT ? ~0ull : (1ull << n) - 1;
+        fq.tile(p.q + next.b * p.q_b + h * p.q_h + q0 * p.q_n, p.q_n, live, sQ + buf * TILE, tid, wave);
+        fg.tile(p.go + next.b * p.g_b + h * p.g_h + q0 * p.g_n, p.g_n, live, sG + buf * TILE, tid, wave);
+        if (tid < RT) {
+            const long long at = ((long long)next.b * p.H + h) * p.Nq + q0 + min(tid, n - 1);
+            const float lse = p.lse[at];
+            rL = tid >= n || lse == -INFINITY ? INFINITY : lse * LOG2E - (BF ? 0.f : P_LOG2);
+            if (!FUSED) rD = tid < n ? p.delta[at] : 0.f;
+        }
+        step(next);
+    };
+    auto settle = [&](int buf) __attribute__((always_inline)) {
+        if (tid < RT) {
+            sL[buf][tid] = rL;
+            if (!FUSED) sD[buf][tid] = rD;
+        }
+    };
+    if (count > 0) fetch(0);
     u32x4 fk[DP / 16], fv[DP / 16];
     {
         const int kk = in ? key : 0;
@@ -932,169 +949,172 @@ template <bool BF, int DP, bool FUSED> __global__ void __launch_bounds__(256, DP
             if (FUSED) *reinterpret_cast<u32x4*>(sK + slot_at<DP>(wave * 32 + l31, s * 2 + hi)) = fk[s];
         }
     }
-    u32x4 rq[NST], rg[NST];
-    float rL = INFINITY, rD = 0.f, rDf[NST];
-    unsigned rmax = 0;
-    const int slot = tid % SLP, trow = tid / SLP;
-    auto load_tile = [&](long long t) {
-        const int b = shared ? (int)(t / tiles) : bk, base = (int)(t % tiles) * RT;
-        rmax = 0;
-#pragma unroll
-        for (int i = 0; i < NST; ++i) {
-            const int r = base + trow + i * (256 / SLP), rr = min(r, rows - 1), qi = rr / p.G, h = hk * p.G + rr % p.G;
-            const bool ok = r < rows && slot * 8 < p.d;
-            const int at = slot * 8 < p.d ? slot * 8 : 0;
-            rq[i] = *reinterpret_cast<const u32x4*>(p.q + b * p.q_b + qi * p.q_n + h * p.q_h + at);
-            rg[i] = *reinterpret_cast<const u32x4*>(p.go + b * p.g_b + qi * p.g_n + h * p.g_h + at);
-            if (!ok) rq[i] = rg[i] = u32x4{0u, 0u, 0u, 0u};
-            if (FUSED) {
-                const u32x4 fo = *reinterpret_cast<const u32x4*>(p.o + (((long long)b * p.Nq + qi) * p.H + h) * p.d + at);
-                rDf[i] = 0.f;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) rDf[i] = dot2<BF>(rg[i][e], fo[e], rDf[i]);
-            }
-            if (!BF)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) rmax = max_abs2(rmax, rg[i][e]);
-        }
-        if (tid < RT) {
-            const int r = base + tid, rr = min(r, rows - 1);
-            const long long at = ((long long)b * p.H + hk * p.G + rr % p.G) * p.Nq + rr / p.G;
-            const float lse = p.lse[at];
-            rL = r >= rows || lse == -INFINITY ? INFINITY : lse * LOG2E - (BF ? 0.f : P_LOG2);
-            if (!FUSED) rD = r < rows ? p.delta[at] : 0.f;
-        }
-    };
-    auto store_tile = [&](int buf) {
-#pragma unroll
-        for (int i = 0; i < NST; ++i) {
-            const int r = trow + i * (256 / SLP);
-            if (DP != 96 || slot < DP / 8) {
-                *reinterpret_cast<u32x4*>(&sQ[buf][slot_at<DP>(r, slot)]) = rq[i];
-                *reinterpret_cast<u32x4*>(&sG[buf][slot_at<DP>(r, slot)]) = rg[i];
-            }
-            if (FUSED) {
-                float x = rDf[i];
-#pragma unroll
-                for (int o = SLP / 2; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
-                if (slot == 0) sD[buf][r] = x;
-            }
-        }
-        if (tid < RT) {
-            sL[buf][tid] = rL;
-            if (!FUSED) sD[buf][tid] = rD;
-        }
-        if (!BF) {
-            unsigned m = rmax;
-#pragma unroll
-            for (int o = 32; o > 0; o >>= 1) m = max_abs2(m, __shfl_xor(m, o, 64));
-            if (lane == 0) sM[buf][wave] = m;
-        }
-    };
+    bool live = shared ? lives(now.b) : any;
+    bool whole = (!FUSED && !shared) || __all(live);                             // one sample's own keys, not FUSED: a dead key spoils its own column alone, which is not stored
     f32x16 ak[ND], av[ND];
 #pragma unroll
-    for (int n = 0; n < ND; ++n)
+    for (int n = 0; n < ND; ++n) ak[n] = av[n] = zero16();
+    float power = BF ? 1.f : 1.152921504606846976e18f;                          // factor of ds in ak: of this key's column, FUSED: of the block
+    settle(0);
+    landed();
+
+    // s -> p (fp32), z = dp; the tile's rows i * 32 ..
+    auto scores = [&](int buf, int i, f32x16& s, f32x16& z) __attribute__((always_inline)) {
+        const u16 *tq = sQ + buf * TILE, *tg = sG + buf * TILE;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) ak[n][e] = av[n][e] = 0.f;
-    float run = BF ? 1.f : 1.152921504606846976e18f;                            // 2^60: any tile with a gradient in it lowers it
-    if (t0 < t1) {
-        load_tile(t0);
-        store_tile(0);
-    }
-    __syncthreads();
-    for (long long t = t0; t < t1; ++t) {
-        const int buf = (int)(t - t0) & 1;
-        const int b = shared ? (int)(t / tiles) : bk, base = (int)(t % tiles) * RT;
-        if (t + 1 < t1) load_tile(t + 1);
-        const bool live = lives(b), whole = __all(live);
-        float fs = 1.f;
-        if (!BF) {
-            unsigned m = max_abs2(max_abs2(sM[buf][0], sM[buf][1]), max_abs2(sM[buf][2], sM[buf][3]));
-            const float now = scale_of(m);
-            if (m && now < run) {
-                const float f = now / run;
+        for (int e = 0; e < DP / 16; ++e) s = mfma<BF>(read_row<DP>(tq, i * 32 + l31, e * 2 + hi), fk[e], e ? s : zero16());
 #pragma unroll
-                for (int n = 0; n < ND; ++n)
+        for (int e = 0; e < DP / 16; ++e) z = mfma<BF>(read_row<DP>(tg, i * 32 + l31, e * 2 + hi), fv[e], e ? z : zero16());
+        if (!whole)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) ak[n][e] *= f;
-                run = now;
-            }
-            fs = run * 2.44140625e-4f;                                          // 2^-12 takes p's factor out of ds
+            for (int e = 0; e < 16; ++e)
+                if (!live) s[e] = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const f32x4 L = *reinterpret_cast<const f32x4*>(&sL[buf][i * 32 + 2 * e + 4 * hi]);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) s[e + w] = __builtin_amdgcn_exp2f(fmaf(s[e + w], p.c, -L[w]));
         }
+    };
+    auto pack = [&](const f32x16& x, float f, u32x4 (&o)[2]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            f32x16 s, dp;
+        for (int e = 0; e < 16; e += 2) o[e >> 3][(e >> 1) & 3] = pack2<BF>(x[e] * f, x[e + 1] * f);
+    };
+    auto products = [&](int buf, int i, const u32x4 (&fp)[2], const u32x4 (&fd)[2]) __attribute__((always_inline)) {
+        const u16 *tq = sQ + buf * TILE, *tg = sG + buf * TILE;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
+        for (int e = 0; e < 2; ++e)
 #pragma unroll
-            for (int e = 0; e < DP / 16; ++e) {
-                s = mfma<BF>(read_row<DP>(sQ[buf], i * 32 + l31, e * 2 + hi), fk[e], s);
-                dp = mfma<BF>(read_row<DP>(sG[buf], i * 32 + l31, e * 2 + hi), fv[e], dp);
+            for (int n = 0; n < ND; ++n) {
+                av[n] = mfma<BF>(read_tr<DP>(tg, i * 32 + e * 16, n * 32, lane), fp[e], av[n]);
+                ak[n] = mfma<BF>(read_tr<DP>(tq, i * 32 + e * 16, n * 32, lane), fd[e], ak[n]);
             }
-            if (!whole)
+    };
+    auto move_power = [&](float f) __attribute__((always_inline)) {
+        const float by = f / power;
 #pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    if (!live) s[e] = -INFINITY;
-            u32x4 fp[2], fd[2];
+        for (int n = 0; n < ND; ++n)
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                const f32x4 L = *reinterpret_cast<const f32x4*>(&sL[buf][i * 32 + 2 * e + 4 * hi]), D = *reinterpret_cast<const f32x4*>(&sD[buf][i * 32 + 2 * e + 4 * hi]);
-                float x[4], z[4];
+            for (int e = 0; e < 16; ++e) ak[n][e] *= by;
+        power = f;
+    };
+    for (int t = 0; t < count; ++t) {
+        const int buf = t & 1;
+        const bool more = t + 1 < count;
+        if (more) fetch(buf ^ 1);
+        if constexpr (!FUSED) {
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    x[w] = __builtin_amdgcn_exp2f(fmaf(s[e + w], p.c, -L[w]));
-                    z[w] = x[w] * (dp[e + w] - D[w]);
-                    if (!BF) z[w] *= fs;
+            for (int i = 0; i < 2; ++i) {
+                f32x16 s, z;
+                scores(buf, i, s, z);
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const f32x4 D = *reinterpret_cast<const f32x4*>(&sD[buf][i * 32 + 2 * e + 4 * hi]);
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) z[e + w] -= D[w];
                 }
+                if (!BF) {
+                    float m = fabsf(z[0]);
 #pragma unroll
-                for (int w = 0; w < 4; w += 2) {
-                    fp[e >> 3][((e + w) >> 1) & 3] = pack2<BF>(x[w], x[w + 1]);
-                    fd[e >> 3][((e + w) >> 1) & 3] = pack2<BF>(z[w], z[w + 1]);
+                    for (int e = 1; e < 16; ++e) m = fmaxf(m, fabsf(z[e]));
+                    if (__builtin_expect(__any(m * power > 16384.f), 0)) move_power(fminf(power, power_for(half_max(m))));
                 }
-                if (FUSED)                                                      // [key][row]: rows i 32 + 2 e + 4 hi + 0..3
+                u32x4 fp[2], fd[2];
+                pack(s, 1.f, fp);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) z[e] *= s[e];
+                pack(z, BF ? 1.f : power * P_BACK, fd);
+                products(buf, i, fp, fd);
+            }
+            if (more) settle(buf ^ 1);
+            landed();
+        } else {
+            f32x16 s[2], z[2];
+            // D: this wave's keys' share of each row, p in its own scale
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                scores(buf, i, s[i], z[i]);
+                f32x16 x;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[e] = s[i][e] * z[i][e];
+                const float sum = rows_sum(x, lane) * (BF ? 1.f : P_BACK);
+                const int e = 2 * (lane & 7) + ((lane >> 4) & 1);
+                if ((lane & 15) < 8) sD[wave][i * 32 + (e & 3) + 8 * (e >> 2) + 4 * hi] = sum;
+            }
+            if (!BF) {
+                float m = 0.f;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) m = fmaxf(fmaxf(m, fabsf(z[0][e])), fabsf(z[1][e]));
+                m = wave_max_f32(m);
+                if (lane == 0) sM[wave] = m;
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");    // (the next tile's fetch stays under way)
+            if (!BF) {
+                const float m = fmaxf(fmaxf(sM[0], sM[1]), fmaxf(sM[2], sM[3]));  // |dp - D| <= 2 m
+                if (m > 0.f && power_for(m) != power) move_power(power_for(m));
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                u32x4 fp[2], fd[2];
+                pack(s[i], 1.f, fp);
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    f32x4 D = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) {
+                        const f32x4 w = *reinterpret_cast<const f32x4*>(&sD[v][i * 32 + 2 * e + 4 * hi]);
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) D[u] += w[u];
+                    }
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) z[i][e + w] = (z[i][e + w] - D[w]) * s[i][e + w];
+                }
+                pack(z[i], BF ? 1.f : power * P_BACK, fd);
+#pragma unroll
+                for (int e = 0; e < 16; e += 4)                                 // [key][row]: rows i 32 + 2 e + 4 hi + 0..3
                     *reinterpret_cast<u32x2*>(sS + slot_at<RT>(wave * 32 + l31, i * 4 + (e >> 2)) + 4 * hi) = u32x2{fd[e >> 3][(e >> 1) & 3], fd[e >> 3][((e >> 1) & 3) + 1]};
+                products(buf, i, fp, fd);
             }
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-#pragma unroll
-                for (int n = 0; n < ND; ++n) {
-                    av[n] = mfma<BF>(read_tr<DP>(sG[buf], i * 32 + e * 16, n * 32, lane), fp[e], av[n]);
-                    ak[n] = mfma<BF>(read_tr<DP>(sQ[buf], i * 32 + e * 16, n * 32, lane), fd[e], ak[n]);
-                }
-        }
-        if (t + 1 < t1) store_tile(buf ^ 1);
-        __syncthreads();
-        if constexpr (FUSED) {
-            const float back = p.scale / run;
+            if (more) settle(buf ^ 1);
+            landed();
+            const float to_dq = p.scale / power;
+            const int h = hk * p.G + now.g;
             for (int w = wave; w < 2 * ND; w += 4) {
                 const int i = w & 1, n = w >> 1;
-                f32x16 acc;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+                f32x16 acc = zero16();
 #pragma unroll
                 for (int e = 0; e < 8; ++e) acc = mfma<BF>(read_tr<DP>(sK, e * 16, n * 32, lane), read_tr<RT>(sS, e * 16, i * 32, lane), acc);
-                const int r = base + i * 32 + l31, rr = min(r, rows - 1);
-                const long long id = ((long long)b * p.Nq + rr / p.G) * p.H + hk * p.G + rr % p.G;
-                store_row<BF>(p.dq + id * p.d, acc, back, n, hi, p.d, r < rows);
+                const int qi = now.i * RT + i * 32 + l31;
+                const long long id = ((long long)now.b * p.Nq + min(qi, p.Nq - 1)) * p.H + h;
+                store_row<BF>(p.dq + id * p.d, acc, to_dq, n, hi, p.d, qi < p.Nq);
             }
-            __syncthreads();                                                    // sS is written again in the next round
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");    // sS and sD are written again in the next round
+        }
+        const int b = now.b;
+        step(now);
+        if (shared && more && now.b != b) {
+            live = lives(now.b);
+            whole = __all(live);
         }
     }
-    const float bk_ = p.scale / run, bv_ = BF ? 1.f : 2.44140625e-4f;
+    const float to_k = any ? p.scale / power : 0.f, to_v = any ? (BF ? 1.f : P_BACK) : 0.f;
+    if (!any)
+#pragma unroll
+        for (int n = 0; n < ND; ++n) ak[n] = av[n] = zero16();                   // (they may hold infinities)
     const long long at = (((long long)bk * p.Nk + (in ? key : 0)) * p.Hk + hk) * p.d, plane = (long long)p.Bk * p.Nk * p.Hk * p.d;
 #pragma unroll
     for (int n = 0; n < ND; ++n) {
         if (!p.part) {
-            store_row<BF>(p.dk + at, ak[n], bk_, n, hi, p.d, in);
-            store_row<BF>(p.dv + at, av[n], bv_, n, hi, p.d, in);
+            store_row<BF>(p.dk + at, ak[n], to_k, n, hi, p.d, in);
+            store_row<BF>(p.dv + at, av[n], to_v, n, hi, p.d, in);
         } else if (in) {
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
                 const int c = n * 32 + 2 * e + 4 * hi;
                 if (c >= p.d) continue;
                 float* o = p.part + 2 * chunk * plane + at + c;
-                *reinterpret_cast<f32x4*>(o) = f32x4{ak[n][e] * bk_, ak[n][e + 1] * bk_, ak[n][e + 2] * bk_, ak[n][e + 3] * bk_};
-                *reinterpret_cast<f32x4*>(o + plane) = f32x4{av[n][e] * bv_, av[n][e + 1] * bv_, av[n][e + 2] * bv_, av[n][e + 3] * bv_};
+                *reinterpret_cast<f32x4*>(o) = f32x4{ak[n][e] * to_k, ak[n][e + 1] * to_k, ak[n][e + 2] * to_k, ak[n][e + 3] * to_k};
+                *reinterpret_cast<f32x4*>(o + plane) = f32x4{av[n][e] * to_v, av[n][e + 1] * to_v, av[n][e + 2] * to_v, av[n][e + 3] * to_v};
             }
         }
     }
@@ -1124,7 +1144,7 @@ BwdPlan make_bwd_plan(int B, int Bk, int Nq, int Nk, int H, int Hk, int d) {
     BwdPlan s{};
     s.fused = Nk <= 128;
     s.ktiles = (Nk + 127) / 128;
-    const long long tiles = ((long long)Nq * (H / Hk) + 63) / 64 * (Bk < B ? B : 1), blocks = (long long)Bk * Hk * s.ktiles;
+    const long long tiles = ((long long)Nq + 63) / 64 * (H / Hk) * (Bk < B ? B : 1), blocks = (long long)Bk * Hk * s.ktiles;
     const long long want = blocks >= 384 ? 1 : (512 + blocks - 1) / blocks;      // about two blocks a CU, at least two tiles each
     long long per = (tiles + want - 1) / want;
     if (per < 2) per = 2;
@@ -1183,12 +1203,12 @@ int vidseg_context_attention_scratch_kib(int B, int Nq, int Np, int Nk, int H, i
 int vidseg_context_attention_fwd(const void* q, long long q_b, long long q_n, long long q_h, const void* k_prefix, long long kp_n, long long kp_h,
                                  const void* v_prefix, long long vp_n, long long vp_h, const void* k, long long k_b, long long k_n, long long k_h,
                                  const void* v, long long v_b, long long v_n, long long v_h, const int* lens, const void* mask, long long mask_b,
-                                 void* out, float* lse, int dtype, int B, int Nq, int Np, int Nk, int H, int Hk, int d, float scale, int causal,
+                                 void* out, void* out_lo, float* lse, int dtype, int B, int Nq, int Np, int Nk, int H, int Hk, int d, float scale, int causal,
                                  void* scratch, long long scratch_kib, hipStream_t st) {
     const int rc = check_sizes("context_attention", dtype, B, Nq, Np, Nk, H, Hk, d, scale);
     if (rc) return rc;
     VS_REQUIRE(q && out && (Nk == 0 || (k && v)) && (Np == 0 || (k_prefix && v_prefix)), "context_attention: null operand");
-    VS_REQUIRE(row_strides_ok(q, q_b, q_n, q_h) && row_strides_ok(out, 0, 0, 0) && (Nk == 0 || (row_strides_ok(k, k_b, k_n, k_h) && row_strides_ok(v, v_b, v_n, v_h))) &&
+    VS_REQUIRE(row_strides_ok(q, q_b, q_n, q_h) && row_strides_ok(out, 0, 0, 0) && row_strides_ok(out_lo, 0, 0, 0) && (Nk == 0 || (row_strides_ok(k, k_b, k_n, k_h) && row_strides_ok(v, v_b, v_n, v_h))) &&
                    (Np == 0 || (row_strides_ok(k_prefix, 0, kp_n, kp_h) && row_strides_ok(v_prefix, 0, vp_n, vp_h))),
                "context_attention: operands must be 16-byte aligned with strides that are multiples of 8 elements (rows below 2^24 apart)");
     VS_REQUIRE(!(causal && mask), "context_attention: a causal call takes no key mask");
@@ -1200,7 +1220,7 @@ int vidseg_context_attention_fwd(const void* q, long long q_b, long long q_n, lo
     p.q = (const u16*)q; p.q_b = q_b; p.q_n = q_n; p.q_h = q_h;
     p.kp = (const u16*)k_prefix; p.kp_n = kp_n; p.kp_h = kp_h; p.vp = (const u16*)v_prefix; p.vp_n = vp_n; p.vp_h = vp_h;
     p.k = (const u16*)k; p.k_b = k_b; p.k_n = k_n; p.k_h = k_h; p.v = (const u16*)v; p.v_b = v_b; p.v_n = v_n; p.v_h = v_h;
-    p.lens = lens; p.mask = (const unsigned char*)mask; p.mask_b = mask_b; p.o = (u16*)out; p.lse = lse;
+    p.lens = lens; p.mask = (const unsigned char*)mask; p.mask_b = mask_b; p.o = (u16*)out; p.o_lo = (u16*)out_lo; p.lse = lse;
     p.B = B; p.Nq = Nq; p.Np = Np; p.Nk = Nk; p.H = H; p.Hk = Hk; p.G = H / Hk; p.d = d; p.causal = causal; p.c = scale * LOG2E;
     if (s.parts) {
         p.po = (float*)scratch;
@@ -1227,25 +1247,26 @@ int vidseg_context_attention_bwd_scratch_kib(int B, int Bk, int Nq, int Nk, int 
 
 int vidseg_context_attention_bwd(const void* dout, long long g_b, long long g_n, long long g_h, const void* q, long long q_b, long long q_n, long long q_h,
                                  const void* k, long long k_b, long long k_n, long long k_h, const void* v, long long v_b, long long v_n,
-                                 long long v_h, const int* lens, const void* mask, long long mask_b, const void* out, const float* lse, void* dq, void* dk,
+                                 long long v_h, const int* lens, const void* mask, long long mask_b, const void* out, const void* out_lo, const float* lse, void* dq, void* dk,
                                  void* dv, int dtype, int B, int Bk, int Nq, int Nk, int H, int Hk, int d, float scale, void* scratch,
                                  long long scratch_kib, hipStream_t st) {
     const int rc = check_sizes("context_attention_bwd", dtype, B, Nq, 0, Nk, H, Hk, d, scale);
     if (rc) return rc;
     VS_REQUIRE(Nk >= 1 && (Bk == 1 || Bk == B), "context_attention_bwd: Nk=%d, %d samples of k for %d", Nk, Bk, B);
-    VS_REQUIRE(dout && q && k && v && out && lse && dq && (!dk == !dv), "context_attention_bwd: null operand");
+    VS_REQUIRE(dout && q && k && v && lse && dq && (!dk == !dv), "context_attention_bwd: null operand");
     VS_REQUIRE(row_strides_ok(dout, g_b, g_n, g_h) && row_strides_ok(q, q_b, q_n, q_h) && row_strides_ok(k, k_b, k_n, k_h) && row_strides_ok(v, v_b, v_n, v_h) &&
-                   row_strides_ok(out, 0, 0, 0) && row_strides_ok(dq, 0, 0, 0) && row_strides_ok(dk, 0, 0, 0) && row_strides_ok(dv, 0, 0, 0),
+                   row_strides_ok(out, 0, 0, 0) && row_strides_ok(out_lo, 0, 0, 0) && row_strides_ok(dq, 0, 0, 0) && row_strides_ok(dk, 0, 0, 0) && row_strides_ok(dv, 0, 0, 0),
                "context_attention_bwd: operands must be 16-byte aligned with strides that are multiples of 8 elements (rows below 2^24 apart)");
     const BwdPlan s = make_bwd_plan(B, Bk, Nq, Nk, H, Hk, d);
     VS_REQUIRE((long long)s.ktiles * s.chunks * Bk * Hk < (1ll << 24), "context_attention_bwd: Nk=%d, Hk=%d are too many blocks", Nk, Hk);
+    VS_REQUIRE(s.fused || (out && out_lo), "context_attention_bwd: null operand (over 128 keys the forward result and what its rounding left are needed)");
     VS_REQUIRE(dk || !s.fused, "context_attention_bwd: up to 128 keys all three gradients come out of one pass");
     const long long need = ((s.delta_floats + s.part_floats) * 4 + 1023) / 1024;
     VS_REQUIRE(need == 0 || (scratch && scratch_kib >= need), "context_attention_bwd: scratch of %lld KiB, needs %lld", scratch_kib, need);
     BwdArgs p{};
     p.q = (const u16*)q; p.q_b = q_b; p.q_n = q_n; p.q_h = q_h; p.k = (const u16*)k; p.k_b = k_b; p.k_n = k_n; p.k_h = k_h;
     p.v = (const u16*)v; p.v_b = v_b; p.v_n = v_n; p.v_h = v_h; p.go = (const u16*)dout; p.g_b = g_b; p.g_n = g_n; p.g_h = g_h;
-    p.o = (const u16*)out; p.lse = lse; p.delta = (float*)scratch; p.lens = lens; p.mask = (const unsigned char*)mask; p.mask_b = mask_b;
+    p.o = (const u16*)out; p.o_lo = (const u16*)out_lo; p.lse = lse; p.delta = (float*)scratch; p.lens = lens; p.mask = (const unsigned char*)mask; p.mask_b = mask_b;
     p.dq = (u16*)dq; p.dk = (u16*)dk; p.dv = (u16*)dv; p.part = s.part_floats ? (float*)scratch + s.delta_floats : nullptr;
     p.B = B; p.Bk = Bk; p.Nq = Nq; p.Nk = Nk; p.H = H; p.Hk = Hk; p.G = H / Hk; p.d = d; p.c = scale * LOG2E; p.scale = scale;
     p.chunks = s.chunks; p.per_chunk = s.per_chunk;
