@@ -870,13 +870,18 @@ __device__ __forceinline__ float rows_sum(const f32x16& x, int lane) {
 // group, and the samples where they share one context, one after the other.  FUSED (at most 128 keys): the block holds every key of its rows, so D is summed
 // here from the unrounded p dp (four partial sums a row through LDS) and dq comes out of the same pass -- ds goes through LDS once more, each wave takes
 // its share of the [64][d] tile of ds k -- and q and do are all that is read per row.
-template <bool BF, int DP, bool FUSED> __global__ void __launch_bounds__(256, DP == 64 ? 2 : 1) k_ctx_bwd_kv(BwdArgs p) {
+// DV, DK: which of the two the block accumulates.
+template <int DP, bool FUSED> struct BwdLds {
+    __attribute__((aligned(16))) u16 q[2 * 64 * DP], g[2 * 64 * DP], k[FUSED ? 128 * DP : 8], s[FUSED ? 128 * 64 : 8];
+    __attribute__((aligned(16))) float l[2][64], d[FUSED ? 4 : 2][64], m[4];
+};
+template <bool BF, int DP, bool FUSED, bool DV, bool DK> __device__ __forceinline__ void keys_walk(const BwdArgs& p, int y, int kt, BwdLds<DP, FUSED>& lds) {
     constexpr int RT = 64, ND = DP / 32, TILE = RT * DP;
-    __shared__ __attribute__((aligned(16))) u16 sQ[2 * TILE], sG[2 * TILE], sK[FUSED ? 128 * DP : 8], sS[FUSED ? 128 * RT : 8];
-    __shared__ __attribute__((aligned(16))) float sL[2][RT], sD[FUSED ? 4 : 2][RT], sM[4];
+    u16 *sQ = lds.q, *sG = lds.g, *sK = lds.k, *sS = lds.s;
+    float(*sL)[64] = lds.l;
+    float(*sD)[64] = lds.d;
+    float* sM = lds.m;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, hi = lane >> 5;
-    int y, kt;
-    block_of(p.xtiles, y, kt);
     const int chunk = y % p.chunks;
     y /= p.chunks;
     const int hk = y % p.Hk, bk = y / p.Hk;                                      // bk: sample of k and v
@@ -944,7 +949,7 @@ template <bool BF, int DP, bool FUSED> __global__ void __launch_bounds__(256, DP
         for (int s = 0; s < DP / 16; ++s) {
             const int at = s * 16 + hi * 8, a = at < p.d ? at : 0;
             fk[s] = *reinterpret_cast<const u32x4*>(kp + a);
-            fv[s] = *reinterpret_cast<const u32x4*>(vp + a);
+            if (DK) fv[s] = *reinterpret_cast<const u32x4*>(vp + a);
             if (at >= p.d || !any) fk[s] = fv[s] = u32x4{0u, 0u, 0u, 0u};
             if (FUSED) *reinterpret_cast<u32x4*>(sK + slot_at<DP>(wave * 32 + l31, s * 2 + hi)) = fk[s];
         }
@@ -963,8 +968,9 @@ template <bool BF, int DP, bool FUSED> __global__ void __launch_bounds__(256, DP
         const u16 *tq = sQ + buf * TILE, *tg = sG + buf * TILE;
 #pragma unroll
         for (int e = 0; e < DP / 16; ++e) s = mfma<BF>(read_row<DP>(tq, i * 32 + l31, e * 2 + hi), fk[e], e ? s : zero16());
+        if (DK)
 #pragma unroll
-        for (int e = 0; e < DP / 16; ++e) z = mfma<BF>(read_row<DP>(tg, i * 32 + l31, e * 2 + hi), fv[e], e ? z : zero16());
+            for (int e = 0; e < DP / 16; ++e) z = mfma<BF>(read_row<DP>(tg, i * 32 + l31, e * 2 + hi), fv[e], e ? z : zero16());
         if (!whole)
 #pragma unroll
             for (int e = 0; e < 16; ++e)
@@ -986,8 +992,8 @@ template <bool BF, int DP, bool FUSED> __global__ void __launch_bounds__(256, DP
         for (int e = 0; e < 2; ++e)
 #pragma unroll
             for (int n = 0; n < ND; ++n) {
-                av[n] = mfma<BF>(read_tr<DP>(tg, i * 32 + e * 16, n * 32, lane), fp[e], av[n]);
-                ak[n] = mfma<BF>(read_tr<DP>(tq, i * 32 + e * 16, n * 32, lane), fd[e], ak[n]);
+                if (DV) av[n] = mfma<BF>(read_tr<DP>(tg, i * 32 + e * 16, n * 32, lane), fp[e], av[n]);
+                if (DK) ak[n] = mfma<BF>(read_tr<DP>(tq, i * 32 + e * 16, n * 32, lane), fd[e], ak[n]);
             }
     };
     auto move_power = [&](float f) __attribute__((always_inline)) {
@@ -1007,23 +1013,25 @@ template <bool BF, int DP, bool FUSED> __global__ void __launch_bounds__(256, DP
             for (int i = 0; i < 2; ++i) {
                 f32x16 s, z;
                 scores(buf, i, s, z);
-#pragma unroll
-                for (int e = 0; e < 16; e += 4) {
-                    const f32x4 D = *reinterpret_cast<const f32x4*>(&sD[buf][i * 32 + 2 * e + 4 * hi]);
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) z[e + w] -= D[w];
-                }
-                if (!BF) {
-                    float m = fabsf(z[0]);
-#pragma unroll
-                    for (int e = 1; e < 16; ++e) m = fmaxf(m, fabsf(z[e]));
-                    if (__builtin_expect(__any(m * power > 16384.f), 0)) move_power(fminf(power, power_for(half_max(m))));
-                }
                 u32x4 fp[2], fd[2];
-                pack(s, 1.f, fp);
+                if (DV) pack(s, 1.f, fp);
+                if (DK) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) z[e] *= s[e];
-                pack(z, BF ? 1.f : power * P_BACK, fd);
+                    for (int e = 0; e < 16; e += 4) {
+                        const f32x4 D = *reinterpret_cast<const f32x4*>(&sD[buf][i * 32 + 2 * e + 4 * hi]);
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) z[e + w] -= D[w];
+                    }
+                    if (!BF) {
+                        float m = fabsf(z[0]);
+#pragma unroll
+                        for (int e = 1; e < 16; ++e) m = fmaxf(m, fabsf(z[e]));
+                        if (__builtin_expect(__any(m * power > 16384.f), 0)) move_power(fminf(power, power_for(half_max(m))));
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) z[e] *= s[e];
+                    pack(z, BF ? 1.f : power * P_BACK, fd);
+                }
                 products(buf, i, fp, fd);
             }
             if (more) settle(buf ^ 1);
@@ -1105,18 +1113,32 @@ template <bool BF, int DP, bool FUSED> __global__ void __launch_bounds__(256, DP
 #pragma unroll
     for (int n = 0; n < ND; ++n) {
         if (!p.part) {
-            store_row<BF>(p.dk + at, ak[n], to_k, n, hi, p.d, in);
-            store_row<BF>(p.dv + at, av[n], to_v, n, hi, p.d, in);
+            if (DK) store_row<BF>(p.dk + at, ak[n], to_k, n, hi, p.d, in);
+            if (DV) store_row<BF>(p.dv + at, av[n], to_v, n, hi, p.d, in);
         } else if (in) {
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
                 const int c = n * 32 + 2 * e + 4 * hi;
                 if (c >= p.d) continue;
                 float* o = p.part + 2 * chunk * plane + at + c;
-                *reinterpret_cast<f32x4*>(o) = f32x4{ak[n][e] * to_k, ak[n][e + 1] * to_k, ak[n][e + 2] * to_k, ak[n][e + 3] * to_k};
-                *reinterpret_cast<f32x4*>(o + plane) = f32x4{av[n][e] * to_v, av[n][e + 1] * to_v, av[n][e + 2] * to_v, av[n][e + 3] * to_v};
+                if (DK) *reinterpret_cast<f32x4*>(o) = f32x4{ak[n][e] * to_k, ak[n][e + 1] * to_k, ak[n][e + 2] * to_k, ak[n][e + 3] * to_k};
+                if (DV) *reinterpret_cast<f32x4*>(o + plane) = f32x4{av[n][e] * to_v, av[n][e + 1] * to_v, av[n][e + 2] * to_v, av[n][e + 3] * to_v};
             }
         }
+    }
+}
+
+// Wide heads, not FUSED: the accumulators of both gradients and K, V leave room for one wave a SIMD only, which waits more than it works; so half of the
+// blocks take dk and the other half dv (five products for four, at two waves a SIMD).
+template <bool BF, int DP, bool FUSED> __global__ void __launch_bounds__(256, DP == 64 || !FUSED ? 2 : 1) k_ctx_bwd_kv(BwdArgs p) {
+    __shared__ BwdLds<DP, FUSED> lds;
+    int y, kt;
+    block_of(p.xtiles, y, kt);
+    if constexpr (FUSED || DP == 64) {
+        keys_walk<BF, DP, FUSED, true, true>(p, y, kt, lds);
+    } else {
+        if (kt & 1) keys_walk<BF, DP, FUSED, true, false>(p, y, kt >> 1, lds);
+        else keys_walk<BF, DP, FUSED, false, true>(p, y, kt >> 1, lds);
     }
 }
 
@@ -1164,8 +1186,9 @@ template <bool BF, int DP> void launch_bwd(BwdArgs p, const BwdPlan& s, bool wan
         p.xtiles = (p.Nq * p.G + 127) / 128;
         hipLaunchKernelGGL((k_ctx_bwd_q<BF, DP>), dim3((unsigned)(p.xtiles * (long long)p.B * p.Hk)), dim3(256), 0, st, p);
         if (!want_kv) return;
-        p.xtiles = s.ktiles;
-        hipLaunchKernelGGL((k_ctx_bwd_kv<BF, DP, false>), dim3(kv_blocks), dim3(256), 0, st, p);
+        constexpr int shares = DP == 64 ? 1 : 2;
+        p.xtiles = s.ktiles * shares;
+        hipLaunchKernelGGL((k_ctx_bwd_kv<BF, DP, false>), dim3(kv_blocks * shares), dim3(256), 0, st, p);
     }
     if (s.chunks > 1) {
         const long long plane = (long long)p.Bk * p.Nk * p.Hk * p.d;
@@ -1258,7 +1281,7 @@ int vidseg_context_attention_bwd(const void* dout, long long g_b, long long g_n,
                    row_strides_ok(out, 0, 0, 0) && row_strides_ok(out_lo, 0, 0, 0) && row_strides_ok(dq, 0, 0, 0) && row_strides_ok(dk, 0, 0, 0) && row_strides_ok(dv, 0, 0, 0),
                "context_attention_bwd: operands must be 16-byte aligned with strides that are multiples of 8 elements (rows below 2^24 apart)");
     const BwdPlan s = make_bwd_plan(B, Bk, Nq, Nk, H, Hk, d);
-    VS_REQUIRE((long long)s.ktiles * s.chunks * Bk * Hk < (1ll << 24), "context_attention_bwd: Nk=%d, Hk=%d are too many blocks", Nk, Hk);
+    VS_REQUIRE((long long)s.ktiles * s.chunks * Bk * Hk < (1ll << 23), "context_attention_bwd: Nk=%d, Hk=%d are too many blocks", Nk, Hk);
     VS_REQUIRE(s.fused || (out && out_lo), "context_attention_bwd: null operand (over 128 keys the forward result and what its rounding left are needed)");
     VS_REQUIRE(dk || !s.fused, "context_attention_bwd: up to 128 keys all three gradients come out of one pass");
     const long long need = ((s.delta_floats + s.part_floats) * 4 + 1023) / 1024;
