@@ -58,6 +58,11 @@ PREFIX = [  # B, Nq, Np, Nk, H, Hk, d, dtype, lens, causal
     (2, 50, 64, 0, 2, 2, 64, F16, None, False),                       # no own keys
     (1, 1, 5000, 3, 1, 1, 64, BF16, (3,), True),                      # one row, one long prefix
     (3, 40, 90, 64, 2, 2, 48, F16, (0, 64, 10), False),
+    (40, 2, 600, 20, 4, 2, 64, BF16, None, True),                     # stacked rows of many samples, few rows of their own
+    (64, 1, 1000, 40, 8, 2, 128, F16, None, True),
+    (3, 40, 700, 64, 2, 2, 48, F16, (0, 64, 10), False),              # stacked rows, and more than 32 of their own
+    (2, 1, 2600, 33, 4, 4, 80, BF16, (33, 2), True),                  # few rows in all, the prefix dealt out over blocks
+    (1, 1, 5000, 2100, 2, 2, 64, F16, (2050,), True),                 # one sample: prefix and own keys in one walk
 ]
 
 

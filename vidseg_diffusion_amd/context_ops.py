@@ -79,21 +79,18 @@ def _rows_of(x):
 
 def _groupnorm_act_fwd(x, gamma, beta, groups, eps, act, save):
     device = x.device
-    y = torch.empty(x.shape, dtype=x.dtype, device=device)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     x, B, HW, xb, xr = _rows_of(x)
     C = x.shape[-1]
     if B * HW == 0:
         return y, torch.zeros(2 * B * groups, dtype=F32, device=device)
     rows = norm_rows_per_chunk(HW, C)
     part = 2 * B * -(-HW // rows) * groups
-    stats, mean, rstd = None, None, None
-    if save:
-        stats = torch.empty(2 * B * groups, dtype=F32, device=device)           # means, then 1 / standard deviations
-        mean = stats.data_ptr()
-        rstd = mean + 4 * B * groups
-    scratch = torch.empty(part, dtype=F32, device=device)
+    stats = torch.empty(2 * B * groups + part, dtype=F32, device=device)        # means, 1 / standard deviations, scratch behind them
+    mean = stats.data_ptr()
+    rstd = mean + 4 * B * groups
     _launch(device, "vidseg_groupnorm_act_fwd", x.data_ptr(), xb, xr, _DTYPE[x.dtype], B, HW, C, groups, gamma.data_ptr(), beta.data_ptr(), eps, act,
-            rows, y.data_ptr(), mean, rstd, scratch.data_ptr(), part)
+            rows, y.data_ptr(), mean if save else None, rstd if save else None, rstd + 4 * B * groups, part)
     return y, stats
 
 
@@ -111,7 +108,7 @@ class _GroupNormAct(torch.autograd.Function):
         x, gamma, beta, stats = ctx.saved_tensors
         G, act = ctx.how
         device = x.device
-        dx = torch.empty(x.shape, dtype=x.dtype, device=device)
+        dx = torch.empty_like(x, memory_format=torch.contiguous_format)
         x, B, HW, xb, xr = _rows_of(x)
         dy, _, _, db, dr = _rows_of(dy)
         C = x.shape[-1]
@@ -198,7 +195,7 @@ def _mask(key_mask):
 def _context_attention(q, k_prefix, v_prefix, k, v, heads, kv_heads, d, k_lens, key_mask, scale, causal, want_lse, out_lo=None):
     B, Nq = q.shape[:2]
     device = q.device
-    out = torch.empty(q.shape, dtype=q.dtype, device=device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((B, heads, Nq), dtype=F32, device=device) if want_lse else None
     if B * Nq == 0:
         return out, lse
@@ -225,7 +222,7 @@ class _CrossAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, heads, kv_heads, d, k_lens, key_mask, scale):
         # over 128 keys the backward pass takes sum(do * o) from the saved result, to more bits than its type has; below, it has no use for it
-        left = torch.empty(q.shape, dtype=q.dtype, device=q.device) if k.shape[1] > 128 else None
+        left = torch.empty_like(q, memory_format=torch.contiguous_format) if k.shape[1] > 128 else None
         out, lse = _context_attention(q, None, None, k, v, heads, kv_heads, d, k_lens, key_mask, scale, 0, True, left)
         ctx.save_for_backward(q, k, v, k_lens, key_mask, None if left is None else out, left, lse)
         ctx.how = heads, kv_heads, d, scale
@@ -244,11 +241,11 @@ class _CrossAttention(torch.autograd.Function):
         (B, Nq), (Bk, Nk) = q.shape[:2], k.shape[:2]
         if B * Nq * Nk == 0:
             return (torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), *(None,) * 6)
-        dq = torch.empty(q.shape, dtype=dtype, device=device)
+        dq = torch.empty_like(q, memory_format=torch.contiguous_format)
         dk = dv = None
         if Nk <= 128 or ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
-            dk = torch.empty(k.shape, dtype=dtype, device=device)
-            dv = torch.empty(v.shape, dtype=dtype, device=device)
+            dk = torch.empty_like(k, memory_format=torch.contiguous_format)
+            dv = torch.empty_like(v, memory_format=torch.contiguous_format)
         dout, *gs = _heads_of(dout, d)
         q, *qs = _heads_of(q, d)
         k, *ks = _heads_of(k, d)

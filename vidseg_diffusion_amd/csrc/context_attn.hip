@@ -657,15 +657,16 @@ Plan make_plan(int B, int Nq, int Np, int Nk, int H, int Hk) {
     const int G = H / Hk;
     const long long rows = (long long)Nq * G, heads = (long long)B * Hk;
     if (Np == 0 && Nk <= 128 && rows >= 64) {
-        // about 1024 blocks (three or four a CU), at least two tiles a wave: the keys are staged once a block
-        const long long tiles = (rows + 31) / 32, want = heads >= 1024 ? 1 : (1024 + heads - 1) / heads;
+        // the keys are staged once a block: one round of the 768 blocks that the chip holds (heads up to 64), or, from half of that in heads alone, rounds of
+        // blocks small enough for the last one to weigh little; at least two tiles a wave
+        const long long tiles = (rows + 31) / 32, want = heads <= 384 ? 768 / heads : (3072 + heads - 1) / heads;
         const long long per = (tiles + want - 1) / want;
         s.one_pass = true;
         s.per_chunk = (int)(per < 8 ? 8 : (per + 3) / 4 * 4);
         s.chunks = (int)((tiles + s.per_chunk - 1) / s.per_chunk);
         return s;
     }
-    auto deal = [](Deal& w, long long tiles_heads, int key_tiles, int least) {      // about 512 blocks, at least `least` key tiles each
+    auto deal = [](Deal& w, long long tiles_heads, int key_tiles, int least) {      // about 512 blocks, at least `least` key tiles each (256 or 512 keys: below, a joining launch costs more than it spreads)
         const long long want = tiles_heads >= 384 ? 1 : (512 + tiles_heads - 1) / tiles_heads;
         long long per = (key_tiles + want - 1) / want;
         if (per < least) per = least;
@@ -673,7 +674,8 @@ Plan make_plan(int B, int Nq, int Np, int Nk, int H, int Hk) {
         w.per_split = (int)per;
         w.blocks = (int)(tiles_heads * w.splits);
     };
-    const bool few = rows <= 32, stack = Np > 0 && rows < 128;      // a row tile of one sample alone would be mostly empty
+    // a row tile of one sample alone would be mostly empty: the rows of all samples are stacked for the prefix, where that is long enough to pay for joining
+    const bool few = rows <= 32, stack = Np >= 512 && rows < 128 && B > 1;
     const bool stack_few = few && rows * B <= 32;
     s.mode = !few ? MANY : (!stack || stack_few) ? FEW : MIXED;
     if (stack) {
@@ -681,7 +683,7 @@ Plan make_plan(int B, int Nq, int Np, int Nk, int H, int Hk) {
         s.first.stacked = 1;
         s.first.np = Np;
         s.first.xtiles = stack_few ? 1 : (int)((rows * B + 127) / 128);
-        deal(s.first, (long long)Hk * s.first.xtiles, (Np + kt - 1) / kt, stack_few ? 2 : 4);
+        deal(s.first, (long long)Hk * s.first.xtiles, (Np + kt - 1) / kt, 4);
         s.parts = s.first.splits;
     }
     if (Nk > 0 || !stack) {
@@ -689,7 +691,7 @@ Plan make_plan(int B, int Nq, int Np, int Nk, int H, int Hk) {
         s.second.np = stack ? 0 : Np;
         s.second.xtiles = few ? 1 : (int)((rows + 127) / 128);
         s.second.part0 = s.parts;
-        deal(s.second, heads * s.second.xtiles, (Nk + kt - 1) / kt + (s.second.np + kt - 1) / kt, few ? 2 : 4);
+        deal(s.second, heads * s.second.xtiles, (Nk + kt - 1) / kt + (s.second.np + kt - 1) / kt, 4);
         s.parts += s.second.splits;
     }
     if (s.parts == 1) s.parts = 0;
