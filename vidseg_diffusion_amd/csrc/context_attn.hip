@@ -140,15 +140,22 @@ struct Row {
     int b, qi, h;
     bool on;
 };
-__device__ __forceinline__ Row row_of(const AttnArgs& p, int b, int hk, long long r, long long rows) {
+__device__ __forceinline__ Row row_of(const AttnArgs& p, int b, int hk, bool stacked, int r, int rows) {      // (divisions only where a call has groups or stacked rows)
     Row x;
     x.on = r < rows;
-    if (!x.on) r = rows - 1;
-    const int per = p.Nq * p.G;
-    const int bb = (int)(r / per), rem = (int)(r - (long long)bb * per);
-    x.b = b + bb;
-    x.qi = rem / p.G;
-    x.h = hk * p.G + rem % p.G;
+    unsigned i = x.on ? r : rows - 1;
+    x.b = b;
+    if (stacked) {
+        const unsigned per = p.Nq * p.G, bb = i / per;
+        x.b += bb;
+        i -= bb * per;
+    }
+    x.qi = i;
+    x.h = hk;
+    if (p.G > 1) {
+        x.qi = i / (unsigned)p.G;
+        x.h = hk * p.G + i - x.qi * p.G;
+    }
     return x;
 }
 
@@ -164,8 +171,7 @@ __device__ __forceinline__ void block_of(int xtiles, int& y, int& xt) {
     xt = (int)(id % xtiles);
 }
 struct Place {
-    int b, hk, split, xt, len;         // len: own keys
-    long long rows;
+    int b, hk, split, xt, len, rows;   // len: own keys
 };
 __device__ __forceinline__ Place place_of(const AttnArgs& p, const Deal& w, unsigned i) {
     Place x;
@@ -176,7 +182,7 @@ __device__ __forceinline__ Place place_of(const AttnArgs& p, const Deal& w, unsi
     y /= w.splits;
     x.hk = y % p.Hk;
     x.b = y / p.Hk;
-    x.rows = (long long)(w.stacked ? p.B : 1) * p.Nq * p.G;
+    x.rows = (w.stacked ? p.B : 1) * p.Nq * p.G;                       // below 2^31 (checked)
     x.len = w.stacked ? 0 : (p.lens ? max(0, min(p.lens[x.b], p.Nk)) : p.Nk);
     return x;
 }
@@ -265,13 +271,13 @@ template <bool BF, int DP> __device__ __forceinline__ void many_rows(const AttnA
     u16 *sK = lds, *sV = lds + 2 * TILE;                              // two buffers each
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, hi = lane >> 5;
     const Place at = place_of(p, w, block);
-    const long long r0 = (long long)at.xt * BR;
-    const Row row = row_of(p, at.b, at.hk, r0 + wave * 32 + l31, at.rows);
+    const int r0 = at.xt * BR;
+    const Row row = row_of(p, at.b, at.hk, w.stacked, r0 + wave * 32 + l31, at.rows);
     u32x4 fq[DP / 16];
     load_q<DP>(p, row, hi, fq);
-    const long long last_r = (r0 + BR < at.rows ? r0 + BR : at.rows) - 1;
-    const int seen = p.causal ? max(0, min(at.len, at.len - p.Nq + 1 + (int)(last_r / p.G))) : at.len;      // own keys that the block's last row sees
-    const int all_see = p.causal ? at.len - p.Nq + 1 + (int)(r0 / p.G) : at.len;                             // own keys that every row sees
+    const int last_r = min(r0 + BR, at.rows) - 1;
+    const int seen = p.causal ? max(0, min(at.len, at.len - p.Nq + 1 + last_r / p.G)) : at.len;      // own keys that the block's last row sees
+    const int all_see = p.causal ? at.len - p.Nq + 1 + r0 / p.G : at.len;                             // own keys that every row sees
     const int T0 = (w.np + KT - 1) / KT, T1 = (seen + KT - 1) / KT;
     const int tb = min(at.split * w.per_split, T0 + T1), te = w.splits == 1 ? T0 + T1 : min(tb + w.per_split, T0 + T1);
 
@@ -338,7 +344,7 @@ template <bool BF, int DP> __device__ __forceinline__ void many_rows(const AttnA
     const long long total = (long long)p.B * p.Nq * p.H, part = w.part0 + at.split;
     l = half_sum(l);
     const long long id = ((long long)row.b * p.Nq + row.qi) * p.H + row.h;
-    const float inv = l > 0.f ? 1.0f / l : 0.f;
+    const float inv = l > 0.f ? __builtin_amdgcn_rcpf(l) : 0.f;
 #pragma unroll
     for (int n = 0; n < ND; ++n) {
         if (!p.po) {
@@ -366,8 +372,8 @@ template <bool BF, int DP> __device__ __forceinline__ void few_rows(const AttnAr
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, hi = lane >> 5;
     u16* sV = lds + wave * 32 * DP;
     const Place at = place_of(p, w, block);
-    const int rows = (int)at.rows;
-    const Row row = row_of(p, at.b, at.hk, l31, rows);
+    const int rows = at.rows;
+    const Row row = row_of(p, at.b, at.hk, w.stacked, l31, rows);
     u32x4 fq[DP / 16];
     load_q<DP>(p, row, hi, fq);
     const int len = at.len;                                           // causal: the last row sees all of them
@@ -470,7 +476,7 @@ template <bool BF, int DP> __device__ __forceinline__ void few_rows(const AttnAr
     __syncthreads();
     const long long total = (long long)p.B * p.Nq * p.H, part = w.part0 + at.split;
     const int rr = tid >> 3;
-    const Row x = row_of(p, at.b, at.hk, rr, rows);
+    const Row x = row_of(p, at.b, at.hk, w.stacked, rr, rows);
     if (!x.on) return;
     float mm = -INFINITY, ll = 0.f, f[4];
 #pragma unroll
@@ -481,7 +487,7 @@ template <bool BF, int DP> __device__ __forceinline__ void few_rows(const AttnAr
         ll += f[i] * sm[128 + i * 32 + rr];
     }
     const long long id = ((long long)x.b * p.Nq + x.qi) * p.H + x.h;
-    const float inv = ll > 0.f ? 1.0f / ll : 0.f;
+    const float inv = ll > 0.f ? __builtin_amdgcn_rcpf(ll) : 0.f;
     for (int c = (tid & 7) * 4; c < p.d; c += 32) {
         f32x4 a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -518,87 +524,91 @@ template <bool BF, int DP, int MODE> __global__ void __launch_bounds__(256, MODE
 }
 
 // A context of at most 128 keys and many rows: the rows are what has to be read and written.  The block keeps every key of its key head in LDS and each wave
-// walks over tiles of 32 rows by itself, the next tile's queries in flight; all scores of a row are there at once, so nothing is rescaled.
+// walks over tiles of 32 rows by itself, the next tile's queries in flight; all scores of a row are there at once, so nothing is rescaled.  Keys that do not
+// exist enter through the first product's accumulator, which starts at -inf for them (0 for the others).
 template <bool BF, int DP> __global__ void __launch_bounds__(256, DP == 64 ? 3 : 2) k_ctx_short(AttnArgs p, int chunks, int per_chunk) {
     constexpr int SL = DP / 8, NST = 128 * SL / 256, ND = DP / 32;
     __shared__ __attribute__((aligned(16))) u16 sK[128 * DP], sV[128 * DP];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, hi = lane >> 5;
+    __shared__ __attribute__((aligned(16))) float sE[128];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, hi = lane >> 5;
     int y, chunk;
     block_of(chunks, y, chunk);
     const int hk = y % p.Hk, b = y / p.Hk, rows = p.Nq * p.G;
-    const int t1 = min((chunk + 1) * per_chunk, (rows + 31) / 32);
-    int t = chunk * per_chunk + wave;
+    const int t1 = min((chunk + 1) * per_chunk, (rows + 31) / 32), t0 = chunk * per_chunk + wave;
     u32x4 next[DP / 16];
-    if (t < t1) load_q<DP>(p, row_of(p, b, hk, t * 32 + l31, rows), hi, next);
-    const int len = p.lens ? max(0, min(p.lens[b], p.Nk)) : p.Nk, NJ = (len + 31) / 32;
+    if (t0 < t1) load_q<DP>(p, row_of(p, b, hk, false, t0 * 32 + l31, rows), hi, next);
+    const int len = p.lens ? max(0, min(p.lens[b], p.Nk)) : p.Nk, blocks = max(1, (len + 31) / 32);
     const u16 *kb = p.k + b * p.k_b + hk * p.k_h, *vb = p.v + b * p.v_b + hk * p.v_h;
     const unsigned char* mk = p.mask ? p.mask + b * p.mask_b : nullptr;
 #pragma unroll
     for (int i = 0; i < NST; ++i) {
         const int id = tid + 256 * i, r = id / SL, slot = id % SL;
-        if (r >= NJ * 32) break;                                      // (r grows with i)
-        const bool ok = r < len && slot * 8 < p.d && (!mk || mk[r]);
-        const int kk = min(r, len - 1), c = slot * 8 < p.d ? slot * 8 : 0;
-        u32x4 rk = *reinterpret_cast<const u32x4*>(kb + kk * p.k_n + c), rv = *reinterpret_cast<const u32x4*>(vb + kk * p.v_n + c);
-        if (!ok) rk = rv = u32x4{0u, 0u, 0u, 0u};
+        if (r >= blocks * 32) break;                                  // (r grows with i)
+        u32x4 rk = {0u, 0u, 0u, 0u}, rv = {0u, 0u, 0u, 0u};
+        if (r < len && slot * 8 < p.d && (!mk || mk[r])) {
+            rk = *reinterpret_cast<const u32x4*>(kb + r * p.k_n + slot * 8);
+            rv = *reinterpret_cast<const u32x4*>(vb + r * p.v_n + slot * 8);
+        }
         *reinterpret_cast<u32x4*>(sK + slot_at<DP>(r, slot)) = rk;
         *reinterpret_cast<u32x4*>(sV + slot_at<DP>(r, slot)) = rv;
     }
-    unsigned bits[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int key = j * 32 + l31;
-        bits[j] = (unsigned)__ballot(key < len && (!mk || mk[key]));
-    }
+    if (tid < 128) sE[tid] = tid < len && (!mk || mk[tid]) ? 0.f : -INFINITY;
     __syncthreads();
-    for (; t < t1; t += 4) {
-        const Row row = row_of(p, b, hk, t * 32 + l31, rows);
-        u32x4 fq[DP / 16];
+    auto walk = [&](auto which) __attribute__((always_inline)) {
+        constexpr int NJ = decltype(which)::value;                    // blocks of 32 keys
+        for (int t = t0; t < t1; t += 4) {
+            asm volatile("" ::: "memory");                            // keeps K and V in LDS: the compiler would carry them through the loop in registers, and spill
+            const Row row = row_of(p, b, hk, false, t * 32 + l31, rows);
+            u32x4 fq[DP / 16];
 #pragma unroll
-        for (int e = 0; e < DP / 16; ++e) fq[e] = next[e];
-        if (t + 4 < t1) load_q<DP>(p, row_of(p, b, hk, (t + 4) * 32 + l31, rows), hi, next);
-        f32x16 s[4];
-        float mx = -INFINITY;
+            for (int e = 0; e < DP / 16; ++e) fq[e] = next[e];
+            if (t + 4 < t1) load_q<DP>(p, row_of(p, b, hk, false, (t + 4) * 32 + l31, rows), hi, next);
+            f32x16 s[NJ];
+            float mx = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (j >= NJ) break;
+            for (int j = 0; j < NJ; ++j) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[j][r] = 0.f;
+                for (int r = 0; r < 16; r += 4) {
+                    const f32x4 x = *reinterpret_cast<const f32x4*>(sE + j * 32 + 2 * r + 4 * hi);
 #pragma unroll
-            for (int e = 0; e < DP / 16; ++e) s[j] = mfma<BF>(read_row<DP>(sK, j * 32 + l31, e * 2 + hi), fq[e], s[j]);
-            if (bits[j] != ~0u) hide(s[j], bits[j], 1 << 30, hi);
+                    for (int w = 0; w < 4; ++w) s[j][r + w] = x[w];
+                }
 #pragma unroll
-            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[j][r]);
-        }
-        const float m = half_max(mx) * p.c, ref = m == -INFINITY ? 0.f : m;
-        float l = 0.f;
-        f32x16 acc[ND];
+                for (int e = 0; e < DP / 16; ++e) s[j] = mfma<BF>(read_row<DP>(sK, j * 32 + l31, e * 2 + hi), fq[e], s[j]);
 #pragma unroll
-        for (int n = 0; n < ND; ++n)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[n][r] = 0.f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (j >= NJ) break;
-            u32x4 fp[2];
-#pragma unroll
-            for (int r = 0; r < 16; r += 2) {
-                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[j][r], p.c, -ref)), p1 = __builtin_amdgcn_exp2f(fmaf(s[j][r + 1], p.c, -ref));
-                l += p0 + p1;
-                fp[r >> 3][(r >> 1) & 3] = pack2<BF>(p0, p1);
+                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[j][r]);
             }
+            const float m = half_max(mx) * p.c, ref = m == -INFINITY ? 0.f : m;
+            float l = 0.f;
+            f32x16 acc[ND];
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
+            for (int n = 0; n < ND; ++n) acc[n] = zero16();
 #pragma unroll
-                for (int n = 0; n < ND; ++n) acc[n] = mfma<BF>(read_tr<DP>(sV, j * 32 + e * 16, n * 32, lane), fp[e], acc[n]);
+            for (int j = 0; j < NJ; ++j) {
+                u32x4 fp[2];
+#pragma unroll
+                for (int r = 0; r < 16; r += 2) {
+                    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[j][r], p.c, -ref)), p1 = __builtin_amdgcn_exp2f(fmaf(s[j][r + 1], p.c, -ref));
+                    l += p0 + p1;
+                    fp[r >> 3][(r >> 1) & 3] = pack2<BF>(p0, p1);
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int n = 0; n < ND; ++n) acc[n] = mfma<BF>(read_tr<DP>(sV, j * 32 + e * 16, n * 32, lane), fp[e], acc[n]);
+            }
+            l = half_sum(l);
+            const float inv = l > 0.f ? __builtin_amdgcn_rcpf(l) : 0.f;
+            const long long id = ((long long)b * p.Nq + row.qi) * p.H + row.h;
+#pragma unroll
+            for (int n = 0; n < ND; ++n) store_row<BF>(p.o + id * p.d, acc[n], inv, n, hi, p.d, row.on);
+            if (p.lse && hi == 0 && row.on) p.lse[((long long)b * p.H + row.h) * p.Nq + row.qi] = (m + __builtin_amdgcn_logf(l)) * LN2;
         }
-        l = half_sum(l);
-        const float inv = l > 0.f ? 1.0f / l : 0.f;
-        const long long id = ((long long)b * p.Nq + row.qi) * p.H + row.h;
-#pragma unroll
-        for (int n = 0; n < ND; ++n) store_row<BF>(p.o + id * p.d, acc[n], inv, n, hi, p.d, row.on);
-        if (p.lse && hi == 0 && row.on) p.lse[((long long)b * p.H + row.h) * p.Nq + row.qi] = (m + __builtin_amdgcn_logf(l)) * LN2;
-    }
+    };
+    if (blocks == 1) walk(Const<1>{});
+    else if (blocks == 2) walk(Const<2>{});
+    else if (blocks == 3) walk(Const<3>{});
+    else walk(Const<4>{});
 }
 
 // Joins the partial results of one row, a wave each: four groups of sixteen lanes take every fourth part, a lane eight channels
@@ -632,7 +642,7 @@ template <bool BF> __global__ void __launch_bounds__(256) k_ctx_join(const float
         for (int e = 0; e < 8; ++e) a[e] += __shfl_xor(a[e], w, 64);
     }
     if (grp) return;
-    const float inv = l > 0.f ? 1.0f / l : 0.f;
+    const float inv = l > 0.f ? __builtin_amdgcn_rcpf(l) : 0.f;
     if (c < d) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) a[e] *= inv;
