@@ -194,8 +194,11 @@ template <int DP> __device__ __forceinline__ void load_q(const AttnArgs& p, cons
     for (int s = 0; s < DP / 16; ++s) {
         const int at = s * 16 + hi * 8;
         f[s] = *reinterpret_cast<const u32x4*>(qp + (at < p.d ? at : 0));
-        if (at >= p.d) f[s] = u32x4{0u, 0u, 0u, 0u};
     }
+    if (p.d < DP)
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s)
+            if (s * 16 + hi * 8 >= p.d) f[s] = u32x4{0u, 0u, 0u, 0u};
 }
 
 // 32 columns n * 32 .. of one row out of its accumulator, times f, as 16-byte pieces: the lane halves hold the rows 4 hi .. of every
@@ -208,14 +211,19 @@ template <bool BF> __device__ __forceinline__ unsigned left2(float a, float b) {
     const unsigned x = pack2<BF>(a, b);
     return pack2<BF>(a - value_of<BF>(x, 0), b - value_of<BF>(x, 1));
 }
-template <bool BF, bool LEFT = false> __device__ __forceinline__ void store_row(u16* row, const f32x16& a, float f, int n, int hi, int d, bool on) {
+// channels 16 g + 8 hi .. + 7 of a block of 32
+template <bool BF, bool LEFT = false> __device__ __forceinline__ u32x4 eight(const f32x16& a, float f, int g) {
     auto two = [&](int r) __attribute__((always_inline)) { return LEFT ? left2<BF>(a[r] * f, a[r + 1] * f) : pack2<BF>(a[r] * f, a[r + 1] * f); };
+    const auto x = __builtin_amdgcn_permlane32_swap(two(8 * g), two(8 * g + 4), false, false);
+    const auto y = __builtin_amdgcn_permlane32_swap(two(8 * g + 2), two(8 * g + 6), false, false);
+    return u32x4{x[0], y[0], x[1], y[1]};
+}
+template <bool BF, bool LEFT = false> __device__ __forceinline__ void store_row(u16* row, const f32x16& a, float f, int n, int hi, int d, bool on) {
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
-        const auto x = __builtin_amdgcn_permlane32_swap(two(8 * g), two(8 * g + 4), false, false);
-        const auto y = __builtin_amdgcn_permlane32_swap(two(8 * g + 2), two(8 * g + 6), false, false);
         const int c = n * 32 + 16 * g + 8 * hi;
-        if (on && c < d) *reinterpret_cast<u32x4*>(row + c) = u32x4{x[0], y[0], x[1], y[1]};
+        const u32x4 x = eight<BF, LEFT>(a, f, g);
+        if (on && c < d) *reinterpret_cast<u32x4*>(row + c) = x;
     }
 }
 
@@ -535,8 +543,22 @@ template <bool BF, int DP> __global__ void __launch_bounds__(256, DP == 64 ? 3 :
     block_of(chunks, y, chunk);
     const int hk = y % p.Hk, b = y / p.Hk, rows = p.Nq * p.G;
     const int t1 = min((chunk + 1) * per_chunk, (rows + 31) / 32), t0 = chunk * per_chunk + wave;
-    u32x4 next[DP / 16];
-    if (t0 < t1) load_q<DP>(p, row_of(p, b, hk, false, t0 * 32 + l31, rows), hi, next);
+    // whole tiles of a head that fills its registers, no groups: uniform base and one offset a lane, for queries and results
+    const bool plain = p.G == 1 && p.d == DP;
+    const unsigned q_off = (unsigned)(l31 * (int)p.q_n + hi * 8) * 2u, o_off = (unsigned)(l31 * p.H * p.d + hi * 8) * 2u;
+    const u16* q0 = p.q + b * p.q_b + hk * p.q_h;
+    u16* o0 = p.o + ((long long)b * p.Nq * p.H + hk) * p.d;
+    u32x4 fq[DP / 16];
+    auto queries = [&](int t) __attribute__((always_inline)) {
+        if (plain && t * 32 + 32 <= rows) {
+            const char* at = reinterpret_cast<const char*>(q0 + t * 32 * p.q_n);
+#pragma unroll
+            for (int s = 0; s < DP / 16; ++s) fq[s] = *reinterpret_cast<const u32x4*>(at + q_off + s * 32);
+        } else {
+            load_q<DP>(p, row_of(p, b, hk, false, t * 32 + l31, rows), hi, fq);
+        }
+    };
+    if (t0 < t1) queries(t0);
     const int len = p.lens ? max(0, min(p.lens[b], p.Nk)) : p.Nk, blocks = max(1, (len + 31) / 32);
     const u16 *kb = p.k + b * p.k_b + hk * p.k_h, *vb = p.v + b * p.v_b + hk * p.v_h;
     const unsigned char* mk = p.mask ? p.mask + b * p.mask_b : nullptr;
@@ -558,11 +580,6 @@ template <bool BF, int DP> __global__ void __launch_bounds__(256, DP == 64 ? 3 :
         constexpr int NJ = decltype(which)::value;                    // blocks of 32 keys
         for (int t = t0; t < t1; t += 4) {
             asm volatile("" ::: "memory");                            // keeps K and V in LDS: the compiler would carry them through the loop in registers, and spill
-            const Row row = row_of(p, b, hk, false, t * 32 + l31, rows);
-            u32x4 fq[DP / 16];
-#pragma unroll
-            for (int e = 0; e < DP / 16; ++e) fq[e] = next[e];
-            if (t + 4 < t1) load_q<DP>(p, row_of(p, b, hk, false, (t + 4) * 32 + l31, rows), hi, next);
             f32x16 s[NJ];
             float mx = -INFINITY;
 #pragma unroll
@@ -575,9 +592,12 @@ template <bool BF, int DP> __global__ void __launch_bounds__(256, DP == 64 ? 3 :
                 }
 #pragma unroll
                 for (int e = 0; e < DP / 16; ++e) s[j] = mfma<BF>(read_row<DP>(sK, j * 32 + l31, e * 2 + hi), fq[e], s[j]);
+            }
+            if (t + 4 < t1) queries(t + 4);                           // the next tile's, into the registers that the scores have left
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[j][r]);
-            }
             const float m = half_max(mx) * p.c, ref = m == -INFINITY ? 0.f : m;
             float l = 0.f;
             f32x16 acc[ND];
@@ -599,6 +619,16 @@ template <bool BF, int DP> __global__ void __launch_bounds__(256, DP == 64 ? 3 :
             }
             l = half_sum(l);
             const float inv = l > 0.f ? __builtin_amdgcn_rcpf(l) : 0.f;
+            if (plain && t * 32 + 32 <= rows) {
+                char* at = reinterpret_cast<char*>(o0 + (long long)t * 32 * p.H * p.d);
+#pragma unroll
+                for (int n = 0; n < ND; ++n)
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) *reinterpret_cast<u32x4*>(at + o_off + n * 64 + g * 32) = eight<BF>(acc[n], inv, g);
+                if (p.lse && hi == 0) p.lse[((long long)b * p.H + hk) * p.Nq + t * 32 + l31] = (m + __builtin_amdgcn_logf(l)) * LN2;
+                continue;
+            }
+            const Row row = row_of(p, b, hk, false, t * 32 + l31, rows);
             const long long id = ((long long)b * p.Nq + row.qi) * p.H + row.h;
 #pragma unroll
             for (int n = 0; n < ND; ++n) store_row<BF>(p.o + id * p.d, acc[n], inv, n, hi, p.d, row.on);
