@@ -107,12 +107,21 @@ def test_far_mean_keeps_its_variance():
     check_all(x + 4096.0, gamma, beta, dy, 8, True)
 
 
+@pytest.mark.parametrize("rows,C,groups,dims", [(1, 8, 8, (20000,)), (1, 320, 32, (64, 64)), (1250, 8, 8, (20000,)), (3, 1280, 32, (40, 40))])
+def test_first_rows_far_from_the_others(rows, C, groups, dims):
+    """The first rows (of a thread, a chunk, a map) are no good reference for the others: 10^4 away from them."""
+    dev = torch.device("cuda:0")
+    x, gamma, beta, dy = data(2, dims, C, torch.float32, 7, dev)
+    x.view(2, -1, C)[:, :rows] += 1e4
+    check_all(x, gamma, beta, dy, groups, True)
+
+
 def test_constant_map():
     dev = torch.device("cuda:0")
     x = torch.full((2, 9, 64), 3.0, device=dev)
     gamma, beta = torch.ones(64, device=dev), torch.linspace(-1, 1, 64, device=dev)
     y = ops.groupnorm_act(x, gamma, beta, groups=8, act=ops.ACT_NONE)
-    assert torch.equal(y, beta.expand_as(y))                          # the chunk's first value is the shift: every difference is exactly zero
+    assert torch.equal(y, beta.expand_as(y))                          # a thread's first value is the shift: every difference is exactly zero
 
 
 def test_slices_and_other_orders():

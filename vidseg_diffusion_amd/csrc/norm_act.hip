@@ -103,54 +103,63 @@ __device__ __forceinline__ float lanes_sum(float v, int lanes) {
     return v;
 }
 
-// ---- forward, launch 1: (mean, M2) of every group over the rows of one chunk.
-// A channel is summed about its own first value of the chunk (x - x[row0]), then mean and sum of squared deviations of the group are put together
-// from the channels': no difference of large squares anywhere, so maps whose mean is far from zero keep their variance.
+// ---- forward, launch 1: (mean, M2) of every group over the rows of one chunk, M2 the sum of squared deviations from that mean.
+// A thread takes its rows less the first of them, x - k, and carries mean and M2 along: with d = (x - k) - mean,  mean += d / n,  M2 += d ((x - k) - mean);
+// row lanes, channels and chunks are then merged by theirs:
+//   mean = mean_a + (mean_b - mean_a) n_b / n,   M2 = M2_a + M2_b + (mean_b - mean_a)^2 n_a n_b / n.
+// No difference of large squares anywhere, so a map whose mean is far from zero, or whose first rows lie far from the others, keeps its variance.
+// (Sums of x - k and its square would take 3 operations a value for 5, and lose a factor of the rows where the first one is an outlier.)
 template <typename T, int VEC> __global__ void __launch_bounds__(NT) k_gna_stats(NormArgs p) {
     extern __shared__ float lds[];
     const int C = p.C, cols = C / VEC, b = blockIdx.y, chunk = blockIdx.x;
     const int pc = cols < NT ? cols : NT, R = NT / pc, width = pc * VEC;
     float* ch_mean = lds;                 // [C]
     float* ch_m2 = lds + C;               // [C]
-    float* s0 = lds + 2 * C;              // [R][width]
-    float* s1 = s0 + R * width;
+    float* s0 = lds + 2 * C;              // [R][width] means of the row lanes
+    float* s1 = s0 + R * width;           // ... and M2
     const long long r0 = (long long)chunk * p.rows;
     const int n = (int)(p.HW - r0 < p.rows ? p.HW - r0 : p.rows);
     const T* x = (const T*)p.x + b * p.x_b + r0 * p.x_row;
     const int col = threadIdx.x % pc, rl = threadIdx.x / pc;
     for (int c0 = 0; c0 < cols; c0 += pc) {
-        const bool on = rl < R && c0 + col < cols;
-        float k[VEC], a[VEC], q[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) k[e] = a[e] = q[e] = 0.f;
-        if (on) {
+        if (rl < R && rl < n && c0 + col < cols) {
+            float k[VEC], a[VEC], q[VEC], count = 1.f;
             const T* xc = x + (long long)(c0 + col) * VEC;
-            load_vec<T, VEC>(xc, k);
+            load_vec<T, VEC>(xc + rl * p.x_row, k);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) a[e] = q[e] = 0.f;
 #pragma unroll 4
-            for (int r = rl; r < n; r += R) {
+            for (int r = rl + R; r < n; r += R) {
                 float v[VEC];
                 load_vec<T, VEC>(xc + r * p.x_row, v);
+                count += 1.f;
+                const float inv = __builtin_amdgcn_rcpf(count);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
-                    const float d = v[e] - k[e];
-                    a[e] += d;
-                    q[e] += d * d;
+                    const float u = v[e] - k[e], d = u - a[e];
+                    a[e] += d * inv;
+                    q[e] += d * (u - a[e]);
                 }
             }
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                s0[rl * width + col * VEC + e] = a[e];
+                s0[rl * width + col * VEC + e] = k[e] + a[e];
                 s1[rl * width + col * VEC + e] = q[e];
             }
         }
-        fold_rows<VEC>(s0, s1, R, width);
-        if (rl == 0 && on) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const float s = s0[col * VEC + e], m = s / (float)n;
-                ch_mean[(c0 + col) * VEC + e] = k[e] + m;
-                ch_m2[(c0 + col) * VEC + e] = fmaxf(s1[col * VEC + e] - s * m, 0.f);
+        __syncthreads();
+        const int w = (cols - c0 < pc ? cols - c0 : pc) * VEC, lanes = R < n ? R : n;
+        for (int c = threadIdx.x; c < w; c += NT) {                 // lane j has (n - j) / R rows, rounded up
+            const float k = s0[c];
+            float s = 0.f, m2 = 0.f;
+            for (int j = 1; j < lanes; ++j) s += (float)((n - j + R - 1) / R) * (s0[j * width + c] - k);
+            const float m = s / (float)n;                           // about lane 0's mean
+            for (int j = 0; j < lanes; ++j) {
+                const float d = s0[j * width + c] - k - m;
+                m2 += s1[j * width + c] + (float)((n - j + R - 1) / R) * d * d;
             }
+            ch_mean[c0 * VEC + c] = k + m;
+            ch_m2[c0 * VEC + c] = m2;
         }
         __syncthreads();
     }
@@ -169,6 +178,14 @@ template <typename T, int VEC> __global__ void __launch_bounds__(NT) k_gna_stats
     }
 }
 
+// rows n_b of mean m_b and M2 m2_b (over cg channels) into (n, m, m2); either may be empty
+__device__ __forceinline__ void merge(float& n, float& m, float& m2, float n_b, float m_b, float m2_b, float cg) {
+    const float all = n + n_b, share = n > 0.f ? n_b * __builtin_amdgcn_rcpf(all) : 1.f, d = m_b - m;      // (the first part is taken as it is)
+    m += d * share;
+    m2 += m2_b + d * d * (n * share) * cg;
+    n = all;
+}
+
 // ---- forward, launch 2: every block merges its sample's chunk statistics (a few KB out of L2) and writes one chunk of y
 template <typename T, int VEC> __global__ void __launch_bounds__(NT) k_gna_apply(NormArgs p) {
     extern __shared__ float lds[];
@@ -179,20 +196,24 @@ template <typename T, int VEC> __global__ void __launch_bounds__(NT) k_gna_apply
     for (int g0 = 0; g0 < p.G; g0 += stride) {
         const int g = min(g0 + (int)threadIdx.x / lanes, p.G - 1);
         const f32x2* o = reinterpret_cast<const f32x2*>(p.part) + (long long)b * p.nchunk * p.G + g;
-        // one pass about the first chunk's mean k: mean = k + s / HW, M2 = q - HW cg (mean - k)^2, where |mean - k| is of the spread's size
-        const float k = o[0][0];
-        float s = 0.f, q = 0.f;
+        float n = 0.f, m = 0.f, m2 = 0.f;                           // rows (exact below 2^24 a lane), mean and M2 of this lane's chunks
 #pragma unroll 4
         for (int i = sub; i < p.nchunk; i += lanes) {
-            const float n = (float)(i + 1 < p.nchunk ? p.rows : (int)(p.HW - (long long)i * p.rows));
+            const float rows = (float)(i + 1 < p.nchunk ? p.rows : (int)(p.HW - (long long)i * p.rows));
             const f32x2 t = o[(long long)i * p.G];
-            const float d = t[0] - k;
-            s += n * d;
-            q += t[1] + n * (float)cg * d * d;
+            merge(n, m, m2, rows, t[0], t[1], (float)cg);
         }
-        s = lanes_sum(s, lanes) / (float)p.HW;
-        q = lanes_sum(q, lanes) / ((float)p.HW * (float)cg) - s * s;
-        const float m = k + s, rstd = 1.0f / sqrtf(fmaxf(q, 0.f) + p.eps);
+        for (int w = 1; w < lanes; w *= 2) {
+            const float n_b = __shfl_xor(n, w, 64), m_b = __shfl_xor(m, w, 64), m2_b = __shfl_xor(m2, w, 64);
+            // the lower lane's part first: both lanes get the same values
+            const bool up = sub & w;
+            float n_a = up ? n_b : n, m_a = up ? m_b : m, m2_a = up ? m2_b : m2;
+            merge(n_a, m_a, m2_a, up ? n : n_b, up ? m : m_b, up ? m2 : m2_b, (float)cg);
+            n = n_a;
+            m = m_a;
+            m2 = m2_a;
+        }
+        const float rstd = 1.0f / sqrtf(m2 / ((float)p.HW * (float)cg) + p.eps);
         if (sub == 0) {
             g_mean[g] = m;
             g_rstd[g] = rstd;
