@@ -103,6 +103,29 @@ def test_key_mask_and_poison(Nq, d, dtype):
     Reference(q, k, v, H, None, None, mask[:1].expand(B, Nk)).check(one)
 
 
+@pytest.mark.parametrize("Nq,Nk", [(70, 77), (1, 77), (70, 300), (1, 300)])
+def test_nothing_to_attend_to_and_no_number_to_ask_with(Nq, Nk):
+    """A padded sample: no key, and queries that hold NaN and infinities.  Zeros, log-sum-exp -inf, gradients of zero, and no other sample's values change."""
+    dev = torch.device("cuda:0")
+    q, k, v, w = (randn((3, n, 128), s, F16).to(dev) for n, s in ((Nq, 1), (Nk, 2), (Nk, 3), (Nq, 4)))
+    lens = torch.tensor([Nk, 0, 5], dtype=torch.int32, device=dev)
+
+    def step(q):
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        out, lse = ops.cross_attention(*leaves, 2, k_lens=lens, return_lse=True)
+        return (out.detach(), lse, *torch.autograd.grad(out, leaves, w))
+    want = step(q)
+    for bad in (float("nan"), float("inf")):
+        q2 = q.clone()
+        q2[1] = bad
+        for a, b in zip(want, step(q2)):
+            assert torch.equal(a, b)
+        mask = torch.arange(Nk, device=dev) < lens.view(3, 1)
+        assert torch.equal(want[0], ops.cross_attention(q2, k, v, 2, key_mask=mask))
+        assert torch.equal(want[0], ops.prefix_attention(q2, k[0, :0], v[0, :0], k, v, 2, k_lens=lens))
+    assert not want[0][1].any() and torch.isneginf(want[1][1]).all() and not any(t[1].any() for t in want[2:])
+
+
 def test_layouts_and_strides():
     """Column slices of a fused projection, heads as a dimension in either order, a context expanded over the batch, unaligned views (copied)."""
     dev = torch.device("cuda:0")

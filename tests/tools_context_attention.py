@@ -9,7 +9,7 @@ Tolerance of an output o = sum p v / sum p whose probabilities p are rounded onc
 Tolerance of the gradients, with ds = p (dp - D), dp = do v^T, D = sum do o:
     dv: u |dv| + (u + 4 e) p^T |do|                                 p rounded once; its error now includes the saved log-sum-exp's
     ds: (u + 4 e) |ds| + p (sum |do| tol(o)) + 2^-24 (d + 8) p (|do| |v|^T + sum |do o|)        rounded once; D is taken from the rounded o
-        + 2^-25 max|do| in fp16                                     (ds is scaled by a power of two >= 1 / max|do|, off by half a subnormal step)
+        + 2^-37 (max|dp| + max|D|) in fp16                          (p is carried as 2^12 p, dp - D with a power of two of at least 1 / its maximum: off by half a subnormal step)
     dq: u |dq| + scale tol(ds) |k|,   dk: u |dk| + scale tol(ds)^T |q|,   each plus half a subnormal step of fp16
 """
 import math
@@ -88,7 +88,7 @@ class Reference:
         r_dv, t_dv = self.p.transpose(2, 3) @ go, (u + 4 * self.e) * (self.p.transpose(2, 3) @ go.abs())
         t_ds = (u + 4 * self.e) * ds.abs() + self.p * (go.abs() * self.tol).sum(-1, keepdim=True) + \
             2.0 ** -24 * (self.d + 8) * self.p * (go.abs() @ self.v.abs().transpose(2, 3) + (go * self.o).abs().sum(-1, keepdim=True))
-        t_ds = (t_ds + sub * float(go.abs().max())) * self.live
+        t_ds = (t_ds + 2.0 ** -12 * sub * float(dp.abs().max() + D.abs().max())) * self.live
         r_dq, t_dq = self.scale * (ds @ self.k), self.scale * (t_ds @ self.k.abs())
         r_dk, t_dk = self.scale * (ds.transpose(2, 3) @ self.q), self.scale * (t_ds.transpose(2, 3) @ self.q.abs())
 

@@ -574,8 +574,18 @@ template <bool BF, int DP> __global__ void __launch_bounds__(256, DP == 64 ? 3 :
         *reinterpret_cast<u32x4*>(sK + slot_at<DP>(r, slot)) = rk;
         *reinterpret_cast<u32x4*>(sV + slot_at<DP>(r, slot)) = rv;
     }
-    if (tid < 128) sE[tid] = tid < len && (!mk || mk[tid]) ? 0.f : -INFINITY;
-    __syncthreads();
+    const bool exists = tid < min(len, 128) && (!mk || mk[tid]);
+    if (tid < 128) sE[tid] = exists ? 0.f : -INFINITY;
+    if (!__syncthreads_or(exists)) {                                  // no key at all: zeros, whatever the queries hold
+        for (int t = t0; t < t1; t += 4) {
+            const Row row = row_of(p, b, hk, false, t * 32 + l31, rows);
+            const long long id = ((long long)b * p.Nq + row.qi) * p.H + row.h;
+#pragma unroll
+            for (int n = 0; n < ND; ++n) store_row<BF>(p.o + id * p.d, zero16(), 0.f, n, hi, p.d, row.on);
+            if (p.lse && hi == 0 && row.on) p.lse[((long long)b * p.H + row.h) * p.Nq + row.qi] = -INFINITY;
+        }
+        return;
+    }
     auto walk = [&](auto which) __attribute__((always_inline)) {
         constexpr int NJ = decltype(which)::value;                    // blocks of 32 keys
         for (int t = t0; t < t1; t += 4) {
@@ -699,7 +709,7 @@ Plan make_plan(int B, int Nq, int Np, int Nk, int H, int Hk) {
     if (Np == 0 && Nk <= 128 && rows >= 64) {
         // the keys are staged once a block: one round of the 768 blocks that the chip holds (heads up to 64), or, from half of that in heads alone, rounds of
         // blocks small enough for the last one to weigh little; at least two tiles a wave
-        const long long tiles = (rows + 31) / 32, want = heads <= 384 ? 768 / heads : (3072 + heads - 1) / heads;
+        const long long tiles = (rows + 31) / 32, want = heads <= 384 ? 768 / heads : (4 * 768 + heads - 1) / heads;
         const long long per = (tiles + want - 1) / want;
         s.one_pass = true;
         s.per_chunk = (int)(per < 8 ? 8 : (per + 3) / 4 * 4);
@@ -715,7 +725,8 @@ Plan make_plan(int B, int Nq, int Np, int Nk, int H, int Hk) {
         w.blocks = (int)(tiles_heads * w.splits);
     };
     // a row tile of one sample alone would be mostly empty: the rows of all samples are stacked for the prefix, where that is long enough to pay for joining
-    const bool few = rows <= 32, stack = Np >= 512 && rows < 128 && B > 1;
+    // (2^26 rows: what the joining launch takes)
+    const bool few = rows <= 32, stack = Np >= 512 && rows < 128 && B > 1 && rows * heads < (1ll << 26);
     const bool stack_few = few && rows * B <= 32;
     s.mode = !few ? MANY : (!stack || stack_few) ? FEW : MIXED;
     if (stack) {
@@ -757,8 +768,9 @@ template <bool BF, int DP> void launch_fwd(const AttnArgs& p, const Plan& s, hip
 // Backward.  With L = lse log2 e and D = sum_keys p dp of a row:  p = exp2(s c - L),  dp = do v^T,  ds = p (dp - D),
 //   dv = p^T do,   dk = scale ds^T q,   dq = scale ds k.
 // p and ds are rounded once to the storage type before they enter a product.  fp16 needs both kept away from its subnormals (p of a row over
-// 4096 keys is 2^-12, its ds smaller still): p is carried as 2^12 p, ds with a power of two that brings the largest |dp - D| in sight to about 1 --
-// exact factors that leave in fp32 at the end; accumulators are rescaled where the power changes.
+// 4096 keys is 2^-12, its ds smaller still): p is carried as 2^12 p, and dp - D with a power of two that brings the largest in sight to 1..4, so ds
+// stays below 2^14 and a subnormal's half step is 2^-37 of the largest |dp - D| -- exact factors that leave in fp32 at the end; accumulators are
+// rescaled where the power changes.
 struct BwdArgs {
     const u16 *q, *k, *v, *o, *o_lo, *go;
     long long q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h, g_b, g_n, g_h;
@@ -824,7 +836,7 @@ template <bool BF, int DP> __global__ void __launch_bounds__(256, DP == 64 ? 3 :
     D = half_sum(D);
     const long long bhq = ((long long)b * p.H + h) * p.Nq + qi;
     const float lse = p.lse[bhq];
-    const float L = lse == -INFINITY ? INFINITY : lse * LOG2E;                  // a row without a key: p = 0
+    const float L = lse == -INFINITY ? INFINITY : lse * LOG2E - (BF ? 0.f : P_LOG2);      // a row without a key: p = 0
     if (on && hi == 0) p.delta[bhq] = D;
     float power = BF ? 1.f : 1.152921504606846976e18f;                          // this row's factor of ds
     f32x16 acc[ND];
@@ -849,7 +861,7 @@ template <bool BF, int DP> __global__ void __launch_bounds__(256, DP == 64 ? 3 :
                 float m = fabsf(z[0]);
 #pragma unroll
                 for (int e = 1; e < 16; ++e) m = fmaxf(m, fabsf(z[e]));
-                if (__builtin_expect(__any(m * power > 16384.f), 0)) {
+                if (__builtin_expect(__any(m * power > 4.f), 0)) {
                     const float f = fminf(power, power_for(half_max(m)));      // both lane halves hold the same row
 #pragma unroll
                     for (int n = 0; n < ND; ++n)
@@ -881,7 +893,7 @@ template <bool BF, int DP> __global__ void __launch_bounds__(256, DP == 64 ? 3 :
         work(Const<0>{}, t);
         if (t + 1 < T) work(Const<1>{}, t + 1);
     }
-    const float back = p.scale / power;
+    const float back = p.scale / power * (BF ? 1.f : P_BACK);
 #pragma unroll
     for (int n = 0; n < ND; ++n) store_row<BF>(p.dq + id * p.d, acc[n], back, n, hi, p.d, on);
 }
@@ -1068,11 +1080,11 @@ template <bool BF, int DP, bool FUSED, bool DV, bool DK> __device__ __forceinlin
                         float m = fabsf(z[0]);
 #pragma unroll
                         for (int e = 1; e < 16; ++e) m = fmaxf(m, fabsf(z[e]));
-                        if (__builtin_expect(__any(m * power > 16384.f), 0)) move_power(fminf(power, power_for(half_max(m))));
+                        if (__builtin_expect(__any(m * power > 4.f), 0)) move_power(fminf(power, power_for(half_max(m))));
                     }
 #pragma unroll
                     for (int e = 0; e < 16; ++e) z[e] *= s[e];
-                    pack(z, BF ? 1.f : power * P_BACK, fd);
+                    pack(z, BF ? 1.f : power, fd);
                 }
                 products(buf, i, fp, fd);
             }
@@ -1119,7 +1131,7 @@ template <bool BF, int DP, bool FUSED, bool DV, bool DK> __device__ __forceinlin
 #pragma unroll
                     for (int w = 0; w < 4; ++w) z[i][e + w] = (z[i][e + w] - D[w]) * s[i][e + w];
                 }
-                pack(z[i], BF ? 1.f : power * P_BACK, fd);
+                pack(z[i], BF ? 1.f : power, fd);
 #pragma unroll
                 for (int e = 0; e < 16; e += 4)                                 // [key][row]: rows i 32 + 2 e + 4 hi + 0..3
                     *reinterpret_cast<u32x2*>(sS + slot_at<RT>(wave * 32 + l31, i * 4 + (e >> 2)) + 4 * hi) = u32x2{fd[e >> 3][(e >> 1) & 3], fd[e >> 3][((e >> 1) & 3) + 1]};
@@ -1127,7 +1139,7 @@ template <bool BF, int DP, bool FUSED, bool DV, bool DK> __device__ __forceinlin
             }
             if (more) settle(buf ^ 1);
             landed();
-            const float to_dq = p.scale / power;
+            const float to_dq = p.scale / power * (BF ? 1.f : P_BACK);
             const int h = hk * p.G + now.g;
             for (int w = wave; w < 2 * ND; w += 4) {
                 const int i = w & 1, n = w >> 1;
@@ -1147,7 +1159,7 @@ template <bool BF, int DP, bool FUSED, bool DV, bool DK> __device__ __forceinlin
             whole = __all(live);
         }
     }
-    const float to_k = any ? p.scale / power : 0.f, to_v = any ? (BF ? 1.f : P_BACK) : 0.f;
+    const float to_k = any ? p.scale / power * (BF ? 1.f : P_BACK) : 0.f, to_v = any ? (BF ? 1.f : P_BACK) : 0.f;
     if (!any)
 #pragma unroll
         for (int n = 0; n < ND; ++n) ak[n] = av[n] = zero16();                   // (they may hold infinities)
