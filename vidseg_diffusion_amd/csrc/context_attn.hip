@@ -559,7 +559,7 @@ template <bool BF, int DP> __global__ void __launch_bounds__(256, DP == 64 ? 3 :
         }
     };
     if (t0 < t1) queries(t0);
-    const int len = p.lens ? max(0, min(p.lens[b], p.Nk)) : p.Nk, blocks = max(1, (len + 31) / 32);
+    const int len = p.lens ? max(0, min(p.lens[b], p.Nk)) : p.Nk, halves = max(1, (len + 15) / 16), blocks = (halves + 1) / 2;
     const u16 *kb = p.k + b * p.k_b + hk * p.k_h, *vb = p.v + b * p.v_b + hk * p.v_h;
     const unsigned char* mk = p.mask ? p.mask + b * p.mask_b : nullptr;
 #pragma unroll
@@ -587,7 +587,7 @@ template <bool BF, int DP> __global__ void __launch_bounds__(256, DP == 64 ? 3 :
         return;
     }
     auto walk = [&](auto which) __attribute__((always_inline)) {
-        constexpr int NJ = decltype(which)::value;                    // blocks of 32 keys
+        constexpr int NH = decltype(which)::value, NJ = (NH + 1) / 2; // half blocks of 16 keys, which an accumulator's first and last eight registers hold; blocks of 32
         for (int t = t0; t < t1; t += 4) {
             asm volatile("" ::: "memory");                            // keeps K and V in LDS: the compiler would carry them through the loop in registers, and spill
             f32x16 s[NJ];
@@ -607,7 +607,7 @@ template <bool BF, int DP> __global__ void __launch_bounds__(256, DP == 64 ? 3 :
 #pragma unroll
             for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[j][r]);
+                for (int r = 0; r < 16 && 2 * j + (r >> 3) < NH; ++r) mx = fmaxf(mx, s[j][r]);
             const float m = half_max(mx) * p.c, ref = m == -INFINITY ? 0.f : m;
             float l = 0.f;
             f32x16 acc[ND];
@@ -617,13 +617,13 @@ template <bool BF, int DP> __global__ void __launch_bounds__(256, DP == 64 ? 3 :
             for (int j = 0; j < NJ; ++j) {
                 u32x4 fp[2];
 #pragma unroll
-                for (int r = 0; r < 16; r += 2) {
+                for (int r = 0; r < 16 && 2 * j + (r >> 3) < NH; r += 2) {
                     const float p0 = __builtin_amdgcn_exp2f(fmaf(s[j][r], p.c, -ref)), p1 = __builtin_amdgcn_exp2f(fmaf(s[j][r + 1], p.c, -ref));
                     l += p0 + p1;
                     fp[r >> 3][(r >> 1) & 3] = pack2<BF>(p0, p1);
                 }
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
+                for (int e = 0; e < 2 && 2 * j + e < NH; ++e)
 #pragma unroll
                     for (int n = 0; n < ND; ++n) acc[n] = mfma<BF>(read_tr<DP>(sV, j * 32 + e * 16, n * 32, lane), fp[e], acc[n]);
             }
@@ -645,10 +645,16 @@ template <bool BF, int DP> __global__ void __launch_bounds__(256, DP == 64 ? 3 :
             if (p.lse && hi == 0 && row.on) p.lse[((long long)b * p.H + row.h) * p.Nq + row.qi] = (m + __builtin_amdgcn_logf(l)) * LN2;
         }
     };
-    if (blocks == 1) walk(Const<1>{});
-    else if (blocks == 2) walk(Const<2>{});
-    else if (blocks == 3) walk(Const<3>{});
-    else walk(Const<4>{});
+    switch (halves) {
+        case 1: walk(Const<1>{}); break;
+        case 2: walk(Const<2>{}); break;
+        case 3: walk(Const<3>{}); break;
+        case 4: walk(Const<4>{}); break;
+        case 5: walk(Const<5>{}); break;
+        case 6: walk(Const<6>{}); break;
+        case 7: walk(Const<7>{}); break;
+        default: walk(Const<8>{});
+    }
 }
 
 // Joins the partial results of one row, a wave each: four groups of sixteen lanes take every fourth part, a lane eight channels
@@ -1221,11 +1227,19 @@ BwdPlan make_bwd_plan(int B, int Bk, int Nq, int Nk, int H, int Hk, int d) {
     s.fused = Nk <= 128;
     s.ktiles = (Nk + 127) / 128;
     const long long tiles = ((long long)Nq + 63) / 64 * (H / Hk) * (Bk < B ? B : 1), blocks = (long long)Bk * Hk * s.ktiles;
-    const long long want = blocks >= 384 ? 1 : (512 + blocks - 1) / blocks;      // about two blocks a CU, at least two tiles each
-    long long per = (tiles + want - 1) / want;
-    if (per < 2) per = 2;
-    s.per_chunk = (int)per;
-    s.chunks = (int)((tiles + per - 1) / per);
+    // The rows are dealt out in chunks where key tiles alone leave part of the chip idle: as many as make the rounds that its `slots` blocks take
+    // shortest (a block's first tile counts twice), at least two tiles each
+    const long long slots = s.fused && d > 64 ? 256 : 512;
+    long long best = tiles, cost = (blocks + slots - 1) / slots * (tiles + 1);
+    for (long long c = 2; blocks < 384 && c <= 512 && c <= tiles / 2; ++c) {
+        const long long per = (tiles + c - 1) / c, rounds = (blocks * ((tiles + per - 1) / per) + slots - 1) / slots;
+        if (rounds * (per + 1) < cost) {
+            cost = rounds * (per + 1);
+            best = per;
+        }
+    }
+    s.per_chunk = (int)best;
+    s.chunks = (int)((tiles + best - 1) / best);
     s.delta_floats = s.fused ? 0 : ((long long)B * H * Nq + 3) / 4 * 4;
     s.part_floats = s.chunks > 1 ? 2ll * s.chunks * Bk * Nk * Hk * d : 0;
     return s;
