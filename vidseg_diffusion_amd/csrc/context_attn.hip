@@ -708,7 +708,20 @@ struct Plan {
     Deal first, second;
     int parts;                 // partial results to join (0: the kernel writes the result)
 };
-Plan make_plan(int B, int Nq, int Np, int Nk, int H, int Hk) {
+// `tiles` tiles of work in each of `blocks` places: how many of them a block takes.  Where the places alone leave part of the chip idle the tiles are dealt
+// out in runs: as many as make the rounds that `slots` resident blocks take shortest (a block's start and its partial results count as two tiles), at least `least` tiles each
+long long dealt(long long blocks, long long tiles, long long slots, long long least) {
+    long long best = tiles, cost = (blocks + slots - 1) / slots * (tiles + 2);
+    for (long long c = 2; blocks < 384 && c <= 512 && c * least <= tiles; ++c) {
+        const long long per = (tiles + c - 1) / c, rounds = (blocks * ((tiles + per - 1) / per) + slots - 1) / slots;
+        if (rounds * (per + 2) < cost) {
+            cost = rounds * (per + 2);
+            best = per;
+        }
+    }
+    return best < 1 ? 1 : best;
+}
+Plan make_plan(int B, int Nq, int Np, int Nk, int H, int Hk, int d) {
     Plan s{};
     const int G = H / Hk;
     const long long rows = (long long)Nq * G, heads = (long long)B * Hk;
@@ -722,25 +735,24 @@ Plan make_plan(int B, int Nq, int Np, int Nk, int H, int Hk) {
         s.chunks = (int)((tiles + s.per_chunk - 1) / s.per_chunk);
         return s;
     }
-    auto deal = [](Deal& w, long long tiles_heads, int key_tiles, int least) {      // about 512 blocks, at least `least` key tiles each (256 or 512 keys: below, a joining launch costs more than it spreads)
-        const long long want = tiles_heads >= 384 ? 1 : (512 + tiles_heads - 1) / tiles_heads;
-        long long per = (key_tiles + want - 1) / want;
-        if (per < least) per = least;
+    auto deal = [](Deal& w, long long places, int key_tiles, int slots) {      // at least 4 tiles (256 or 512 keys): below, a joining launch costs more than it spreads
+        const long long per = dealt(places, key_tiles, slots, 4);
         w.splits = key_tiles > per ? (int)((key_tiles + per - 1) / per) : 1;
         w.per_split = (int)per;
-        w.blocks = (int)(tiles_heads * w.splits);
+        w.blocks = (int)(places * w.splits);
     };
     // a row tile of one sample alone would be mostly empty: the rows of all samples are stacked for the prefix, where that is long enough to pay for joining
     // (2^26 rows: what the joining launch takes)
     const bool few = rows <= 32, stack = Np >= 512 && rows < 128 && B > 1 && rows * heads < (1ll << 26);
     const bool stack_few = few && rows * B <= 32;
+    const int slots = d <= 64 ? 768 : 512;
     s.mode = !few ? MANY : (!stack || stack_few) ? FEW : MIXED;
     if (stack) {
         const int kt = stack_few ? 128 : 64;
         s.first.stacked = 1;
         s.first.np = Np;
         s.first.xtiles = stack_few ? 1 : (int)((rows * B + 127) / 128);
-        deal(s.first, (long long)Hk * s.first.xtiles, (Np + kt - 1) / kt, 4);
+        deal(s.first, (long long)Hk * s.first.xtiles, (Np + kt - 1) / kt, slots);
         s.parts = s.first.splits;
     }
     if (Nk > 0 || !stack) {
@@ -748,7 +760,7 @@ Plan make_plan(int B, int Nq, int Np, int Nk, int H, int Hk) {
         s.second.np = stack ? 0 : Np;
         s.second.xtiles = few ? 1 : (int)((rows + 127) / 128);
         s.second.part0 = s.parts;
-        deal(s.second, heads * s.second.xtiles, (Nk + kt - 1) / kt + (s.second.np + kt - 1) / kt, 4);
+        deal(s.second, heads * s.second.xtiles, (Nk + kt - 1) / kt + (s.second.np + kt - 1) / kt, slots);
         s.parts += s.second.splits;
     }
     if (s.parts == 1) s.parts = 0;
@@ -1227,17 +1239,7 @@ BwdPlan make_bwd_plan(int B, int Bk, int Nq, int Nk, int H, int Hk, int d) {
     s.fused = Nk <= 128;
     s.ktiles = (Nk + 127) / 128;
     const long long tiles = ((long long)Nq + 63) / 64 * (H / Hk) * (Bk < B ? B : 1), blocks = (long long)Bk * Hk * s.ktiles;
-    // The rows are dealt out in chunks where key tiles alone leave part of the chip idle: as many as make the rounds that its `slots` blocks take
-    // shortest (a block's first tile counts twice), at least two tiles each
-    const long long slots = s.fused && d > 64 ? 256 : 512;
-    long long best = tiles, cost = (blocks + slots - 1) / slots * (tiles + 1);
-    for (long long c = 2; blocks < 384 && c <= 512 && c <= tiles / 2; ++c) {
-        const long long per = (tiles + c - 1) / c, rounds = (blocks * ((tiles + per - 1) / per) + slots - 1) / slots;
-        if (rounds * (per + 1) < cost) {
-            cost = rounds * (per + 1);
-            best = per;
-        }
-    }
+    const long long best = dealt(blocks, tiles, s.fused && d > 64 ? 256 : 512, 2);
     s.per_chunk = (int)best;
     s.chunks = (int)((tiles + best - 1) / best);
     s.delta_floats = s.fused ? 0 : ((long long)B * H * Nq + 3) / 4 * 4;
@@ -1287,7 +1289,7 @@ extern "C" {
 
 int vidseg_context_attention_scratch_kib(int B, int Nq, int Np, int Nk, int H, int Hk, int d) {
     if (check_sizes("context_attention", 1, B, Nq, Np, Nk, H, Hk, d, 1.f)) return -1;
-    const Plan s = make_plan(B, Nq, Np, Nk, H, Hk);
+    const Plan s = make_plan(B, Nq, Np, Nk, H, Hk, d);
     return (int)(((long long)s.parts * B * Nq * H * (d + 2) * 4 + 1023) / 1024);
 }
 
@@ -1303,7 +1305,7 @@ int vidseg_context_attention_fwd(const void* q, long long q_b, long long q_n, lo
                    (Np == 0 || (row_strides_ok(k_prefix, 0, kp_n, kp_h) && row_strides_ok(v_prefix, 0, vp_n, vp_h))),
                "context_attention: operands must be 16-byte aligned with strides that are multiples of 8 elements (rows below 2^24 apart)");
     VS_REQUIRE(!(causal && mask), "context_attention: a causal call takes no key mask");
-    const Plan s = make_plan(B, Nq, Np, Nk, H, Hk);
+    const Plan s = make_plan(B, Nq, Np, Nk, H, Hk, d);
     const long long total = (long long)B * Nq * H;
     const long long need = ((long long)s.parts * total * (d + 2) * 4 + 1023) / 1024;
     VS_REQUIRE(need == 0 || (scratch && scratch_kib >= need), "context_attention: scratch of %lld KiB, needs %lld", scratch_kib, need);
