@@ -63,6 +63,10 @@ PREFIX = [  # B, Nq, Np, Nk, H, Hk, d, dtype, lens, causal
     (3, 40, 700, 64, 2, 2, 48, F16, (0, 64, 10), False),              # stacked rows, and more than 32 of their own
     (2, 1, 2600, 33, 4, 4, 80, BF16, (33, 2), True),                  # few rows in all, the prefix dealt out over blocks
     (1, 1, 5000, 2100, 2, 2, 64, F16, (2050,), True),                 # one sample: prefix and own keys in one walk
+    (70, 2, 500, 20, 4, 2, 64, BF16, None, True),                     # a prefix long enough to stack the rows: own rows few,
+    (3, 40, 11000, 64, 2, 2, 48, F16, (0, 64, 10), False),            # own rows many,
+    (2, 1, 17000, 33, 4, 4, 80, BF16, (33, 2), True),                 # few rows in all,
+    (45, 1, 900, 0, 6, 2, 104, F16, None, False),                     # no own keys
 ]
 
 

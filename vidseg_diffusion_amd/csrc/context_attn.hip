@@ -373,12 +373,12 @@ template <bool BF, int DP> __device__ __forceinline__ void many_rows(const AttnA
 }
 
 // Few rows (at most 32 per key head): the keys are what has to be read, so every wave walks over its own runs of 32 of them with all rows as
-// columns, no barrier in the loop.  K goes from memory straight into A operands (a lane reads its key's row); V passes through a piece of LDS
-// that only this wave uses, for the transpose.  The next 32 keys are in flight while these are worked on; the four waves' results are merged at the end.
+// columns, no barrier in the loop.  K and V pass through a piece of LDS that only this wave uses (read whole rows at a time).
+// The next 32 keys are in flight while these are worked on; the four waves' results are merged at the end.
 template <bool BF, int DP> __device__ __forceinline__ void few_rows(const AttnArgs& p, const Deal& w, unsigned block, u16* lds) {
     constexpr int SL = DP / 8, NV = 32 * SL / 64, ND = DP / 32;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, hi = lane >> 5;
-    u16* sV = lds + wave * 32 * DP;
+    u16 *sK = lds + wave * 64 * DP, *sV = sK + 32 * DP;
     const Place at = place_of(p, w, block);
     const int rows = at.rows;
     const Row row = row_of(p, at.b, at.hk, w.stacked, l31, rows);
@@ -387,30 +387,21 @@ template <bool BF, int DP> __device__ __forceinline__ void few_rows(const AttnAr
     const int len = at.len;                                           // causal: the last row sees all of them
     const int T0 = (w.np + 127) / 128, T1 = (len + 127) / 128;
     const int tb = min(at.split * w.per_split, T0 + T1), te = w.splits == 1 ? T0 + T1 : min(tb + w.per_split, T0 + T1);
-    u32x4 rk[DP / 16], rv[NV];
+    u32x4 rk[NV], rv[NV];
     const u16 *kown = p.k + at.b * p.k_b + at.hk * p.k_h, *vown = p.v + at.b * p.v_b + at.hk * p.v_h;
     const unsigned char* mrow = p.mask ? p.mask + at.b * p.mask_b : nullptr;
-    // the tile's first key, number of keys in its segment and this lane's key; a tile's last runs may lie behind the segment
+    // the tile's first key; a tile's last runs may lie behind the segment
     auto first = [&](int t) __attribute__((always_inline)) { return (t >= T0 ? t - T0 : t) * 128 + wave * 32; };
-    auto load_k = [&](int t) __attribute__((always_inline)) {
-        const bool own = t >= T0;
-        const int n = own ? len : w.np, kk = min(first(t) + l31, n - 1);
-        const u16* kb = (own ? kown : p.kp + at.hk * p.kp_h) + kk * (own ? p.k_n : p.kp_n);
-#pragma unroll
-        for (int s = 0; s < DP / 16; ++s) {
-            const int c = s * 16 + hi * 8;
-            rk[s] = *reinterpret_cast<const u32x4*>(kb + (c < p.d ? c : 0));
-        }
-    };
-    auto load_v = [&](int t) __attribute__((always_inline)) {
+    auto load = [&](int t) __attribute__((always_inline)) {
         const bool own = t >= T0;
         const int n = own ? len : w.np, k0 = first(t);
-        const u16* vb = own ? vown : p.vp + at.hk * p.vp_h;
-        const long long vn = own ? p.v_n : p.vp_n;
+        const u16 *kb = own ? kown : p.kp + at.hk * p.kp_h, *vb = own ? vown : p.vp + at.hk * p.vp_h;
+        const long long kn = own ? p.k_n : p.kp_n, vn = own ? p.v_n : p.vp_n;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int id = lane + 64 * i, c = id % SL * 8;
-            rv[i] = *reinterpret_cast<const u32x4*>(vb + min(k0 + id / SL, n - 1) * vn + (c < p.d ? c : 0));
+            const int id = lane + 64 * i, c = id % SL * 8, r = min(k0 + id / SL, n - 1);
+            rk[i] = *reinterpret_cast<const u32x4*>(kb + r * kn + (c < p.d ? c : 0));
+            rv[i] = *reinterpret_cast<const u32x4*>(vb + r * vn + (c < p.d ? c : 0));
         }
     };
     auto exists = [&](int t) -> unsigned {
@@ -426,38 +417,31 @@ template <bool BF, int DP> __device__ __forceinline__ void few_rows(const AttnAr
         for (int r = 0; r < 16; ++r) acc[n][r] = 0.f;
     unsigned bits = 0;
     if (tb < te) {
-        load_k(tb);
-        load_v(tb);
+        load(tb);
         bits = exists(tb);
     }
     for (int t = tb; t < te; ++t) {
         const unsigned now = bits;
         const bool more = t + 1 < te;
         if (more) bits = exists(t + 1);
-        // K of keys that do not exist and channels behind d are zero
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s)
-            if (s * 16 + hi * 8 >= p.d || !((now >> l31) & 1u)) rk[s] = u32x4{0u, 0u, 0u, 0u};
-        f32x16 s;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = 0.f;
-#pragma unroll
-        for (int e = 0; e < DP / 16; ++e) s = mfma<BF>(rk[e], fq[e], s);
-        if (more) load_k(t + 1);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
+        for (int i = 0; i < NV; ++i) {                                // keys that do not exist and channels behind d are zero
             const int id = lane + 64 * i, r = id / SL, slot = id % SL;
-            if (slot * 8 >= p.d || !((now >> r) & 1u)) rv[i] = u32x4{0u, 0u, 0u, 0u};
+            if (slot * 8 >= p.d || !((now >> r) & 1u)) rk[i] = rv[i] = u32x4{0u, 0u, 0u, 0u};
+            *reinterpret_cast<u32x4*>(sK + slot_at<DP>(r, slot)) = rk[i];
             *reinterpret_cast<u32x4*>(sV + slot_at<DP>(r, slot)) = rv[i];
         }
-        if (more) load_v(t + 1);
+        if (more) load(t + 1);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");        // the other lanes' rows are in place (a wave's LDS operations keep their order)
+        __builtin_amdgcn_wave_barrier();
+        f32x16 s = zero16();
+#pragma unroll
+        for (int e = 0; e < DP / 16; ++e) s = mfma<BF>(read_row<DP>(sK, l31, e * 2 + hi), fq[e], s);
         const int k0 = first(t);
         const bool edge = p.causal && t >= T0 && k0 + 32 > len - p.Nq + 1;
         if (now != ~0u || edge) hide(s, now, edge ? len - p.Nq + row.qi - k0 - 4 * hi : 1 << 30, hi);
         u32x4 fp[2];
         soften<BF, ND>(s, p.c, m, l, acc, fp);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");        // the other lanes' V rows are in place (a wave's LDS operations keep their order)
-        __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -741,9 +725,12 @@ Plan make_plan(int B, int Nq, int Np, int Nk, int H, int Hk, int d) {
         w.per_split = (int)per;
         w.blocks = (int)(places * w.splits);
     };
-    // a row tile of one sample alone would be mostly empty: the rows of all samples are stacked for the prefix, where that is long enough to pay for joining
-    // (2^26 rows: what the joining launch takes)
-    const bool few = rows <= 32, stack = Np >= 512 && rows < 128 && B > 1 && rows * heads < (1ll << 26);
+    // Few rows: where a wave's 32 columns hold all rows of a key head the keys are what has to be read, and k_ctx_attn's few_rows reads them faster
+    // (64 samples of 16 rows over 2000 keys, 16 heads of 64: 111 us, 4.7 TB/s, for 124 as many_rows; 256 samples over 77 keys 33 us for 51).
+    // Stacked: a row tile of one sample alone would be mostly empty, so the rows of all samples share row tiles for the prefix, where what that saves
+    // pays for the joining launch (single tokens, stacked / each sample by itself: 64 samples over 1024 prefix keys 42.8 / 48.1 us, over 512 38.4 / 37.0;
+    // 4 over 16384 23.7 / 48.2, over 512 23.5 / 19.8; 1024 over 64 59.4 / 63.2).  2^26 rows are what the joining launch takes.
+    const bool few = rows <= 32, stack = B > 1 && rows < 128 && (long long)B * Np >= 32768 && rows * heads < (1ll << 26);
     const bool stack_few = few && rows * B <= 32;
     const int slots = d <= 64 ? 768 : 512;
     s.mode = !few ? MANY : (!stack || stack_few) ? FEW : MIXED;
