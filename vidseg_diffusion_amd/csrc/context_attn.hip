@@ -9,6 +9,10 @@
 // probabilities already lie in the order in which the second product takes its B operand (the k order of an MFMA is free as long as A
 // uses the same: V^T is fetched with the transpose read in that order).  Keys that do not exist are zeroed while they are staged (a NaN
 // there reaches nothing) and their scores are -inf.
+//
+// What bounds the products: a wave's 32 columns use every A operand that LDS gives (1 KB, 8 clocks of its 128 B) for one MFMA of 32 clocks, on four SIMDs at
+// once: LDS and the matrix pipes are full together.  64 columns a wave would halve the reads, but its accumulators leave one wave a SIMD, which
+// waits more than it saves (measured slower at every size).  Rates below are of the products that the formulas need.
 #include "common.h"
 
 namespace {
@@ -273,7 +277,10 @@ __device__ __forceinline__ void hide(f32x16& s, unsigned bits, int lim, int hi) 
     }
 }
 
-// Many rows: the block's four waves own 32 rows each and share key tiles of 64 in LDS, fetched one tile ahead.
+// Many rows: the block's four waves own 32 rows each and share key tiles of 64 in LDS, fetched one tile ahead.  14 x 5 heads x 4096 rows x 8192 keys of 64
+// (fp16) 650 us, 925 TFLOP/s; 2 x 16 heads x 4096 x 4096 of 128 (bf16) 294 us, 935 TFLOP/s; a large library product reaches 1250 on the same card.
+// Single tokens of 64 samples over a prefix of 16384, 32 heads of 128 on 8: 41 us alone, 420 TFLOP/s -- 8 tiles a block, too few to hide a block's
+// start and its partial results (68 MB in all).
 template <bool BF, int DP> __device__ __forceinline__ void many_rows(const AttnArgs& p, const Deal& w, unsigned block, u16* lds) {
     constexpr int KT = 64, ND = DP / 32, TILE = KT * DP, BR = 128;
     u16 *sK = lds, *sV = lds + 2 * TILE;                              // two buffers each
@@ -373,7 +380,8 @@ template <bool BF, int DP> __device__ __forceinline__ void many_rows(const AttnA
 }
 
 // Few rows (at most 32 per key head): the keys are what has to be read, so every wave walks over its own runs of 32 of them with all rows as
-// columns, no barrier in the loop.  K and V pass through a piece of LDS that only this wave uses (read whole rows at a time).
+// columns, no barrier in the loop.  64 samples of one query over 2000 keys, 16 heads of 64 (fp16): 111 us, 4.7 TB/s; 32 over 5000, 8 heads of 128: 125 us,
+// 5.2 TB/s, the rate of a large copy (K read row by row into the operands, past LDS: 128 and 136 us, every line fetched four times).  K and V pass through a piece of LDS that only this wave uses (read whole rows at a time).
 // The next 32 keys are in flight while these are worked on; the four waves' results are merged at the end.
 template <bool BF, int DP> __device__ __forceinline__ void few_rows(const AttnArgs& p, const Deal& w, unsigned block, u16* lds) {
     constexpr int SL = DP / 8, NV = 32 * SL / 64, ND = DP / 32;
@@ -517,7 +525,8 @@ template <bool BF, int DP, int MODE> __global__ void __launch_bounds__(256, MODE
 
 // A context of at most 128 keys and many rows: the rows are what has to be read and written.  The block keeps every key of its key head in LDS and each wave
 // walks over tiles of 32 rows by itself, the next tile's queries in flight; all scores of a row are there at once, so nothing is rescaled.  Keys that do not
-// exist enter through the first product's accumulator, which starts at -inf for them (0 for the others).
+// exist enter through the first product's accumulator, which starts at -inf for them (0 for the others).  28 x 4096 rows x 77 keys, 5 heads of 64 (fp16):
+// 47 us with fresh inputs (3.1 TB/s; a copy of the same bytes 29), 32 us with inputs in the last-level cache: products and exponentials take as long as the bytes.
 template <bool BF, int DP> __global__ void __launch_bounds__(256, DP == 64 ? 3 : 2) k_ctx_short(AttnArgs p, int chunks, int per_chunk) {
     constexpr int SL = DP / 8, NST = 128 * SL / 256, ND = DP / 32;
     __shared__ __attribute__((aligned(16))) u16 sK[128 * DP], sV[128 * DP];
@@ -694,6 +703,7 @@ struct Plan {
 };
 // `tiles` tiles of work in each of `blocks` places: how many of them a block takes.  Where the places alone leave part of the chip idle the tiles are dealt
 // out in runs: as many as make the rounds that `slots` resident blocks take shortest (a block's start and its partial results count as two tiles), at least `least` tiles each
+// (2 x 1000 rows x 4000 keys, 10 heads of 128: 3 runs, 480 blocks, 65 us; 4 runs, 640 blocks in two rounds, 77 us)
 long long dealt(long long blocks, long long tiles, long long slots, long long least) {
     long long best = tiles, cost = (blocks + slots - 1) / slots * (tiles + 2);
     for (long long c = 2; blocks < 384 && c <= 512 && c * least <= tiles; ++c) {
@@ -710,6 +720,8 @@ Plan make_plan(int B, int Nq, int Np, int Nk, int H, int Hk, int d) {
     const int G = H / Hk;
     const long long rows = (long long)Nq * G, heads = (long long)B * Hk;
     if (Np == 0 && Nk <= 128 && rows >= 64) {
+        // (k_ctx_short / k_ctx_attn: 28 x 4096 rows, 5 heads of 64, 77 keys 49 / 59 us, 128 keys 51 / 55; 14 x 4096, 8 heads of 128, 77 keys 64 / 82;
+        // 256 x 64 rows, 16 heads of 64 39 / 47)
         // the keys are staged once a block: one round of the 768 blocks that the chip holds (heads up to 64), or, from half of that in heads alone, rounds of
         // blocks small enough for the last one to weigh little; at least two tiles a wave
         const long long tiles = (rows + 31) / 32, want = heads <= 384 ? 768 / heads : (4 * 768 + heads - 1) / heads;
@@ -796,7 +808,8 @@ constexpr float P_LOG2 = 12.f, P_BACK = 2.44140625e-4f;                         
 __device__ __forceinline__ float power_for(float m) { return __uint_as_float((254u - max(67u, min(__float_as_uint(m) >> 23, 253u))) << 23); }
 
 // dq: a wave owns 32 rows as accumulator columns, the block's waves share key tiles of 64 (the forward kernel's arrangement); K serves as rows (scores)
-// and transposed (ds k).  D comes out of the saved result: o was rounded, o_lo holds what the rounding left.
+// and transposed (ds k).  Three products: 2 x 16 heads x 4096 x 4096 of 128 (bf16) 381 us, 1080 TFLOP/s; 4 x 10 heads x 1456 x 2311 of 64 (fp16) 79 us, 655
+// (480 blocks: two on most CUs where three would fit).  D comes out of the saved result: o was rounded, o_lo holds what the rounding left.
 template <bool BF, int DP> __global__ void __launch_bounds__(256, DP == 64 ? 3 : 2) k_ctx_bwd_q(BwdArgs p) {
     constexpr int KT = 64, ND = DP / 32, TILE = KT * DP;
     __shared__ __attribute__((aligned(16))) u16 sK[2 * TILE], sV[2 * TILE];
@@ -930,6 +943,8 @@ __device__ __forceinline__ float rows_sum(const f32x16& x, int lane) {
 // here from the unrounded p dp (four partial sums a row through LDS) and dq comes out of the same pass -- ds goes through LDS once more, each wave takes
 // its share of the [64][d] tile of ds k -- and q and do are all that is read per row.
 // DV, DK: which of the two the block accumulates.
+// FUSED 28 x 4096 rows x 77 keys, 5 heads of 64, forward and gradients: 179 us bf16, as three passes 218; 14 x 4096, 8 heads of 128: 265 and 354.
+// Not FUSED, 4 x 10 heads x 1456 x 2311 of 64 (fp16): 111 us, 620 TFLOP/s; 2 x 16 heads on 4 x 4096 x 4096 of 128 (bf16): 849 us, 650.
 template <int DP, bool FUSED> struct BwdLds {
     __attribute__((aligned(16))) u16 q[2 * 64 * DP], g[2 * 64 * DP], k[FUSED ? 128 * DP : 8], s[FUSED ? 128 * 64 : 8];
     __attribute__((aligned(16))) float l[2][64], d[FUSED ? 4 : 2][64], m[4];
@@ -1188,7 +1203,8 @@ template <bool BF, int DP, bool FUSED, bool DV, bool DK> __device__ __forceinlin
 }
 
 // Wide heads, not FUSED: the accumulators of both gradients and K, V leave room for one wave a SIMD only, which waits more than it works; so half of the
-// blocks take dk and the other half dv (five products for four, at two waves a SIMD).
+// blocks take dk and the other half dv (five products for four, at two waves a SIMD).  Forward and gradients, separate / together: 4 x 10 heads x 1456 x 2311
+// of 96 bf16 356 / 376 us, of 128 fp16 460 / 479, bf16 432 / 422; 2 x 16 heads on 4 x 4096 x 4096 of 128 fp16 1589 / 1675, bf16 1470 / 1450.
 template <bool BF, int DP, bool FUSED> __global__ void __launch_bounds__(256, DP == 64 || !FUSED ? 2 : 1) k_ctx_bwd_kv(BwdArgs p) {
     __shared__ BwdLds<DP, FUSED> lds;
     int y, kt;
