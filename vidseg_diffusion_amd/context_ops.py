@@ -7,7 +7,8 @@
 
 Unlike the `*_a16` operators of ops.py, which run in the library's one 16-bit type, these take the type of their tensors.  They launch
 asynchronously on torch's current stream of the tensors' device; scratch memory comes from torch's allocator call by call, so two streams
-or two captured graphs never share any.
+or two captured graphs never share any.  A backward pass can be captured too, on leaves of which no eager graph is alive: torch ties a leaf's
+gradient to the stream on which the leaf was first used, and a captured pass cannot wait for another stream.
 """
 from __future__ import annotations
 
