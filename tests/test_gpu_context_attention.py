@@ -226,3 +226,29 @@ def test_streams_and_graph():
         torch.cuda.synchronize()
         want = ops.prefix_attention(q, kp, vp, k, v, H, k_lens=lens), ops.cross_attention(q, k, v, H, k_lens=lens)
         assert all(torch.equal(a, b) for o in outs for a, b in zip(o, want))
+
+
+def test_graphs_of_stacked_rows():
+    """Single tokens of many samples behind a prefix long enough to be dealt out and joined: two captured graphs in flight on two streams, each with its own scratch."""
+    dev = torch.device("cuda:0")
+    B, H, d = 40, 4, 64
+    q, k, v = (randn((B, n, H * d), s, BF16).to(dev) for n, s in ((1, 1), (70, 2), (70, 3)))
+    kp, vp = (randn((3000, H * d), s, BF16).to(dev) for s in (4, 5))
+    lens = torch.full((B,), 70, dtype=torch.int32, device=dev)
+    graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(ops.prefix_attention(q, kp, vp, k, v, H, k_lens=lens, causal=True))
+        graphs.append(g)
+    for seed in (11, 12, 13):
+        q.copy_(randn(q.shape, seed, BF16))
+        lens.copy_(torch.randint(0, 71, (B,), generator=torch.Generator().manual_seed(seed), dtype=torch.int32))
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        want = ops.prefix_attention(q, kp, vp, k, v, H, k_lens=lens, causal=True)
+        assert all(torch.equal(o, want) for o in outs)
+        Reference(q, k, v, H, None, lens, None, None, kp, vp, True).check(want)

@@ -706,7 +706,10 @@ struct Plan {
 // (2 x 1000 rows x 4000 keys, 10 heads of 128: 3 runs, 480 blocks, 65 us; 4 runs, 640 blocks in two rounds, 77 us)
 long long dealt(long long blocks, long long tiles, long long slots, long long least) {
     long long best = tiles, cost = (blocks + slots - 1) / slots * (tiles + 2);
-    for (long long c = 2; blocks < 384 && c <= 512 && c * least <= tiles; ++c) {
+    for (int r = 1; blocks < 384 && r <= 8; ++r) {                    // as many runs as r rounds hold
+        long long c = r * slots / blocks;
+        if (c > tiles / least) c = tiles / least;
+        if (c < 2) continue;
         const long long per = (tiles + c - 1) / c, rounds = (blocks * ((tiles + per - 1) / per) + slots - 1) / slots;
         if (rounds * (per + 2) < cost) {
             cost = rounds * (per + 2);
