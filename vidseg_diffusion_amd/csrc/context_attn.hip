@@ -526,29 +526,60 @@ template <bool BF, int DP, int MODE> __global__ void __launch_bounds__(256, MODE
 // A context of at most 128 keys and many rows: the rows are what has to be read and written.  The block keeps every key of its key head in LDS and each wave
 // walks over tiles of 32 rows by itself, the next tile's queries in flight; all scores of a row are there at once, so nothing is rescaled.  Keys that do not
 // exist enter through the first product's accumulator, which starts at -inf for them (0 for the others).  28 x 4096 rows x 77 keys, 5 heads of 64 (fp16):
-// 47 us with fresh inputs (3.1 TB/s; a copy of the same bytes 29), 32 us with inputs in the last-level cache: products and exponentials take as long as the bytes.
-template <bool BF, int DP> __global__ void __launch_bounds__(256, DP == 64 ? 3 : 2) k_ctx_short(AttnArgs p, int chunks, int per_chunk) {
-    constexpr int SL = DP / 8, NST = 128 * SL / 256, ND = DP / 32;
-    __shared__ __attribute__((aligned(16))) u16 sK[128 * DP], sV[128 * DP];
-    __shared__ __attribute__((aligned(16))) float sE[128];
+// 36 us with fresh inputs (4.1 TB/s; a copy of the same bytes 29).  KEYS: 96 where the context is no longer, which leaves registers for three waves a SIMD
+// (128 alone: 40 us; 120 keys at three waves, spilling, 58 us for 50.6 at two).
+template <bool BF, int DP, int KEYS> __global__ void __launch_bounds__(256, DP == 64 && KEYS == 96 ? 3 : 2) k_ctx_short(AttnArgs p, int chunks, int per_chunk) {
+    constexpr int SL = DP / 8, NST = (KEYS * SL + 255) / 256, ND = DP / 32;
+    __shared__ __attribute__((aligned(16))) u16 sK[KEYS * DP], sV[KEYS * DP];
+    __shared__ __attribute__((aligned(16))) float sE[KEYS];
+    // A lane computes one row, but memory wants whole rows an instruction (each lane its own row, 32 bytes of a line at a time: 28 x 4096 x 77 keys 49 us for
+    // 36, 33 keys 46 for 31): queries and results change places through a piece of LDS of this wave's own.  Heads over 96 wide leave no room for
+    // it beside a second block.
+    constexpr bool STAGED = DP <= 96;
+    __shared__ __attribute__((aligned(16))) u16 sT[STAGED ? 4 * 32 * DP : 8];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, hi = lane >> 5;
     int y, chunk;
     block_of(chunks, y, chunk);
     const int hk = y % p.Hk, b = y / p.Hk, rows = p.Nq * p.G;
     const int t1 = min((chunk + 1) * per_chunk, (rows + 31) / 32), t0 = chunk * per_chunk + wave;
-    // whole tiles of a head that fills its registers, no groups: uniform base and one offset a lane, for queries and results
-    const bool plain = p.G == 1 && p.d == DP;
-    const unsigned q_off = (unsigned)(l31 * (int)p.q_n + hi * 8) * 2u, o_off = (unsigned)(l31 * p.H * p.d + hi * 8) * 2u;
+    const bool plain = p.G == 1;                                     // whole tiles without groups: uniform base, offsets below 2^32
     const u16* q0 = p.q + b * p.q_b + hk * p.q_h;
-    u16* o0 = p.o + ((long long)b * p.Nq * p.H + hk) * p.d;
+    u16 *o0 = p.o + ((long long)b * p.Nq * p.H + hk) * p.d, *mine = sT + (STAGED ? wave * 32 * DP : 0);
     u32x4 fq[DP / 16];
+    auto in_order = [&]() __attribute__((always_inline)) {           // what the wave's other lanes wrote is there (its LDS operations keep their order)
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    };
+    // piece i of a lane: 16 bytes at (row, slot) of the tile
+    auto row_at = [&](int i) __attribute__((always_inline)) { return (lane + 64 * i) / SL; };
+    auto slot_of = [&](int i) __attribute__((always_inline)) { return (lane + 64 * i) % SL; };
     auto queries = [&](int t) __attribute__((always_inline)) {
-        if (plain && t * 32 + 32 <= rows) {
+        if constexpr (!STAGED) {
+            load_q<DP>(p, row_of(p, b, hk, false, t * 32 + l31, rows), hi, fq);
+        } else if (plain && t * 32 + 32 <= rows) {
             const char* at = reinterpret_cast<const char*>(q0 + t * 32 * p.q_n);
 #pragma unroll
-            for (int s = 0; s < DP / 16; ++s) fq[s] = *reinterpret_cast<const u32x4*>(at + q_off + s * 32);
+            for (int i = 0; i < DP / 16; ++i) {
+                const int c = slot_of(i) * 8;
+                fq[i] = *reinterpret_cast<const u32x4*>(at + (unsigned)(row_at(i) * (int)p.q_n + (c < p.d ? c : 0)) * 2u);
+            }
         } else {
-            load_q<DP>(p, row_of(p, b, hk, false, t * 32 + l31, rows), hi, fq);
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i) {
+                const Row row = row_of(p, b, hk, false, t * 32 + row_at(i), rows);
+                const int c = slot_of(i) * 8;
+                fq[i] = *reinterpret_cast<const u32x4*>(p.q + b * p.q_b + row.qi * p.q_n + row.h * p.q_h + (c < p.d ? c : 0));
+            }
+        }
+    };
+    auto settle = [&]() __attribute__((always_inline)) {
+        if constexpr (STAGED) {
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i) *reinterpret_cast<u32x4*>(mine + slot_at<DP>(row_at(i), slot_of(i))) = slot_of(i) * 8 < p.d ? fq[i] : u32x4{0u, 0u, 0u, 0u};
+            in_order();
+#pragma unroll
+            for (int e = 0; e < DP / 16; ++e) fq[e] = read_row<DP>(mine, l31, e * 2 + hi);
+            in_order();
         }
     };
     if (t0 < t1) queries(t0);
@@ -567,8 +598,8 @@ template <bool BF, int DP> __global__ void __launch_bounds__(256, DP == 64 ? 3 :
         *reinterpret_cast<u32x4*>(sK + slot_at<DP>(r, slot)) = rk;
         *reinterpret_cast<u32x4*>(sV + slot_at<DP>(r, slot)) = rv;
     }
-    const bool exists = tid < min(len, 128) && (!mk || mk[tid]);
-    if (tid < 128) sE[tid] = exists ? 0.f : -INFINITY;
+    const bool exists = tid < min(len, KEYS) && (!mk || mk[tid]);
+    if (tid < KEYS) sE[tid] = exists ? 0.f : -INFINITY;
     if (!__syncthreads_or(exists)) {                                  // no key at all: zeros, whatever the queries hold
         for (int t = t0; t < t1; t += 4) {
             const Row row = row_of(p, b, hk, false, t * 32 + l31, rows);
@@ -579,6 +610,7 @@ template <bool BF, int DP> __global__ void __launch_bounds__(256, DP == 64 ? 3 :
         }
         return;
     }
+    if (t0 < t1) settle();
     auto walk = [&](auto which) __attribute__((always_inline)) {
         constexpr int NH = decltype(which)::value, NJ = (NH + 1) / 2; // half blocks of 16 keys, which an accumulator's first and last eight registers hold; blocks of 32
         for (int t = t0; t < t1; t += 4) {
@@ -622,20 +654,33 @@ template <bool BF, int DP> __global__ void __launch_bounds__(256, DP == 64 ? 3 :
             }
             l = half_sum(l);
             const float inv = l > 0.f ? __builtin_amdgcn_rcpf(l) : 0.f;
-            if (plain && t * 32 + 32 <= rows) {
-                char* at = reinterpret_cast<char*>(o0 + (long long)t * 32 * p.H * p.d);
+            const Row row = row_of(p, b, hk, false, t * 32 + l31, rows);
+            if (p.lse && hi == 0 && row.on) p.lse[((long long)b * p.H + row.h) * p.Nq + row.qi] = (m + __builtin_amdgcn_logf(l)) * LN2;
+            if constexpr (!STAGED) {
+                const long long id = ((long long)b * p.Nq + row.qi) * p.H + row.h;
+#pragma unroll
+                for (int n = 0; n < ND; ++n) store_row<BF>(p.o + id * p.d, acc[n], inv, n, hi, p.d, row.on);
+            } else {
 #pragma unroll
                 for (int n = 0; n < ND; ++n)
 #pragma unroll
-                    for (int g = 0; g < 2; ++g) *reinterpret_cast<u32x4*>(at + o_off + n * 64 + g * 32) = eight<BF>(acc[n], inv, g);
-                if (p.lse && hi == 0) p.lse[((long long)b * p.H + hk) * p.Nq + t * 32 + l31] = (m + __builtin_amdgcn_logf(l)) * LN2;
-                continue;
-            }
-            const Row row = row_of(p, b, hk, false, t * 32 + l31, rows);
-            const long long id = ((long long)b * p.Nq + row.qi) * p.H + row.h;
+                    for (int g = 0; g < 2; ++g) *reinterpret_cast<u32x4*>(mine + slot_at<DP>(l31, n * 4 + g * 2 + hi)) = eight<BF>(acc[n], inv, g);
+                in_order();
+                const bool whole = plain && t * 32 + 32 <= rows;
+                char* at = reinterpret_cast<char*>(o0 + (long long)t * 32 * p.H * p.d);
 #pragma unroll
-            for (int n = 0; n < ND; ++n) store_row<BF>(p.o + id * p.d, acc[n], inv, n, hi, p.d, row.on);
-            if (p.lse && hi == 0 && row.on) p.lse[((long long)b * p.H + row.h) * p.Nq + row.qi] = (m + __builtin_amdgcn_logf(l)) * LN2;
+                for (int i = 0; i < DP / 16; ++i) {
+                    const u32x4 x = read_row<DP>(mine, row_at(i), slot_of(i));
+                    if (whole) {
+                        if (slot_of(i) * 8 < p.d) *reinterpret_cast<u32x4*>(at + (unsigned)(row_at(i) * p.H * p.d + slot_of(i) * 8) * 2u) = x;
+                    } else {
+                        const Row to = row_of(p, b, hk, false, t * 32 + row_at(i), rows);
+                        if (to.on && slot_of(i) * 8 < p.d) *reinterpret_cast<u32x4*>(p.o + (((long long)b * p.Nq + to.qi) * p.H + to.h) * p.d + slot_of(i) * 8) = x;
+                    }
+                }
+                in_order();
+            }
+            if (t + 4 < t1) settle();
         }
     };
     switch (halves) {
@@ -645,8 +690,11 @@ template <bool BF, int DP> __global__ void __launch_bounds__(256, DP == 64 ? 3 :
         case 4: walk(Const<4>{}); break;
         case 5: walk(Const<5>{}); break;
         case 6: walk(Const<6>{}); break;
-        case 7: walk(Const<7>{}); break;
-        default: walk(Const<8>{});
+        default:
+            if constexpr (KEYS > 96) {
+                if (halves == 7) walk(Const<7>{});
+                else walk(Const<8>{});
+            }
     }
 }
 
@@ -723,7 +771,7 @@ Plan make_plan(int B, int Nq, int Np, int Nk, int H, int Hk, int d) {
     const int G = H / Hk;
     const long long rows = (long long)Nq * G, heads = (long long)B * Hk;
     if (Np == 0 && Nk <= 128 && rows >= 64) {
-        // (k_ctx_short / k_ctx_attn: 28 x 4096 rows, 5 heads of 64, 77 keys 49 / 59 us, 128 keys 51 / 55; 14 x 4096, 8 heads of 128, 77 keys 64 / 82;
+        // (k_ctx_short / k_ctx_attn: 28 x 4096 rows, 5 heads of 64, 77 keys 36 / 59 us, 128 keys 51 / 55; 14 x 4096, 8 heads of 128, 77 keys 64 / 82;
         // 256 x 64 rows, 16 heads of 64 39 / 47)
         // the keys are staged once a block: one round of the 768 blocks that the chip holds (heads up to 64), or, from half of that in heads alone, rounds of
         // blocks small enough for the last one to weigh little; at least two tiles a wave
@@ -771,7 +819,9 @@ Plan make_plan(int B, int Nq, int Np, int Nk, int H, int Hk, int d) {
 
 template <bool BF, int DP> void launch_fwd(const AttnArgs& p, const Plan& s, hipStream_t st) {
     if (s.one_pass) {
-        hipLaunchKernelGGL((k_ctx_short<BF, DP>), dim3((unsigned)((long long)s.chunks * p.B * p.Hk)), dim3(256), 0, st, p, s.chunks, s.per_chunk);
+        const dim3 grid((unsigned)((long long)s.chunks * p.B * p.Hk));
+        if (p.Nk <= 96) hipLaunchKernelGGL((k_ctx_short<BF, DP, 96>), grid, dim3(256), 0, st, p, s.chunks, s.per_chunk);
+        else hipLaunchKernelGGL((k_ctx_short<BF, DP, 128>), grid, dim3(256), 0, st, p, s.chunks, s.per_chunk);
         return;
     }
     const dim3 grid((unsigned)(s.first.blocks + s.second.blocks));
