@@ -526,7 +526,7 @@ template <bool BF, int DP, int MODE> __global__ void __launch_bounds__(256, MODE
 // A context of at most 128 keys and many rows: the rows are what has to be read and written.  The block keeps every key of its key head in LDS and each wave
 // walks over tiles of 32 rows by itself, the next tile's queries in flight; all scores of a row are there at once, so nothing is rescaled.  Keys that do not
 // exist enter through the first product's accumulator, which starts at -inf for them (0 for the others).  28 x 4096 rows x 77 keys, 5 heads of 64 (fp16):
-// 36 us with fresh inputs (4.1 TB/s; a copy of the same bytes 29).  KEYS: 96 where the context is no longer, which leaves registers for three waves a SIMD
+// 33.5 to 36 us with fresh inputs (4.1 to 4.5 TB/s; a copy of the same bytes 29).  KEYS: 96 where the context is no longer, which leaves registers for three waves a SIMD
 // (128 alone: 40 us; 120 keys at three waves, spilling, 58 us for 50.6 at two).
 template <bool BF, int DP, int KEYS> __global__ void __launch_bounds__(256, DP == 64 && KEYS == 96 ? 3 : 2) k_ctx_short(AttnArgs p, int chunks, int per_chunk) {
     constexpr int SL = DP / 8, NST = (KEYS * SL + 255) / 256, ND = DP / 32;
