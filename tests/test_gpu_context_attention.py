@@ -27,6 +27,9 @@ CROSS = [  # B, Nq, Nk, H, Hk, d, dtype, lens, shared context
     (1, 128, 64, 2, 2, 64, BF16, None, False),                 # exact tiles
     (2, 40, 0, 2, 2, 64, F16, None, False),                    # no keys at all
     (9, 3, 64, 8, 8, 16, F16, (64, 63, 33, 32, 31, 1, 0, 64, 5), False),
+    (2, 130, 96, 3, 3, 80, F16, (96, 81), False),                     # around the longest context that one block holds
+    (2, 130, 97, 3, 3, 128, BF16, (97, 96), False),
+    (3, 70, 85, 6, 2, 40, F16, (85, 16, 17), True),
 ]
 
 

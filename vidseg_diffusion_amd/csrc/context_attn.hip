@@ -523,15 +523,15 @@ template <bool BF, int DP, int MODE> __global__ void __launch_bounds__(256, MODE
     else few_rows<BF, DP>(p, w, block, lds);
 }
 
-// A context of at most 128 keys and many rows: the rows are what has to be read and written.  The block keeps every key of its key head in LDS and each wave
+// A context of at most 96 keys and many rows: the rows are what has to be read and written.  The block keeps every key of its key head in LDS and each wave
 // walks over tiles of 32 rows by itself, the next tile's queries in flight; all scores of a row are there at once, so nothing is rescaled.  Keys that do not
 // exist enter through the first product's accumulator, which starts at -inf for them (0 for the others).  28 x 4096 rows x 77 keys, 5 heads of 64 (fp16):
-// 33.5 to 36 us with fresh inputs (4.1 to 4.5 TB/s; a copy of the same bytes 29).  KEYS: 96 where the context is no longer, which leaves registers for three waves a SIMD
-// (128 alone: 40 us; 120 keys at three waves, spilling, 58 us for 50.6 at two).
-template <bool BF, int DP, int KEYS> __global__ void __launch_bounds__(256, DP == 64 && KEYS == 96 ? 3 : 2) k_ctx_short(AttnArgs p, int chunks, int per_chunk) {
-    constexpr int SL = DP / 8, NST = (KEYS * SL + 255) / 256, ND = DP / 32;
-    __shared__ __attribute__((aligned(16))) u16 sK[KEYS * DP], sV[KEYS * DP];
-    __shared__ __attribute__((aligned(16))) float sE[KEYS];
+// 33.5 to 41 us with fresh inputs (3.7 to 4.5 TB/s; a copy of the same bytes 29).  96 keys leave registers for three waves a SIMD.
+constexpr int SHORT = 96;
+template <bool BF, int DP> __global__ void __launch_bounds__(256, DP == 64 ? 3 : 2) k_ctx_short(AttnArgs p, int chunks, int per_chunk) {
+    constexpr int SL = DP / 8, NST = (SHORT * SL + 255) / 256, ND = DP / 32;
+    __shared__ __attribute__((aligned(16))) u16 sK[SHORT * DP], sV[SHORT * DP];
+    __shared__ __attribute__((aligned(16))) float sE[SHORT];
     // A lane computes one row, but memory wants whole rows an instruction (each lane its own row, 32 bytes of a line at a time: 28 x 4096 x 77 keys 49 us for
     // 36, 33 keys 46 for 31): queries and results change places through a piece of LDS of this wave's own.  Heads over 96 wide leave no room for
     // it beside a second block.
@@ -598,8 +598,8 @@ template <bool BF, int DP, int KEYS> __global__ void __launch_bounds__(256, DP =
         *reinterpret_cast<u32x4*>(sK + slot_at<DP>(r, slot)) = rk;
         *reinterpret_cast<u32x4*>(sV + slot_at<DP>(r, slot)) = rv;
     }
-    const bool exists = tid < min(len, KEYS) && (!mk || mk[tid]);
-    if (tid < KEYS) sE[tid] = exists ? 0.f : -INFINITY;
+    const bool exists = tid < min(len, SHORT) && (!mk || mk[tid]);
+    if (tid < SHORT) sE[tid] = exists ? 0.f : -INFINITY;
     if (!__syncthreads_or(exists)) {                                  // no key at all: zeros, whatever the queries hold
         for (int t = t0; t < t1; t += 4) {
             const Row row = row_of(p, b, hk, false, t * 32 + l31, rows);
@@ -689,12 +689,7 @@ template <bool BF, int DP, int KEYS> __global__ void __launch_bounds__(256, DP =
         case 3: walk(Const<3>{}); break;
         case 4: walk(Const<4>{}); break;
         case 5: walk(Const<5>{}); break;
-        case 6: walk(Const<6>{}); break;
-        default:
-            if constexpr (KEYS > 96) {
-                if (halves == 7) walk(Const<7>{});
-                else walk(Const<8>{});
-            }
+        default: walk(Const<6>{});
     }
 }
 
@@ -770,9 +765,10 @@ Plan make_plan(int B, int Nq, int Np, int Nk, int H, int Hk, int d) {
     Plan s{};
     const int G = H / Hk;
     const long long rows = (long long)Nq * G, heads = (long long)B * Hk;
-    if (Np == 0 && Nk <= 128 && rows >= 64) {
-        // (k_ctx_short / k_ctx_attn: 28 x 4096 rows, 5 heads of 64, 77 keys 36 / 59 us, 128 keys 51 / 55; 14 x 4096, 8 heads of 128, 77 keys 64 / 82;
-        // 256 x 64 rows, 16 heads of 64 39 / 47)
+    if (Np == 0 && Nk <= SHORT && rows >= 64) {
+        // (k_ctx_short / k_ctx_attn: 28 x 4096 rows, 5 heads of 64, 33 keys 31 / 44 us, 77 keys 36 to 41 / 58, 96 keys 40 / 55; 14 x 4096, 8 heads, 77 keys of 96
+        // 50 / 68, of 128 70 / 79; 256 x 64 rows, 16 heads of 64 39 / 47.  With room for 128 keys, 120 of them: of 64 51 / 54, of 96 76 / 75, of 128 94 / 82;
+        // 28 x 1024 rows, 10 heads of 64 28.6 / 27.6)
         // the keys are staged once a block: one round of the 768 blocks that the chip holds (heads up to 64), or, from half of that in heads alone, rounds of
         // blocks small enough for the last one to weigh little; at least two tiles a wave
         const long long tiles = (rows + 31) / 32, want = heads <= 384 ? 768 / heads : (4 * 768 + heads - 1) / heads;
@@ -820,8 +816,7 @@ Plan make_plan(int B, int Nq, int Np, int Nk, int H, int Hk, int d) {
 template <bool BF, int DP> void launch_fwd(const AttnArgs& p, const Plan& s, hipStream_t st) {
     if (s.one_pass) {
         const dim3 grid((unsigned)((long long)s.chunks * p.B * p.Hk));
-        if (p.Nk <= 96) hipLaunchKernelGGL((k_ctx_short<BF, DP, 96>), grid, dim3(256), 0, st, p, s.chunks, s.per_chunk);
-        else hipLaunchKernelGGL((k_ctx_short<BF, DP, 128>), grid, dim3(256), 0, st, p, s.chunks, s.per_chunk);
+        hipLaunchKernelGGL((k_ctx_short<BF, DP>), grid, dim3(256), 0, st, p, s.chunks, s.per_chunk);
         return;
     }
     const dim3 grid((unsigned)(s.first.blocks + s.second.blocks));
