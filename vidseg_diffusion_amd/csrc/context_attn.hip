@@ -765,13 +765,15 @@ Plan make_plan(int B, int Nq, int Np, int Nk, int H, int Hk, int d) {
     Plan s{};
     const int G = H / Hk;
     const long long rows = (long long)Nq * G, heads = (long long)B * Hk;
+    const int slots = d <= 64 ? 768 : 512;                            // blocks that the chip holds: three a CU, or two
     if (Np == 0 && Nk <= SHORT && rows >= 64) {
         // (k_ctx_short / k_ctx_attn: 28 x 4096 rows, 5 heads of 64, 33 keys 31 / 44 us, 77 keys 36 to 41 / 58, 96 keys 40 / 55; 14 x 4096, 8 heads, 77 keys of 96
-        // 50 / 68, of 128 70 / 79; 256 x 64 rows, 16 heads of 64 39 / 47.  With room for 128 keys, 120 of them: of 64 51 / 54, of 96 76 / 75, of 128 94 / 82;
+        // 42 / 68, of 128 73 / 79; 256 x 64 rows, 16 heads of 64 39 / 47.  With room for 128 keys, 120 of them: of 64 51 / 54, of 96 76 / 75, of 128 94 / 82;
         // 28 x 1024 rows, 10 heads of 64 28.6 / 27.6)
-        // the keys are staged once a block: one round of the 768 blocks that the chip holds (heads up to 64), or, from half of that in heads alone, rounds of
+        // the keys are staged once a block: one round of the blocks that the chip holds, or, from half of that in heads alone, rounds of
         // blocks small enough for the last one to weigh little; at least two tiles a wave
-        const long long tiles = (rows + 31) / 32, want = heads <= 384 ? 768 / heads : (4 * 768 + heads - 1) / heads;
+        // (14 x 4096 rows x 77 keys, 8 heads of 96: 448 blocks 42 us, 672 in two rounds 51)
+        const long long tiles = (rows + 31) / 32, want = heads <= slots / 2 ? slots / heads : (4 * slots + heads - 1) / heads;
         const long long per = (tiles + want - 1) / want;
         s.one_pass = true;
         s.per_chunk = (int)(per < 8 ? 8 : (per + 3) / 4 * 4);
@@ -791,7 +793,6 @@ Plan make_plan(int B, int Nq, int Np, int Nk, int H, int Hk, int d) {
     // 4 over 16384 23.7 / 48.2, over 512 23.5 / 19.8; 1024 over 64 59.4 / 63.2).  2^26 rows are what the joining launch takes.
     const bool few = rows <= 32, stack = B > 1 && rows < 128 && (long long)B * Np >= 32768 && rows * heads < (1ll << 26);
     const bool stack_few = few && rows * B <= 32;
-    const int slots = d <= 64 ? 768 : 512;
     s.mode = !few ? MANY : (!stack || stack_few) ? FEW : MIXED;
     if (stack) {
         const int kt = stack_few ? 128 : 64;
