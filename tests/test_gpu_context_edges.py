@@ -1,0 +1,39 @@
+"""Edges of the context operators: the causal limit without a prefix, samples and keys that one sample of a shared context lacks, remainders of short contexts,
+maps far from zero (bounds: tests/tools_context_attention.py, tests/test_gpu_norm_act.py)."""
+import os
+import sys
+
+import pytest
+import torch
+
+from vidseg_diffusion_amd import ops
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+from tools_context_attention import Reference, randn  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+@pytest.mark.parametrize("B,Nq,Nk,H,Hk,d,dtype,lens", [
+    (1, 64, 64, 1, 1, 64, F16, None),
+    (2, 77, 77, 2, 2, 64, BF16, (77, 40)),                   # 40 tokens and 77 queries: the first 37 see nothing
+    (3, 70, 96, 4, 2, 64, F16, (96, 70, 0)),
+    (2, 32, 77, 4, 1, 96, F16, (77, 5)),                     # 128 rows of a group of four heads
+    (2, 64, 96, 2, 2, 96, BF16, (90, 64)),
+    (2, 96, 64, 2, 1, 128, F16, (64, 33)),
+    (1, 130, 96, 3, 3, 128, BF16, None),
+    (2, 5, 9, 26, 2, 40, F16, (9, 2)),                       # 65 rows, all of them groups
+    (2, 200, 300, 2, 2, 80, F16, (300, 200)),                # a context over 96 keys
+])
+def test_causal_without_a_prefix(B, Nq, Nk, H, Hk, d, dtype, lens):
+    """The own tokens alone, whatever their number: query i sees keys up to lens - Nq + i."""
+    dev = torch.device("cuda:0")
+    q = randn((B, Nq, H * d), 1, dtype, 1.5).to(dev)
+    k, v = (randn((B, Nk, Hk * d), s, dtype).to(dev) for s in (2, 3))
+    n = None if lens is None else torch.tensor(lens, dtype=torch.int32, device=dev)
+    none = k[0, :0]
+    out, lse = ops.prefix_attention(q, none, none, k, v, H, kv_heads=Hk, k_lens=n, causal=True, return_lse=True)
+    Reference(q, k, v, H, Hk, n, causal=True).check(out, lse)
+    free, f_lse = ops.prefix_attention(q, none, none, k, v, H, kv_heads=Hk, k_lens=n, return_lse=True)
+    Reference(q, k, v, H, Hk, n).check(free, f_lse)
