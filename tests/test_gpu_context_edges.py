@@ -37,3 +37,48 @@ def test_causal_without_a_prefix(B, Nq, Nk, H, Hk, d, dtype, lens):
     Reference(q, k, v, H, Hk, n, causal=True).check(out, lse)
     free, f_lse = ops.prefix_attention(q, none, none, k, v, H, kv_heads=Hk, k_lens=n, return_lse=True)
     Reference(q, k, v, H, Hk, n).check(free, f_lse)
+
+
+def step(q, k, v, heads, dout, **how):
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    out = ops.cross_attention(*leaves, heads, **how)
+    return (out.detach(), *torch.autograd.grad(out, leaves, dout))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("Nq,Nk,d", [(70, 77, 64), (1, 77, 64), (70, 300, 64), (700, 300, 128), (70, 100, 80)])
+def test_samples_without_a_key_beside_a_shared_context(Nq, Nk, d, dtype):
+    """One context for the batch; the samples without a key hold NaN or infinities in their queries and in the gradients of their rows: no gradient of
+    the context and of the other samples changes, theirs are zero."""
+    dev = torch.device("cuda:0")
+    q, dout = randn((4, Nq, 2 * d), 1, dtype).to(dev), randn((4, Nq, 2 * d), 4, dtype).to(dev)
+    k, v = (randn((1, Nk, 2 * d), s, dtype).to(dev) for s in (2, 3))
+    lens = torch.tensor([Nk, 0, 5, 0], dtype=torch.int32, device=dev)
+    mask = torch.arange(Nk, device=dev) < lens.view(4, 1)
+    for how in (dict(k_lens=lens), dict(key_mask=mask)):
+        want = step(q, k, v, 2, dout, **how)
+        Reference(q, k, v, 2, None, lens).check_gradients(dout, *want[1:], True)
+        for bad in (float("nan"), float("inf")):
+            q2, g2 = q.clone(), dout.clone()
+            q2[1], g2[1], q2[3] = bad, bad, bad
+            for a, b in zip(want, step(q2, k, v, 2, g2, **how)):
+                assert torch.equal(a, b)
+        assert not want[1][[1, 3]].any()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("Nq,Nk", [(70, 77), (1, 77), (70, 300), (1, 300)])
+def test_gradients_of_rows_without_a_key(Nq, Nk, dtype):
+    """A padded sample's rows carry NaN or infinities in the output's gradient: its own gradients are zero, the others' unchanged."""
+    dev = torch.device("cuda:0")
+    q, k, v, dout = (randn((3, n, 128), s, dtype).to(dev) for n, s in ((Nq, 1), (Nk, 2), (Nk, 3), (Nq, 4)))
+    lens = torch.tensor([Nk, 0, 5], dtype=torch.int32, device=dev)
+    mask = torch.arange(Nk, device=dev) < lens.view(3, 1)
+    for how in (dict(k_lens=lens), dict(key_mask=mask)):
+        want = step(q, k, v, 2, dout, **how)
+        for bad in (float("nan"), float("inf")):
+            q2, g2 = q.clone(), dout.clone()
+            q2[1], g2[1] = bad, bad
+            for a, b in zip(want, step(q2, k, v, 2, g2, **how)):
+                assert torch.equal(a, b)
+        assert not any(t[1].any() for t in want[1:])

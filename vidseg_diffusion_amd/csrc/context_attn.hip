@@ -887,6 +887,9 @@ template <bool BF, int DP> __global__ void __launch_bounds__(256, DP == 64 ? 3 :
     const long long id = ((long long)b * p.Nq + qi) * p.H + h;
     u32x4 fq[DP / 16], fg[DP / 16];
     float D = 0.f;
+    const long long bhq = ((long long)b * p.H + h) * p.Nq + qi;
+    const float lse = p.lse[bhq];
+    const bool none = lse == -INFINITY;                                         // a row without a key is taken as zeros, whatever it holds: p = 0 would be multiplied by it
     {
         const u16 *qp = p.q + b * p.q_b + qi * p.q_n + h * p.q_h, *gp = p.go + b * p.g_b + qi * p.g_n + h * p.g_h;
 #pragma unroll
@@ -895,15 +898,13 @@ template <bool BF, int DP> __global__ void __launch_bounds__(256, DP == 64 ? 3 :
             fq[s] = *reinterpret_cast<const u32x4*>(qp + a);
             fg[s] = *reinterpret_cast<const u32x4*>(gp + a);
             const u32x4 fo = *reinterpret_cast<const u32x4*>(p.o + id * p.d + a), fl = *reinterpret_cast<const u32x4*>(p.o_lo + id * p.d + a);
-            if (at >= p.d) fq[s] = fg[s] = u32x4{0u, 0u, 0u, 0u};
+            if (at >= p.d || none) fq[s] = fg[s] = u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
             for (int e = 0; e < 4; ++e) D = dot2<BF>(fg[s][e], fl[e], dot2<BF>(fg[s][e], fo[e], D));
         }
     }
     D = half_sum(D);
-    const long long bhq = ((long long)b * p.H + h) * p.Nq + qi;
-    const float lse = p.lse[bhq];
-    const float L = lse == -INFINITY ? INFINITY : lse * LOG2E - (BF ? 0.f : P_LOG2);      // a row without a key: p = 0
+    const float L = none ? INFINITY : lse * LOG2E - (BF ? 0.f : P_LOG2);         // (p = 0)
     if (on && hi == 0) p.delta[bhq] = D;
     float power = BF ? 1.f : 1.152921504606846976e18f;                          // this row's factor of ds
     f32x16 acc[ND];
@@ -1044,13 +1045,23 @@ template <bool BF, int DP, bool FUSED, bool DV, bool DK> __device__ __forceinlin
     fq.init(tid, p.q_n, p.d);
     fg.init(tid, p.g_n, p.d);
     float rL = INFINITY, rD = 0.f;
+    // A sample that has none of the block's keys adds nothing to their gradients; its rows are taken as zeros, for its probabilities of zero would still be
+    // multiplied by what they hold, and a padded sample's rows may hold NaN.
+    // (Not FUSED, one sample's own keys: such a block has no tiles.)
+    const bool ask = (FUSED || shared) && (p.lens || p.mask);
+    int asked = -1;
+    bool there = true;
     auto fetch = [&](int buf) __attribute__((always_inline)) {
-        const int q0 = next.i * RT, n = p.Nq - q0, h = hk * p.G + next.g;
+        if (ask && next.b != asked) {                                            // (the same for all threads of the block)
+            asked = next.b;
+            there = p.mask ? __builtin_amdgcn_readfirstlane(__syncthreads_or(lives(asked))) != 0 : p.lens[asked] > kt * 128;
+        }
+        const int q0 = next.i * RT, n = there ? p.Nq - q0 : 0, h = hk * p.G + next.g;
         const unsigned long long live = n >= RT ? ~0ull : (1ull << n) - 1;
         fq.tile(p.q + next.b * p.q_b + h * p.q_h + q0 * p.q_n, p.q_n, live, sQ + buf * TILE, tid, wave);
         fg.tile(p.go + next.b * p.g_b + h * p.g_h + q0 * p.g_n, p.g_n, live, sG + buf * TILE, tid, wave);
         if (tid < RT) {
-            const long long at = ((long long)next.b * p.H + h) * p.Nq + q0 + min(tid, n - 1);
+            const long long at = ((long long)next.b * p.H + h) * p.Nq + q0 + max(0, min(tid, n - 1));
             const float lse = p.lse[at];
             rL = tid >= n || lse == -INFINITY ? INFINITY : lse * LOG2E - (BF ? 0.f : P_LOG2);
             if (!FUSED) rD = tid < n ? p.delta[at] : 0.f;
