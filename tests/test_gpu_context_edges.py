@@ -82,3 +82,24 @@ def test_gradients_of_rows_without_a_key(Nq, Nk, dtype):
             for a, b in zip(want, step(q2, k, v, 2, g2, **how)):
                 assert torch.equal(a, b)
         assert not any(t[1].any() for t in want[1:])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("Nq,Nk,d", [(70, 77, 64), (1, 77, 64), (70, 128, 128), (70, 300, 64)])
+def test_keys_that_one_sample_of_a_shared_context_lacks(Nq, Nk, d, dtype):
+    """Keys that exist for the first sample only hold NaN or infinities: nothing of that reaches the second sample's result and gradient."""
+    dev = torch.device("cuda:0")
+    q, dout = randn((3, Nq, 2 * d), 1, dtype).to(dev), randn((3, Nq, 2 * d), 4, dtype).to(dev)
+    k, v = (randn((1, Nk, 2 * d), s, dtype).to(dev) for s in (2, 3))
+    lens = torch.tensor([30, Nk, 30], dtype=torch.int32, device=dev)
+    mask = torch.arange(Nk, device=dev) < lens.view(3, 1)
+    for how in (dict(k_lens=lens), dict(key_mask=mask)):
+        want = step(q, k, v, 2, dout, **how)
+        Reference(q, k, v, 2, None, lens).check_gradients(dout, *want[1:], True)
+        for bad in (float("nan"), float("inf")):
+            for which in (0, 1):
+                kv = [k.clone(), v.clone()]
+                kv[which][:, 30:] = bad
+                got = step(q, *kv, 2, dout, **how)
+                for b in (0, 2):
+                    assert torch.equal(got[0][b], want[0][b]) and torch.equal(got[1][b], want[1][b])

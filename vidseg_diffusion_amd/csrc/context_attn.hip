@@ -1085,10 +1085,15 @@ template <bool BF, int DP, bool FUSED, bool DV, bool DK> __device__ __forceinlin
             fk[s] = *reinterpret_cast<const u32x4*>(kp + a);
             if (DK) fv[s] = *reinterpret_cast<const u32x4*>(vp + a);
             if (at >= p.d || !any) fk[s] = fv[s] = u32x4{0u, 0u, 0u, 0u};
-            if (FUSED) *reinterpret_cast<u32x4*>(sK + slot_at<DP>(wave * 32 + l31, s * 2 + hi)) = fk[s];
         }
     }
     bool live = shared ? lives(now.b) : any;
+    // FUSED: K for dq, zero where the rows' sample has no such key (another sample of a shared context may, with anything in it)
+    auto keep_k = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) *reinterpret_cast<u32x4*>(sK + slot_at<DP>(wave * 32 + l31, s * 2 + hi)) = live ? fk[s] : u32x4{0u, 0u, 0u, 0u};
+    };
+    if constexpr (FUSED) keep_k();
     bool whole = (!FUSED && !shared) || __all(live);                             // one sample's own keys, not FUSED: a dead key spoils its own column alone, which is not stored
     f32x16 ak[ND], av[ND];
 #pragma unroll
@@ -1108,7 +1113,10 @@ template <bool BF, int DP, bool FUSED, bool DV, bool DK> __device__ __forceinlin
         if (!whole)
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-                if (!live) s[e] = -INFINITY;
+                if (!live) {
+                    s[e] = -INFINITY;
+                    if (FUSED) z[e] = 0.f;                                        // D sums over the keys: 0 times what lies there may be NaN
+                }
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
             const f32x4 L = *reinterpret_cast<const f32x4*>(&sL[buf][i * 32 + 2 * e + 4 * hi]);
@@ -1237,6 +1245,7 @@ template <bool BF, int DP, bool FUSED, bool DV, bool DK> __device__ __forceinlin
         if (shared && more && now.b != b) {
             live = lives(now.b);
             whole = __all(live);
+            if constexpr (FUSED) keep_k();                                        // (every wave has read the old rows, and reads the new ones two barriers on)
         }
     }
     const float to_k = any ? p.scale / power * (BF ? 1.f : P_BACK) : 0.f, to_v = any ? (BF ? 1.f : P_BACK) : 0.f;
