@@ -103,3 +103,28 @@ def test_keys_that_one_sample_of_a_shared_context_lacks(Nq, Nk, d, dtype):
                 got = step(q, *kv, 2, dout, **how)
                 for b in (0, 2):
                     assert torch.equal(got[0][b], want[0][b]) and torch.equal(got[1][b], want[1][b])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("Nq,Nk,lens", [(100, 77, (77, 3)), (100, 96, (0, 96)), (3, 77, (77, 5)), (100, 300, (300, 1)), (2, 2600, (2600, 0))])
+def test_what_the_rounding_left(Nq, Nk, lens, dtype):
+    """The C entry's out_lo at every length: written everywhere, at most half a step of out, and not zero where several keys were averaged."""
+    from vidseg_diffusion_amd import _lib
+    dev = torch.device("cuda:0")
+    B, H, d = 2, 2, 64
+    q = randn((B, Nq, H, d), 1, dtype, 1.5).to(dev)
+    k, v = (randn((B, Nk, H, d), s, dtype).to(dev) for s in (2, 3))
+    n = torch.tensor(lens, dtype=torch.int32, device=dev)
+    out, left = torch.full_like(q, float("nan")), torch.full_like(q, float("nan"))
+    kib = _lib.lib().vidseg_context_attention_scratch_kib(B, Nq, 0, Nk, H, H, d)
+    scratch = torch.empty(max(kib, 1) * 256, device=dev)
+    own = [a for t in (k, v) for a in (t.data_ptr(), *t.stride()[:3])]
+    _lib.call("vidseg_context_attention_fwd", q.data_ptr(), *q.stride()[:3], *(None, 0, 0) * 2, *own, n.data_ptr(), None, 0, out.data_ptr(), left.data_ptr(), None,
+              1 if dtype == F16 else 2, B, Nq, 0, Nk, H, H, d, d ** -0.5, 0, scratch.data_ptr(), kib, torch.cuda.current_stream().cuda_stream)
+    Reference(q.flatten(2), k.flatten(2), v.flatten(2), H, None, n).check(out.flatten(2))
+    assert torch.isfinite(left).all()
+    half = torch.finfo(dtype).eps / 2
+    # what the rounding left is at most half a step of out (half a subnormal step of fp16 at the least)
+    assert (left.double().abs() <= half * out.double().abs() * (1 + 2 * half) + 2.0 ** -25).all()
+    if max(lens) > 1:
+        assert (left != 0).float().mean() > 0.2 * sum(x > 0 for x in lens) / 2

@@ -761,12 +761,12 @@ long long dealt(long long blocks, long long tiles, long long slots, long long le
     }
     return best < 1 ? 1 : best;
 }
-Plan make_plan(int B, int Nq, int Np, int Nk, int H, int Hk, int d, bool causal) {
+Plan make_plan(int B, int Nq, int Np, int Nk, int H, int Hk, int d, bool short_ok) {
     Plan s{};
     const int G = H / Hk;
     const long long rows = (long long)Nq * G, heads = (long long)B * Hk;
     const int slots = d <= 64 ? 768 : 512;                            // blocks that the chip holds: three a CU, or two
-    if (Np == 0 && Nk <= SHORT && rows >= 64 && !causal) {             // (k_ctx_short has no limit by row)
+    if (Np == 0 && Nk <= SHORT && rows >= 64 && short_ok) {            // (k_ctx_short has no limit by row, and writes no o_lo)
         // (k_ctx_short / k_ctx_attn: 28 x 4096 rows, 5 heads of 64, 33 keys 31 / 44 us, 77 keys 36 to 41 / 58, 96 keys 40 / 55; 14 x 4096, 8 heads, 77 keys of 96
         // 42 / 68, of 128 73 / 79; 256 x 64 rows, 16 heads of 64 39 / 47.  With room for 128 keys, 120 of them: of 64 51 / 54, of 96 76 / 75, of 128 94 / 82;
         // 28 x 1024 rows, 10 heads of 64 28.6 / 27.6)
@@ -1361,8 +1361,8 @@ extern "C" {
 
 int vidseg_context_attention_scratch_kib(int B, int Nq, int Np, int Nk, int H, int Hk, int d) {
     if (check_sizes("context_attention", 1, B, Nq, Np, Nk, H, Hk, d, 1.f)) return -1;
-    // for either plan: where a causal call takes k_ctx_attn and another one k_ctx_short, the two key tiles at most are not dealt out and leave no partial results
-    const Plan s = make_plan(B, Nq, Np, Nk, H, Hk, d, true);
+    // for either plan: a context short enough for k_ctx_short has two key tiles at most, which k_ctx_attn does not deal out, so neither leaves partial results
+    const Plan s = make_plan(B, Nq, Np, Nk, H, Hk, d, false);
     return (int)(((long long)s.parts * B * Nq * H * (d + 2) * 4 + 1023) / 1024);
 }
 
@@ -1378,7 +1378,7 @@ int vidseg_context_attention_fwd(const void* q, long long q_b, long long q_n, lo
                    (Np == 0 || (row_strides_ok(k_prefix, 0, kp_n, kp_h) && row_strides_ok(v_prefix, 0, vp_n, vp_h))),
                "context_attention: operands must be 16-byte aligned with strides that are multiples of 8 elements (rows below 2^24 apart)");
     VS_REQUIRE(!(causal && mask), "context_attention: a causal call takes no key mask");
-    const Plan s = make_plan(B, Nq, Np, Nk, H, Hk, d, causal != 0);
+    const Plan s = make_plan(B, Nq, Np, Nk, H, Hk, d, !causal && !out_lo);
     const long long total = (long long)B * Nq * H;
     const long long need = ((long long)s.parts * total * (d + 2) * 4 + 1023) / 1024;
     VS_REQUIRE(need == 0 || (scratch && scratch_kib >= need), "context_attention: scratch of %lld KiB, needs %lld", scratch_kib, need);
