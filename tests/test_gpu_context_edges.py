@@ -128,3 +128,19 @@ def test_what_the_rounding_left(Nq, Nk, lens, dtype):
     assert (left.double().abs() <= half * out.double().abs() * (1 + 2 * half) + 2.0 ** -25).all()
     if max(lens) > 1:
         assert (left != 0).float().mean() > 0.2 * sum(x > 0 for x in lens) / 2
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF16])
+@pytest.mark.parametrize("B,dims,C,groups", [(2, (8, 8), 1280, 32), (1, (1,), 64, 8), (2, (33, 7), 640, 32), (2, (2000,), 30, 3), (1, (700,), 2560, 32)])
+def test_maps_far_from_zero(B, dims, C, groups, dtype):
+    """Means whose square passes fp32's range, spreads whose square does not."""
+    from test_gpu_norm_act import check_all, data
+    dev = torch.device("cuda:0")
+    for far in (3e19, -1e25):
+        x, gamma, beta, dy = data(B, dims, C, torch.float32, 5, dev)
+        x = (far + x * 2.0 ** 58).to(dtype)                  # bf16: steps of 2^57 at 3e19; at 1e25 (steps of 2^75) mostly one value, some beside it
+        check_all(x, gamma, beta, dy.to(dtype), groups, True)
+    x = torch.full((B, *dims, C), 3e38, device=dev, dtype=dtype)
+    beta = torch.linspace(-1, 1, C, device=dev)
+    y = ops.groupnorm_act(x, torch.ones(C, device=dev), beta, groups=groups, act=ops.ACT_NONE)
+    assert torch.equal(y, beta.to(dtype).expand_as(y))

@@ -73,11 +73,11 @@ struct NormArgs {
     long long dy_b, dy_row;
     long long HW;
     int B, C, G, rows, nchunk, act;
-    float eps;
+    float eps, down;                      // down: exact factor of every M2
     const float *gamma, *beta;
     void* out;                            // y or dx, contiguous [B][HW][C]
     float *mean, *rstd;                   // [B][G]
-    float* part;                          // [B][nchunk][G][2]; forward (mean, M2) of a group over a chunk, backward its sums of gamma * dz and gamma * dz * xh
+    float* part;                          // [B][nchunk][G][2]; forward (mean, M2 * down) of a group over a chunk, backward its sums of gamma * dz and gamma * dz * xh
     float* chan;                          // backward: [B][nchunk][2][C] sums of dz and dz * xh over a chunk
     float *dgamma, *dbeta;
 };
@@ -113,7 +113,9 @@ __device__ __forceinline__ float lanes_sum(float v, int lanes) {
 // A thread takes its rows less the first of them, x - k, and carries mean and M2 along: with d = (x - k) - mean,  mean += d / n,  M2 += d ((x - k) - mean);
 // row lanes, channels and chunks are then merged by theirs:
 //   mean = mean_a + (mean_b - mean_a) n_b / n,   M2 = M2_a + M2_b + (mean_b - mean_a)^2 n_a n_b / n.
-// No difference of large squares anywhere, so a map whose mean is far from zero, or whose first rows lie far from the others, keeps its variance.
+// No difference of large squares anywhere, so a map whose mean is far from zero, or whose first rows lie far from the others, keeps its variance.  M2 is n times the
+// variance, and fp32 would not hold it for maps whose variance it holds: it is carried times 2^-32 (exact; every bit is as without), except where eps is below 2^-60
+// and a small M2's bits that this costs (variances of 2^-94 and less) would count.  Channel means are summed times 2^-13, the most there are, for the same reason.
 // (Sums of x - k and its square would take 3 operations a value for 5, and lose a factor of the rows where the first one is an outlier.)
 template <typename T, int VEC> __global__ void __launch_bounds__(NT) k_gna_stats(NormArgs p) {
     extern __shared__ float lds[];
@@ -123,6 +125,7 @@ template <typename T, int VEC> __global__ void __launch_bounds__(NT) k_gna_stats
     float* ch_m2 = lds + C;               // [C]
     float* s0 = lds + 2 * C;              // [R][width] means of the row lanes
     float* s1 = s0 + R * width;           // ... and M2
+    constexpr float MEANS = 1.220703125e-4f;
     const long long r0 = (long long)chunk * p.rows;
     const int n = (int)(p.HW - r0 < p.rows ? p.HW - r0 : p.rows);
     const T* x = (const T*)p.x + b * p.x_b + r0 * p.x_row;
@@ -150,7 +153,7 @@ template <typename T, int VEC> __global__ void __launch_bounds__(NT) k_gna_stats
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 s0[rl * width + col * VEC + e] = k[e] + a[e];
-                s1[rl * width + col * VEC + e] = q[e];
+                s1[rl * width + col * VEC + e] = q[e] * p.down;
             }
         }
         __syncthreads();
@@ -162,7 +165,7 @@ template <typename T, int VEC> __global__ void __launch_bounds__(NT) k_gna_stats
             const float m = s / (float)n;                           // about lane 0's mean
             for (int j = 0; j < lanes; ++j) {
                 const float d = s0[j * width + c] - k - m;
-                m2 += s1[j * width + c] + (float)((n - j + R - 1) / R) * d * d;
+                m2 += s1[j * width + c] + (float)((n - j + R - 1) / R) * p.down * d * d;
             }
             ch_mean[c0 * VEC + c] = k + m;
             ch_m2[c0 * VEC + c] = m2;
@@ -173,22 +176,24 @@ template <typename T, int VEC> __global__ void __launch_bounds__(NT) k_gna_stats
     for (int g0 = 0; g0 < p.G; g0 += stride) {                      // whole waves take part in the shuffles; lanes past G work on the last group
         const int g = min(g0 + (int)threadIdx.x / lanes, p.G - 1);
         float m = 0.f, m2 = 0.f;
-        for (int c = sub; c < cg; c += lanes) m += ch_mean[g * cg + c];
-        m = lanes_sum(m, lanes) / (float)cg;
+        for (int c = sub; c < cg; c += lanes) m += ch_mean[g * cg + c] * MEANS;
+        m = lanes_sum(m, lanes) / ((float)cg * MEANS);
         for (int c = sub; c < cg; c += lanes) {
             const float d = ch_mean[g * cg + c] - m;
-            m2 += ch_m2[g * cg + c] + (float)n * d * d;
+            m2 += ch_m2[g * cg + c] + (float)n * p.down * d * d;
         }
         m2 = lanes_sum(m2, lanes);
         if (sub == 0) *reinterpret_cast<f32x2*>(p.part + (((long long)b * p.nchunk + chunk) * p.G + g) * 2) = f32x2{m, m2};
     }
 }
 
-// rows n_b of mean m_b and M2 m2_b (over cg channels) into (n, m, m2); either may be empty
-__device__ __forceinline__ void merge(float& n, float& m, float& m2, float n_b, float m_b, float m2_b, float cg) {
+// rows n_b of mean m_b and M2 m2_b (over cg channels, times down) into (n, m, m2); either may be empty (a mean of 0, from which the other's may lie further than a
+// square can hold)
+__device__ __forceinline__ void merge(float& n, float& m, float& m2, float n_b, float m_b, float m2_b, float cg, float down) {
     const float all = n + n_b, share = n > 0.f ? n_b * __builtin_amdgcn_rcpf(all) : 1.f, d = m_b - m;      // (the first part is taken as it is)
+    const float both = n * share, d0 = both > 0.f ? d : 0.f;
     m += d * share;
-    m2 += m2_b + d * d * (n * share) * cg;
+    m2 += m2_b + d0 * down * d0 * both * cg;
     n = all;
 }
 
@@ -207,19 +212,19 @@ template <typename T, int VEC> __global__ void __launch_bounds__(NT) k_gna_apply
         for (int i = sub; i < p.nchunk; i += lanes) {
             const float rows = (float)(i + 1 < p.nchunk ? p.rows : (int)(p.HW - (long long)i * p.rows));
             const f32x2 t = o[(long long)i * p.G];
-            merge(n, m, m2, rows, t[0], t[1], (float)cg);
+            merge(n, m, m2, rows, t[0], t[1], (float)cg, p.down);
         }
         for (int w = 1; w < lanes; w *= 2) {
             const float n_b = __shfl_xor(n, w, 64), m_b = __shfl_xor(m, w, 64), m2_b = __shfl_xor(m2, w, 64);
             // the lower lane's part first: both lanes get the same values
             const bool up = sub & w;
             float n_a = up ? n_b : n, m_a = up ? m_b : m, m2_a = up ? m2_b : m2;
-            merge(n_a, m_a, m2_a, up ? n : n_b, up ? m : m_b, up ? m2 : m2_b, (float)cg);
+            merge(n_a, m_a, m2_a, up ? n : n_b, up ? m : m_b, up ? m2 : m2_b, (float)cg, p.down);
             n = n_a;
             m = m_a;
             m2 = m2_a;
         }
-        const float rstd = 1.0f / sqrtf(m2 / ((float)p.HW * (float)cg) + p.eps);
+        const float rstd = 1.0f / sqrtf(m2 / ((float)p.HW * (float)cg * p.down) + p.eps);
         if (sub == 0) {
             g_mean[g] = m;
             g_rstd[g] = rstd;
@@ -481,6 +486,7 @@ int vidseg_groupnorm_act_fwd(const void* x, long long x_batch_stride, long long 
     NormArgs p{};
     p.x = x; p.x_b = x_batch_stride; p.x_row = x_row_stride; p.HW = HW; p.B = B; p.C = C; p.G = G; p.rows = rows_per_chunk;
     p.nchunk = (int)((HW + rows_per_chunk - 1) / rows_per_chunk);
+    p.down = eps >= 0x1p-60f ? 0x1p-32f : 1.0f;
     p.act = act; p.eps = eps; p.gamma = gamma; p.beta = beta; p.out = y; p.mean = mean; p.rstd = rstd; p.part = scratch;
     VS_REQUIRE((long long)B * p.nchunk * G * 2 <= scratch_floats, "groupnorm_act: scratch of %lld floats, needs %lld", scratch_floats,
                (long long)B * p.nchunk * G * 2);
