@@ -1,0 +1,27 @@
+"""Limits of the context operators that are checked before anything reaches a device (CPU only)."""
+import pytest
+import torch
+
+from vidseg_diffusion_amd import _lib, ops
+from vidseg_diffusion_amd._lib import VidsegError
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(131072, None), (1025, None), (2048, 2)])
+def test_number_of_heads(heads, kv_heads):
+    """More heads than the library takes are refused by their number: rows of 2^24 elements cannot be made any shorter by copying them."""
+    q = torch.zeros(1, 1, heads * 128, dtype=torch.float16)
+    k = q[..., :(kv_heads or heads) * 128]
+    with pytest.raises(VidsegError, match="heads"):
+        ops.cross_attention(q, k, k, heads, kv_heads=kv_heads)
+    with pytest.raises(VidsegError, match="heads"):
+        ops.prefix_attention(q, k[0], k[0], k, k, heads, kv_heads=kv_heads)
+
+
+def test_rows_are_copied_once_at_most():
+    from vidseg_diffusion_amd.context_ops import _heads_of
+    rows = torch.zeros(1, 1, 1 << 24, dtype=torch.float16)                          # already contiguous, and as long as a stride may not be
+    with pytest.raises(VidsegError, match="rows"):
+        _heads_of(rows, 128)
+    far = torch.zeros(1).to(torch.float16).as_strided((2, 1, 64), (0, 1 << 24, 0))
+    t, _, b, n, h = _heads_of(far, 64)
+    assert t.is_contiguous() and (b, n, h) == (64, 64, 64)

@@ -152,12 +152,13 @@ def groupnorm_act(x, gamma, beta, *, groups=32, eps=1e-5, act=1):
 def _heads_of(t, d):
     """[.., N, heads * d] or [.., N, heads, d] as (tensor, pointer, first, row and head stride): a copy only where the last dimension is not contiguous,
     16-byte pieces are not aligned or rows lie 2^24 elements and more apart."""
-    while True:
+    for copied in (False, True):
         st = t.stride()
         n, h = (st[-2], d) if len(st) == 3 else (st[-3], st[-2])
         at = t.data_ptr()
         if st[-1] == 1 and not (st[0] | n | h) & 7 and not at & 15 and n < 1 << 24:
             return t, at, st[0] if t.shape[0] > 1 else 0, n, h
+        _need(not copied, "rows of %d elements cannot be laid out for the kernels", n)
         t = t.clone(memory_format=torch.contiguous_format)
 
 
@@ -170,6 +171,7 @@ def _attention_shapes(name, q, heads, kv_heads, kv):
     _need(heads >= 1 and (shape[2] == heads if four else shape[2] % heads == 0), "%s: q of shape %s does not hold %d heads", name, tuple(shape), heads)
     d = shape[3] if four else shape[2] // heads
     kv_heads = heads if kv_heads is None else kv_heads
+    _need(heads <= 1024, "%s: %d heads, at most 1024", name, heads)
     _need(kv_heads >= 1 and heads % kv_heads == 0, "%s: %d heads on %d key heads", name, heads, kv_heads)
     _need(8 <= d <= 128 and d % 8 == 0, "%s: head width %d: a multiple of 8 up to 128", name, d)
     for n, t, lead in kv:
