@@ -25,3 +25,26 @@ def test_rows_are_copied_once_at_most():
     far = torch.zeros(1).to(torch.float16).as_strided((2, 1, 64), (0, 1 << 24, 0))
     t, _, b, n, h = _heads_of(far, 64)
     assert t.is_contiguous() and (b, n, h) == (64, 64, 64)
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor asks for no gradient, but a result without a tangent would read as a derivative of zero."""
+    import torch.autograd.forward_ad as fwd
+    x, g, b = torch.zeros(2, 4, 64), torch.ones(64), torch.zeros(64)
+    q = torch.zeros(2, 3, 128, dtype=torch.float16)
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))                       # noqa: E731
+        for a in ((dual(x), g, b), (x, dual(g), b), (x, g, dual(b))):
+            with pytest.raises(VidsegError, match="forward-mode"):
+                ops.groupnorm_act(*a, groups=8)
+        for i in range(3):
+            a = [dual(q) if j == i else q for j in range(3)]
+            with pytest.raises(VidsegError, match="forward-mode"):
+                ops.cross_attention(*a, 2)
+        for i in range(5):
+            a = [q, q[0], q[0], q, q]
+            a[i] = dual(a[i])
+            with pytest.raises(VidsegError, match="forward-mode"):
+                ops.prefix_attention(*a, 2)
+        with pytest.raises(VidsegError, match="HIP device"):                        # a level without dual operands changes nothing
+            ops.cross_attention(q, q, q, 2)

@@ -15,6 +15,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -50,6 +51,12 @@ def _launch(device, name, *args):
 def _need(cond, message, *args):
     if not cond:
         raise VidsegError(message % args if args else message)
+
+
+def _no_tangents(name, *tensors):
+    """Refuses dual tensors: they ask for no gradient, and a result without a tangent would read as a derivative of zero."""
+    if forward_ad._current_level >= 0:
+        _need(all(forward_ad.unpack_dual(t).tangent is None for t in tensors), "%s: carries no forward-mode derivatives", name)
 
 
 # ----------------------------------------------------------------------------- GroupNorm + activation
@@ -129,8 +136,8 @@ class _GroupNormAct(torch.autograd.Function):
 def groupnorm_act(x, gamma, beta, *, groups=32, eps=1e-5, act=1):
     """act((x - mean_g) / sqrt(var_g + eps) * gamma + beta) over a channels-last map x [B, ..., C] (fp32 / fp16 / bf16; statistics and
     arithmetic in fp32, one rounding), group g = channels [g C / groups, (g + 1) C / groups) of one sample.  act: ops.ACT_SILU or
-    ops.ACT_NONE.  gamma, beta: fp32 [C].  x may be a column slice of a wider map.  Differentiable in x, gamma and beta (once)
-    (diffusionmodules/util.py:276-278 GroupNorm32, openaimodel.py:267-271)."""
+    ops.ACT_NONE.  gamma, beta: fp32 [C].  x may be a column slice of a wider map.  Differentiable in x, gamma and beta (once, in
+    reverse mode) (diffusionmodules/util.py:276-278 GroupNorm32, openaimodel.py:267-271)."""
     shape = x.shape
     _need(len(shape) >= 2, "groupnorm_act: x must be [B, ..., C]")
     C = shape[-1]
@@ -142,6 +149,7 @@ def groupnorm_act(x, gamma, beta, *, groups=32, eps=1e-5, act=1):
     for n, t in (("gamma", gamma), ("beta", beta)):
         _need(t.dtype == F32 and t.shape == (C,) and t.stride(0) == 1 and t.device == x.device,
               "groupnorm_act: %s must be a contiguous fp32 [%d] tensor on x's device", n, C)
+    _no_tangents("groupnorm_act", x, gamma, beta)
     _need(x.is_cuda, "groupnorm_act: x must be a HIP device tensor (no CPU path)")
     if torch.is_grad_enabled() and (x.requires_grad or gamma.requires_grad or beta.requires_grad):
         return _GroupNormAct.apply(x, gamma, beta, groups, float(eps), act)
@@ -265,8 +273,8 @@ def cross_attention(q, k, v, heads, *, kv_heads=None, k_lens=None, key_mask=None
     be a dimension of their own, in any order of strides; d a multiple of 8 up to 128; fp16 / bf16, fp32 inside; scale defaults to d^-1/2).
     Query head h reads key head h * kv_heads // heads.  One sample of k / v serves the whole batch.  A key exists if it lies below k_lens[b] (int32 [B] on the device)
     and key_mask[b or 0, key] (bool) is true; what k / v hold elsewhere, NaN included, reaches nothing, and a query without any key gets zeros.
-    return_lse: also log(sum exp) of the scores, fp32 [B, heads, Nq] (-inf without a key).  Differentiable (once) in q, k and v, not through the
-    log-sum-exp.  Gradients of one shared k / v are summed over the batch  (attention.py:286-364)."""
+    return_lse: also log(sum exp) of the scores, fp32 [B, heads, Nq] (-inf without a key).  Differentiable (once, in reverse mode) in q, k and v,
+    not through the log-sum-exp.  Gradients of one shared k / v are summed over the batch  (attention.py:286-364)."""
     name = "cross_attention"
     d, kv_heads = _attention_shapes(name, q, heads, kv_heads, (("k", k, 1), ("v", v, 1)))
     B, sk = q.shape[0], k.shape
@@ -279,6 +287,7 @@ def cross_attention(q, k, v, heads, *, kv_heads=None, k_lens=None, key_mask=None
               and (key_mask.stride(1) == 1 or sk[1] == 1), "%s: key_mask must be a bool [%d or 1, %d] tensor with contiguous rows on q's device", name, B, sk[1])
     scale = d ** -0.5 if scale is None else float(scale)
     _need(0 < scale < float("inf"), "%s: scale must be positive and finite", name)
+    _no_tangents(name, q, k, v)
     _need(q.is_cuda, "%s: q must be a HIP device tensor (no CPU path)", name)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, lse = _CrossAttention.apply(q, k, v, heads, kv_heads, d, k_lens, key_mask, scale)
@@ -306,6 +315,7 @@ def prefix_attention(q, k_prefix, v_prefix, k, v, heads, *, kv_heads=None, k_len
     _need(0 < scale < float("inf"), "%s: scale must be positive and finite", name)
     _need(not (torch.is_grad_enabled() and any(t.requires_grad for t in (q, k_prefix, v_prefix, k, v))),
           "%s: carries no gradients (use it under torch.no_grad())", name)
+    _no_tangents(name, q, k_prefix, v_prefix, k, v)
     _need(q.is_cuda, "%s: q must be a HIP device tensor (no CPU path)", name)
     out, lse = _context_attention(q, k_prefix, v_prefix, k, v, heads, kv_heads, d, k_lens, None, scale, int(causal), return_lse)
     return (out, lse) if return_lse else out
