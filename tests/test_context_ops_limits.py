@@ -48,3 +48,15 @@ def test_forward_mode_derivatives_are_refused():
                 ops.prefix_attention(*a, 2)
         with pytest.raises(VidsegError, match="HIP device"):                        # a level without dual operands changes nothing
             ops.cross_attention(q, q, q, 2)
+
+
+@pytest.mark.parametrize("scale", [2.5e38, 3.0e38, 1e39, 1e-50])
+def test_scales_that_fp32_cannot_hold(scale):
+    """scale * log2 e is what the kernels multiply by: it has to be finite (0 * inf would be NaN), and the scale itself not zero in fp32."""
+    p = 4096                                                                        # a pointer that is never followed
+    for name, args in (("vidseg_context_attention_fwd", (p, 192, 64, 64, None, 0, 0, None, 0, 0, p, 320, 64, 64, p, 320, 64, 64, None, None, 0, p, None, None, 1, 1, 3, 0, 5,
+                                                         1, 1, 64, scale, 0, None, 0, None)),
+                       ("vidseg_context_attention_bwd", (*(p, 192, 64, 64) * 2, *(p, 320, 64, 64) * 2, None, None, 0, None, None, p, p, p, p, 1, 1, 1, 3, 5, 1, 1, 64, scale,
+                                                         None, 0, None))):
+        assert getattr(_lib.lib(), name)(*args) == -1, name
+        assert b"scale" in _lib.lib().vidseg_last_error()
