@@ -60,3 +60,12 @@ def test_scales_that_fp32_cannot_hold(scale):
                                                          None, 0, None))):
         assert getattr(_lib.lib(), name)(*args) == -1, name
         assert b"scale" in _lib.lib().vidseg_last_error()
+
+
+def test_row_numbers_stay_within_32_bits():
+    """Row numbers are 32-bit, and the last tile of 128 runs past the last row: 2^31 - 8 rows (34 GB of queries, 8 wide) are refused."""
+    for B, Nq, H in ((1, (1 << 28) - 1, 8), (1, (1 << 28) - 16, 8), (7, 1 << 28, 2)):
+        assert _lib.lib().vidseg_context_attention_scratch_kib(B, Nq, 0, 5, H, 1, 8) == -1
+        assert b"too many rows" in _lib.lib().vidseg_last_error()
+    assert _lib.lib().vidseg_context_attention_scratch_kib(1, (1 << 28) - 64, 0, 5, 8, 1, 8) >= 0
+    assert _lib.lib().vidseg_context_attention_bwd_scratch_kib(1, 1, (1 << 28) - 1, 5, 8, 1, 8) == -1

@@ -1349,8 +1349,8 @@ int check_sizes(const char* name, int dtype, int B, int Nq, int Np, int Nk, int 
     VS_REQUIRE(Hk >= 1 && H >= Hk && H % Hk == 0 && H <= 1024, "%s: %d heads on %d key heads", name, H, Hk);
     VS_REQUIRE(d >= 8 && d <= 128 && d % 8 == 0, "%s: head width %d (a multiple of 8, at most 128)", name, d);
     VS_REQUIRE(scale > 0.f && scale <= 2.0e38f, "%s: scale must be positive and finite, also times log2 e", name);
-    // 2^24 blocks of 256 threads are one launch's limit; splits only multiply small grids
-    VS_REQUIRE((long long)Nq * (H / Hk) * B < (1ll << 31) && (long long)B * Hk * (((long long)Nq * (H / Hk) + 127) / 128) < (1ll << 24), "%s: B=%d Nq=%d H=%d are too many rows",
+    // 2^24 blocks of 256 threads are one launch's limit; splits only multiply small grids.  Row numbers are 32-bit, and a last tile's run up to 127 past the last row
+    VS_REQUIRE((long long)Nq * (H / Hk) * B <= (1ll << 31) - 256 && (long long)B * Hk * (((long long)Nq * (H / Hk) + 127) / 128) < (1ll << 24), "%s: B=%d Nq=%d H=%d are too many rows",
                name, B, Nq, H);
     return VS_OK;
 }
