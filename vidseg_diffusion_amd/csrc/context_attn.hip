@@ -992,14 +992,15 @@ __device__ __forceinline__ float rows_sum(const f32x16& x, int lane) {
 // group, and the samples where they share one context, one after the other.  FUSED (at most 128 keys): the block holds every key of its rows, so D is summed
 // here from the unrounded p dp (four partial sums a row through LDS) and dq comes out of the same pass -- ds goes through LDS once more, each wave takes
 // its share of the [64][d] tile of ds k -- and q and do are all that is read per row.
-// DV, DK: which of the two the block accumulates.
+// DV, DK: which of the two the block accumulates.  SHARED: whether not FUSED blocks walk over the samples of one context; a variant of its own, for what that
+// asks at each sample makes the compiler lay out the other's loop worse (4 x 10 heads x 1456 x 2311 of 64, fp16, nothing shared: 125 us as one variant, 105 as two).
 // FUSED 28 x 4096 rows x 77 keys, 5 heads of 64, forward and gradients: 179 us bf16, as three passes 218; 14 x 4096, 8 heads of 128: 265 and 354.
 // Not FUSED, 4 x 10 heads x 1456 x 2311 of 64 (fp16): 111 us, 620 TFLOP/s; 2 x 16 heads on 4 x 4096 x 4096 of 128 (bf16): 849 us, 650.
 template <int DP, bool FUSED> struct BwdLds {
     __attribute__((aligned(16))) u16 q[2 * 64 * DP], g[2 * 64 * DP], k[FUSED ? 128 * DP : 8], s[FUSED ? 128 * 64 : 8];
     __attribute__((aligned(16))) float l[2][64], d[FUSED ? 4 : 2][64], m[4];
 };
-template <bool BF, int DP, bool FUSED, bool DV, bool DK> __device__ __forceinline__ void keys_walk(const BwdArgs& p, int y, int kt, BwdLds<DP, FUSED>& lds) {
+template <bool BF, int DP, bool FUSED, bool DV, bool DK, bool SHARED> __device__ __forceinline__ void keys_walk(const BwdArgs& p, int y, int kt, BwdLds<DP, FUSED>& lds) {
     constexpr int RT = 64, ND = DP / 32, TILE = RT * DP;
     u16 *sQ = lds.q, *sG = lds.g, *sK = lds.k, *sS = lds.s;
     float(*sL)[64] = lds.l;
@@ -1009,14 +1010,15 @@ template <bool BF, int DP, bool FUSED, bool DV, bool DK> __device__ __forceinlin
     const int chunk = y % p.chunks;
     y /= p.chunks;
     const int hk = y % p.Hk, bk = y / p.Hk;                                      // bk: sample of k and v
-    const bool shared = p.Bk < p.B;
+    const bool shared = FUSED ? p.Bk < p.B : SHARED;
     const int tiles = (p.Nq + RT - 1) / RT;                                      // of one head
     const long long all = (long long)tiles * p.G * (shared ? p.B : 1), t0 = (long long)chunk * p.per_chunk;
     int count = (int)((t0 + p.per_chunk < all ? t0 + p.per_chunk : all) - t0);
     const int key = kt * 128 + wave * 32 + l31;
     const bool in = key < p.Nk;
     // a key that no sample of this block has is taken as zero, so nothing that lies there reaches a product
-    auto lives = [&](int b) __attribute__((always_inline)) { return in && (!p.lens || key < p.lens[b]) && (!p.mask || p.mask[b * p.mask_b + key]); };
+    auto exists = [&](int k, int b) __attribute__((always_inline)) { return k < p.Nk && (!p.lens || k < p.lens[b]) && (!p.mask || p.mask[b * p.mask_b + k]); };
+    auto lives = [&](int b) __attribute__((always_inline)) { return exists(key, b); };
     bool any = false;
     if (shared) {
         for (int i = 0; i < p.B; ++i) any |= lives(i);
@@ -1046,22 +1048,20 @@ template <bool BF, int DP, bool FUSED, bool DV, bool DK> __device__ __forceinlin
     fg.init(tid, p.g_n, p.d);
     float rL = INFINITY, rD = 0.f;
     // A sample that has none of the block's keys adds nothing to their gradients; its rows are taken as zeros, for its probabilities of zero would still be
-    // multiplied by what they hold, and a padded sample's rows may hold NaN.
-    // (Not FUSED, one sample's own keys: such a block has no tiles.)
-    const bool ask = (FUSED || shared) && (p.lens || p.mask);
-    int asked = -1;
-    bool there = true;
+    // multiplied by what they hold, and a padded sample's rows may hold NaN.  (Not FUSED, one sample's own keys: such a block has no tiles.)
+    int asked = -1, have = p.Nq;                                                 // the sample of the next fetch, its rows that are fetched
+    auto ask = [&](int b) __attribute__((always_inline)) {                       // (every wave looks at the block's 128 keys)
+        if (b == asked || b >= p.B) return;
+        asked = b;
+        if (p.lens || p.mask) have = __builtin_amdgcn_readfirstlane(__any(exists(kt * 128 + lane, asked) || exists(kt * 128 + 64 + lane, asked)) ? p.Nq : 0);
+    };
     auto fetch = [&](int buf) __attribute__((always_inline)) {
-        if (ask && next.b != asked) {                                            // (the same for all threads of the block)
-            asked = next.b;
-            there = p.mask ? __builtin_amdgcn_readfirstlane(__syncthreads_or(lives(asked))) != 0 : p.lens[asked] > kt * 128;
-        }
-        const int q0 = next.i * RT, n = there ? p.Nq - q0 : 0, h = hk * p.G + next.g;
+        const int q0 = next.i * RT, n = max(0, have - q0), h = hk * p.G + next.g;
         const unsigned long long live = n >= RT ? ~0ull : (1ull << n) - 1;
         fq.tile(p.q + next.b * p.q_b + h * p.q_h + q0 * p.q_n, p.q_n, live, sQ + buf * TILE, tid, wave);
         fg.tile(p.go + next.b * p.g_b + h * p.g_h + q0 * p.g_n, p.g_n, live, sG + buf * TILE, tid, wave);
         if (tid < RT) {
-            const long long at = ((long long)next.b * p.H + h) * p.Nq + q0 + max(0, min(tid, n - 1));
+            const long long at = ((long long)next.b * p.H + h) * p.Nq + min(q0 + tid, p.Nq - 1);
             const float lse = p.lse[at];
             rL = tid >= n || lse == -INFINITY ? INFINITY : lse * LOG2E - (BF ? 0.f : P_LOG2);
             if (!FUSED) rD = tid < n ? p.delta[at] : 0.f;
@@ -1086,6 +1086,15 @@ template <bool BF, int DP, bool FUSED, bool DV, bool DK> __device__ __forceinlin
             if (DK) fv[s] = *reinterpret_cast<const u32x4*>(vp + a);
             if (at >= p.d || !any) fk[s] = fv[s] = u32x4{0u, 0u, 0u, 0u};
         }
+    }
+    if (FUSED || shared) {                                                       // the first tile is on its way already: fetched anew in the rare case
+        ask(now.b);
+        if (!have && count > 0) {
+            landed();
+            next = now;
+            fetch(0);
+        }
+        if (shared) ask(next.b);
     }
     bool live = shared ? lives(now.b) : any;
     // FUSED: K for dq, zero where the rows' sample has no such key (another sample of a shared context may, with anything in it)
@@ -1242,10 +1251,13 @@ template <bool BF, int DP, bool FUSED, bool DV, bool DK> __device__ __forceinlin
         }
         const int b = now.b;
         step(now);
-        if (shared && more && now.b != b) {
-            live = lives(now.b);
-            whole = __all(live);
-            if constexpr (FUSED) keep_k();                                        // (every wave has read the old rows, and reads the new ones two barriers on)
+        if (shared && more) {
+            ask(next.b);
+            if (now.b != b) {
+                live = lives(now.b);
+                whole = __all(live);
+                if constexpr (FUSED) keep_k();                                    // (every wave has read the old rows, and reads the new ones two barriers on)
+            }
         }
     }
     const float to_k = any ? p.scale / power * (BF ? 1.f : P_BACK) : 0.f, to_v = any ? (BF ? 1.f : P_BACK) : 0.f;
@@ -1274,15 +1286,15 @@ template <bool BF, int DP, bool FUSED, bool DV, bool DK> __device__ __forceinlin
 // Wide heads, not FUSED: the accumulators of both gradients and K, V leave room for one wave a SIMD only, which waits more than it works; so half of the
 // blocks take dk and the other half dv (five products for four, at two waves a SIMD).  Forward and gradients, separate / together: 4 x 10 heads x 1456 x 2311
 // of 96 bf16 356 / 376 us, of 128 fp16 460 / 479, bf16 432 / 422; 2 x 16 heads on 4 x 4096 x 4096 of 128 fp16 1589 / 1675, bf16 1470 / 1450.
-template <bool BF, int DP, bool FUSED> __global__ void __launch_bounds__(256, DP == 64 || !FUSED ? 2 : 1) k_ctx_bwd_kv(BwdArgs p) {
+template <bool BF, int DP, bool FUSED, bool SHARED = false> __global__ void __launch_bounds__(256, DP == 64 || !FUSED ? 2 : 1) k_ctx_bwd_kv(BwdArgs p) {
     __shared__ BwdLds<DP, FUSED> lds;
     int y, kt;
     block_of(p.xtiles, y, kt);
     if constexpr (FUSED || DP == 64) {
-        keys_walk<BF, DP, FUSED, true, true>(p, y, kt, lds);
+        keys_walk<BF, DP, FUSED, true, true, SHARED>(p, y, kt, lds);
     } else {
-        if (kt & 1) keys_walk<BF, DP, FUSED, true, false>(p, y, kt >> 1, lds);
-        else keys_walk<BF, DP, FUSED, false, true>(p, y, kt >> 1, lds);
+        if (kt & 1) keys_walk<BF, DP, FUSED, true, false, SHARED>(p, y, kt >> 1, lds);
+        else keys_walk<BF, DP, FUSED, false, true, SHARED>(p, y, kt >> 1, lds);
     }
 }
 
@@ -1330,7 +1342,8 @@ template <bool BF, int DP> void launch_bwd(BwdArgs p, const BwdPlan& s, bool wan
         if (!want_kv) return;
         constexpr int shares = DP == 64 ? 1 : 2;
         p.xtiles = s.ktiles * shares;
-        hipLaunchKernelGGL((k_ctx_bwd_kv<BF, DP, false>), dim3(kv_blocks * shares), dim3(256), 0, st, p);
+        if (p.Bk < p.B) hipLaunchKernelGGL((k_ctx_bwd_kv<BF, DP, false, true>), dim3(kv_blocks * shares), dim3(256), 0, st, p);
+        else hipLaunchKernelGGL((k_ctx_bwd_kv<BF, DP, false, false>), dim3(kv_blocks * shares), dim3(256), 0, st, p);
     }
     if (s.chunks > 1) {
         const long long plane = (long long)p.Bk * p.Nk * p.Hk * p.d;
