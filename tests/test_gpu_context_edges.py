@@ -144,3 +144,13 @@ def test_maps_far_from_zero(B, dims, C, groups, dtype):
     beta = torch.linspace(-1, 1, C, device=dev)
     y = ops.groupnorm_act(x, torch.ones(C, device=dev), beta, groups=groups, act=ops.ACT_NONE)
     assert torch.equal(y, beta.to(dtype).expand_as(y))
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-20, 1e-17])
+def test_small_spreads_without_an_eps(eps):
+    """Deviations of 2^-60, whose squares are the variance where eps is zero and nothing beside it where eps is not; ordinary maps on both sides of 2^-60."""
+    from test_gpu_norm_act import check_all, data
+    dev = torch.device("cuda:0")
+    x, gamma, beta, dy = data(2, (33, 7), 640, torch.float32, 5, dev)
+    check_all(x, gamma, beta, dy, 32, True, eps)
+    check_all(x * 2.0 ** -60, gamma, beta, dy, 32, False, eps)
