@@ -399,6 +399,7 @@ int vidseg_groupnorm_act_bwd(const void* dy, long long dy_batch_stride, long lon
  * mask[b * mask_b + key] != 0 (mask NULL: all); causal: query i sees own keys up to lens[b] - Nq + i (no mask then).  Heads of width d (8..128, d % 8
  * == 0), query head h on key head h * Hk / H; element strides per sample, row and head (multiples of 8, rows below 2^24; 0 shares one sample), 16-byte aligned.
  * out [B][Nq][H][d]; out_lo (opt): what the rounding of out left, same type; lse (opt) fp32 [B][H][Nq].  A query without a key: out 0, lse -inf.  Keys that do not exist are not read for their value.
+ * At most 1024 heads, and B * Nq * H / Hk rows within 256 of 2^31; scale * log2 e within fp32.
  * scratch: vidseg_context_attention_scratch_kib(...) KiB (0: none; -1: sizes refused). */
 int vidseg_context_attention_scratch_kib(int B, int Nq, int Np, int Nk, int H, int Hk, int d);
 int vidseg_context_attention_fwd(const void* q, long long q_b, long long q_n, long long q_h, const void* k_prefix, long long kp_n, long long kp_h,
@@ -408,7 +409,7 @@ int vidseg_context_attention_fwd(const void* q, long long q_b, long long q_n, lo
                                  void* scratch, long long scratch_kib, vidseg_stream_t stream);
 /* its gradients (no prefix, not causal): lse and, over 128 keys, out and out_lo as the forward call wrote them (NULL otherwise); dq [B][Nq][H][d], dk / dv [Bk][Nk][Hk][d] contiguous.  Bk = 1 < B: one sample of
  * k / v serves all (k_b = v_b = 0) and its gradients are summed over the batch.  dk = dv = NULL: dq alone (more than 128 keys only).  Sums in a fixed order, no atomics.
- * fp16: exact powers of two keep the intermediate gradients in range.
+ * fp16: exact powers of two keep the intermediate gradients in range.  Rows without a key (lse -inf) take and give no gradient, whatever q and dout hold there.
  * scratch: vidseg_context_attention_bwd_scratch_kib(...) KiB (-1: sizes refused). */
 int vidseg_context_attention_bwd_scratch_kib(int B, int Bk, int Nq, int Nk, int H, int Hk, int d);
 int vidseg_context_attention_bwd(const void* dout, long long g_b, long long g_n, long long g_h, const void* q, long long q_b, long long q_n, long long q_h,

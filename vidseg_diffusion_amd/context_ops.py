@@ -270,7 +270,9 @@ class _CrossAttention(torch.autograd.Function):
 
 def cross_attention(q, k, v, heads, *, kv_heads=None, k_lens=None, key_mask=None, scale=None, return_lse=False):
     """softmax(scale q k^T over the keys that exist) v, heads side by side: q [B, Nq, heads * d], k / v [B or 1, Nk, kv_heads * d] (the heads may also
-    be a dimension of their own, in any order of strides; d a multiple of 8 up to 128; fp16 / bf16, fp32 inside; scale defaults to d^-1/2).
+    be a dimension of their own, in any order of strides; d a multiple of 8 up to 128, at most 1024 heads; fp16 / bf16; scale defaults to d^-1/2).
+    Scores, maxima, sums and accumulators are fp32; probabilities and, in the gradients, dp - D times them are rounded once to the tensors' type before the
+    product that takes them, so a result is off by up to about two half steps of that type where attention in fp32 would be off by one.
     Query head h reads key head h * kv_heads // heads.  One sample of k / v serves the whole batch.  A key exists if it lies below k_lens[b] (int32 [B] on the device)
     and key_mask[b or 0, key] (bool) is true; what k / v hold elsewhere, NaN included, reaches nothing, and a query without any key gets zeros.
     return_lse: also log(sum exp) of the scores, fp32 [B, heads, Nq] (-inf without a key).  Differentiable (once, in reverse mode) in q, k and v,
@@ -301,7 +303,8 @@ def prefix_attention(q, k_prefix, v_prefix, k, v, heads, *, kv_heads=None, k_len
     k_prefix / v_prefix [Np, kv_heads * d], k / v [B, Nk, kv_heads * d] with k_lens[b] keys in use (all without k_lens); layouts and types as in
     cross_attention, Np and Nk may be 0.  The prefix is read once for all samples where they bring few queries each (single tokens behind one
     prompt), and through each XCD's cache where they bring many (frames over an anchor frame's keys).
-    causal: the queries are the last Nq of the k_lens[b] own tokens, and query i sees own keys up to its own position k_lens[b] - Nq + i.
+    causal: the queries are the last Nq of the k_lens[b] own tokens, and query i sees own keys up to its own position k_lens[b] - Nq + i.  Later keys
+    of the k_lens[b] have probability zero for it, but their values have to be finite: zero times NaN or infinity is NaN.
     No gradients: the call is refused where one is asked for."""
     name = "prefix_attention"
     d, kv_heads = _attention_shapes(name, q, heads, kv_heads, (("k", k, 1), ("v", v, 1), ("k_prefix", k_prefix, 0), ("v_prefix", v_prefix, 0)))

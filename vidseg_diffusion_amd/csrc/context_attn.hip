@@ -10,9 +10,11 @@
 // uses the same: V^T is fetched with the transpose read in that order).  Keys that do not exist are zeroed while they are staged (a NaN
 // there reaches nothing) and their scores are -inf.
 //
-// What bounds the products: a wave's 32 columns use every A operand that LDS gives (1 KB, 8 clocks of its 128 B) for one MFMA of 32 clocks, on four SIMDs at
-// once: LDS and the matrix pipes are full together.  64 columns a wave would halve the reads, but its accumulators leave one wave a SIMD, which
-// waits more than it saves (measured slower at every size).  Rates below are of the products that the formulas need.
+// What bounds the products: no pipe alone.  On full grids the matrix pipes are busy 37 to 56 % of a SIMD's clocks and vector instructions (the softmax, roundings,
+// addresses) are issued in 28 to 59 %, LDS has no bank conflicts (counters, all keys in use: k_ctx_attn 14 x 5 x 4096 x 8192 of 64 41 and 59 %, 2 x 16 x 4096 x 4096 of 128
+// 43 and 37, k_ctx_bwd_q 56 and 38, k_ctx_bwd_kv 37 and 28): two or three waves a SIMD do not cover each other's waits for LDS and between the products.
+// A wave's 32 columns use every A operand that LDS gives (1 KB, 8 clocks of its 128 B) for one MFMA of 32 clocks; 64 columns would halve the reads, but their
+// accumulators leave one wave a SIMD (a version of many_rows, slower).  Rates below are of the products that the formulas need, with all keys in use.
 #include "common.h"
 
 namespace {
@@ -163,8 +165,8 @@ __device__ __forceinline__ Row row_of(const AttnArgs& p, int b, int hk, bool sta
     return x;
 }
 
-// Blocks reach the 8 XCDs round-robin by their index: every XCD gets one contiguous run of the (key head, split, row tile) space, so the row
-// tiles that read the same keys share them through one L2.
+// Blocks reach the 8 XCDs round-robin by their index: every XCD gets one contiguous run of the (sample, key head, split, row tile) space, so the row
+// tiles that read the same keys share them through one L2.  Samples are outermost: of a few samples of unequal length the short ones' XCDs are done first.
 __device__ __forceinline__ unsigned swizzled(unsigned i, unsigned tot) {
     const unsigned q = tot / 8, r = tot % 8, xcd = i % 8;
     return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + i / 8;
@@ -278,8 +280,9 @@ __device__ __forceinline__ void hide(f32x16& s, unsigned bits, int lim, int hi) 
 }
 
 // Many rows: the block's four waves own 32 rows each and share key tiles of 64 in LDS, fetched one tile ahead.  14 x 5 heads x 4096 rows x 8192 keys of 64
-// (fp16) 650 us, 925 TFLOP/s; 2 x 16 heads x 4096 x 4096 of 128 (bf16) 294 us, 935 TFLOP/s; a large library product reaches 1250 on the same card.
-// Single tokens of 64 samples over a prefix of 16384, 32 heads of 128 on 8: 41 us alone, 420 TFLOP/s -- 8 tiles a block, too few to hide a block's
+// (fp16) 725 to 780 us one after the other, 775 to 830 TFLOP/s at the clock that the power limit leaves; 2 x 16 heads x 4096 x 4096 of 128 (bf16) 299 us, 920 TFLOP/s;
+// a large library product reaches 1250 on the same card.  8 samples' prompts of 512 behind 4096 shared keys, causal, 32 heads of 128 on 8 (bf16): 359 us, 815.
+// Single tokens of 64 samples over a prefix of 16384, 32 heads of 128 on 8: 38 us alone, 455 TFLOP/s -- 8 tiles a block, too few to hide a block's
 // start and its partial results (68 MB in all).
 template <bool BF, int DP> __device__ __forceinline__ void many_rows(const AttnArgs& p, const Deal& w, unsigned block, u16* lds) {
     constexpr int KT = 64, ND = DP / 32, TILE = KT * DP, BR = 128;
@@ -380,8 +383,8 @@ template <bool BF, int DP> __device__ __forceinline__ void many_rows(const AttnA
 }
 
 // Few rows (at most 32 per key head): the keys are what has to be read, so every wave walks over its own runs of 32 of them with all rows as
-// columns, no barrier in the loop.  64 samples of one query over 2000 keys, 16 heads of 64 (fp16): 111 us, 4.7 TB/s; 32 over 5000, 8 heads of 128: 125 us,
-// 5.2 TB/s, the rate of a large copy (K read row by row into the operands, past LDS: 128 and 136 us, every line fetched four times).  K and V pass through a piece of LDS that only this wave uses (read whole rows at a time).
+// columns, no barrier in the loop.  64 samples of one query over 2000 keys, 16 heads of 64 (fp16): 111 us, 4.7 TB/s; 32 over 5000, 8 heads of 128: 124 us,
+// 5.3 TB/s, the rate of a large copy (K read row by row into the operands, past LDS: 128 and 136 us, every line fetched four times).  K and V pass through a piece of LDS that only this wave uses (read whole rows at a time).
 // The next 32 keys are in flight while these are worked on; the four waves' results are merged at the end.
 template <bool BF, int DP> __device__ __forceinline__ void few_rows(const AttnArgs& p, const Deal& w, unsigned block, u16* lds) {
     constexpr int SL = DP / 8, NV = 32 * SL / 64, ND = DP / 32;
@@ -746,7 +749,10 @@ struct Plan {
 };
 // `tiles` tiles of work in each of `blocks` places: how many of them a block takes.  Where the places alone leave part of the chip idle the tiles are dealt
 // out in runs: as many as make the rounds that `slots` resident blocks take shortest (a block's start and its partial results count as two tiles), at least `least` tiles each
-// (2 x 1000 rows x 4000 keys, 10 heads of 128: 3 runs, 480 blocks, 65 us; 4 runs, 640 blocks in two rounds, 77 us)
+// (2 x 1000 rows x 4000 keys, 10 heads of 128: 3 runs, 480 blocks, 65 us; 4 runs, 640 blocks in two rounds, 77 us).  From 384 places on nothing is dealt out: dealt / as it
+// is, fp16, 4 x 1456 rows x 2311 keys: 8 heads of 64 (384 places) 60 / 52 us, of 128 104 / 79; 10 heads (480) 78 / 55 and 87 / 87; 12 heads (576) 91 / 70 and
+// 150 / 140.  Below: 2 x 1000 x 4000, 10 heads (160) 50 / 71 and 68 / 106; 2 x 1900 x 4000, 10 heads (300) 76 / 88 and 124 / 128; but 3 x 1900 x 2000, 8 heads
+// (360), 57 / 46 and 93 / 69; and single tokens would gain above: 8 x 1 x 20000, 80 heads (640) 553 / 739 and 1092 / 1187.
 long long dealt(long long blocks, long long tiles, long long slots, long long least) {
     long long best = tiles, cost = (blocks + slots - 1) / slots * (tiles + 2);
     for (int r = 1; blocks < 384 && r <= 8; ++r) {                    // as many runs as r rounds hold
@@ -857,7 +863,7 @@ constexpr float P_LOG2 = 12.f, P_BACK = 2.44140625e-4f;                         
 __device__ __forceinline__ float power_for(float m) { return __uint_as_float((254u - max(67u, min(__float_as_uint(m) >> 23, 253u))) << 23); }
 
 // dq: a wave owns 32 rows as accumulator columns, the block's waves share key tiles of 64 (the forward kernel's arrangement); K serves as rows (scores)
-// and transposed (ds k).  Three products: 2 x 16 heads x 4096 x 4096 of 128 (bf16) 381 us, 1080 TFLOP/s; 4 x 10 heads x 1456 x 2311 of 64 (fp16) 79 us, 655
+// and transposed (ds k).  Three products: 2 x 16 heads x 4096 x 4096 of 128 (bf16) 377 us, 1090 TFLOP/s; 4 x 10 heads x 1456 x 2311 of 64 (fp16) 84 us, 620
 // (480 blocks: two on most CUs where three would fit).  D comes out of the saved result: o was rounded, o_lo holds what the rounding left.
 template <bool BF, int DP> __global__ void __launch_bounds__(256, DP == 64 ? 3 : 2) k_ctx_bwd_q(BwdArgs p) {
     constexpr int KT = 64, ND = DP / 32, TILE = KT * DP;
@@ -994,8 +1000,9 @@ __device__ __forceinline__ float rows_sum(const f32x16& x, int lane) {
 // its share of the [64][d] tile of ds k -- and q and do are all that is read per row.
 // DV, DK: which of the two the block accumulates.  SHARED: whether not FUSED blocks walk over the samples of one context; a variant of its own, for what that
 // asks at each sample makes the compiler lay out the other's loop worse (4 x 10 heads x 1456 x 2311 of 64, fp16, nothing shared: 125 us as one variant, 105 as two).
-// FUSED 28 x 4096 rows x 77 keys, 5 heads of 64, forward and gradients: 179 us bf16, as three passes 218; 14 x 4096, 8 heads of 128: 265 and 354.
-// Not FUSED, 4 x 10 heads x 1456 x 2311 of 64 (fp16): 111 us, 620 TFLOP/s; 2 x 16 heads on 4 x 4096 x 4096 of 128 (bf16): 849 us, 650.
+// FUSED 28 x 4096 rows x 77 keys, 5 heads of 64, forward and gradients: 171 us bf16, as three passes 234; 14 x 4096, 8 heads of 128: 295 and 375; with 120 keys 185 / 239
+// and 306 / 388.  77 keys take no less than 96 would: a wave owns 32 keys, so the fourth wave has none, and the third 13.
+// Not FUSED, 4 x 10 heads x 1456 x 2311 of 64 (fp16): 116 us, 595 TFLOP/s; 2 x 16 heads on 4 x 4096 x 4096 of 128 (bf16): 833 us, 660.
 template <int DP, bool FUSED> struct BwdLds {
     __attribute__((aligned(16))) u16 q[2 * 64 * DP], g[2 * 64 * DP], k[FUSED ? 128 * DP : 8], s[FUSED ? 128 * 64 : 8];
     __attribute__((aligned(16))) float l[2][64], d[FUSED ? 4 : 2][64], m[4];
@@ -1285,7 +1292,8 @@ template <bool BF, int DP, bool FUSED, bool DV, bool DK, bool SHARED> __device__
 
 // Wide heads, not FUSED: the accumulators of both gradients and K, V leave room for one wave a SIMD only, which waits more than it works; so half of the
 // blocks take dk and the other half dv (five products for four, at two waves a SIMD).  Forward and gradients, separate / together: 4 x 10 heads x 1456 x 2311
-// of 96 bf16 356 / 376 us, of 128 fp16 460 / 479, bf16 432 / 422; 2 x 16 heads on 4 x 4096 x 4096 of 128 fp16 1589 / 1675, bf16 1470 / 1450.
+// of 96 fp16 357 / 363 us, bf16 327 / 371, of 128 fp16 444 / 461, bf16 420 / 421; 2 x 16 heads on 4 x 4096 x 4096 of 96 fp16 1192 / 1214, bf16 1102 / 1269, of 128 fp16
+// 1521 / 1590, bf16 1429 / 1441.
 template <bool BF, int DP, bool FUSED, bool SHARED = false> __global__ void __launch_bounds__(256, DP == 64 || !FUSED ? 2 : 1) k_ctx_bwd_kv(BwdArgs p) {
     __shared__ BwdLds<DP, FUSED> lds;
     int y, kt;

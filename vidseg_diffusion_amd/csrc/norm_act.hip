@@ -13,9 +13,9 @@
 //
 // What bounds it: bytes.  28 x 64 x 64 x 320 fp16: statistics 17.8 us (73 MB read, 4.1 TB/s), apply 28.4 us (147 MB, 5.2 TB/s; a large copy reaches 5.1);
 // 14 x 32 x 32 x 1920 bf16 with SiLU, backward: sums 28.7 us (110 MB; exp2 and rcp of every value are most of it: without SiLU 22), dx 31.3 us (165 MB,
-// 5.3 TB/s).  x (and dy) are read twice, the second time out of the last-level cache: one launch would have to keep a sample's rows on chip
-// across blocks, and its blocks to wait for each other.  Deeper unrolling of either pass changed nothing; 28 x 4096 x 320 and 14 x 1024 x 1920 take 51 / 40 us
-// at 40 K values a chunk, 49 / 47 at 20 K, 63 / 53 at 80 K.
+// 5.3 TB/s).  x (and dy) are read twice, the second time out of the last-level cache: a block owns a run of rows, so a group's statistics need every block of
+// its sample.  (A block that owned whole groups -- 80 KB each at 64 x 64 x 320 -- could keep them on its CU and read x once; that form is not here.)
+// Deeper unrolling of either pass changed nothing; 28 x 4096 x 320 and 14 x 1024 x 1920 take 51 / 40 us at 40 K values a chunk, 49 / 47 at 20 K, 63 / 53 at 80 K.
 #include "common.h"
 
 namespace {
@@ -197,7 +197,8 @@ __device__ __forceinline__ void merge(float& n, float& m, float& m2, float n_b, 
     n = all;
 }
 
-// ---- forward, launch 2: every block merges its sample's chunk statistics (a few KB out of L2) and writes one chunk of y
+// ---- forward, launch 2: every block merges its sample's chunk statistics and writes one chunk of y.  Those are 8 bytes a group and chunk out of L2, 8 KB at 64 x 64 x 320
+// (32 chunks); chunks do not grow with the map, so what all blocks read of them grows with its square: 210 KB a block at 512 x 512 x 128 (820 chunks), beside 82 KB of x
 template <typename T, int VEC> __global__ void __launch_bounds__(NT) k_gna_apply(NormArgs p) {
     extern __shared__ float lds[];
     const int C = p.C, cols = C / VEC, b = blockIdx.y, chunk = blockIdx.x, cg = C / p.G;
