@@ -399,7 +399,7 @@ int vidseg_groupnorm_act_bwd(const void* dy, long long dy_batch_stride, long lon
  * mask[b * mask_b + key] != 0 (mask NULL: all); causal: query i sees own keys up to lens[b] - Nq + i (no mask then).  Heads of width d (8..128, d % 8
  * == 0), query head h on key head h * Hk / H; element strides per sample, row and head (multiples of 8, rows below 2^24; 0 shares one sample), 16-byte aligned.
  * out [B][Nq][H][d]; out_lo (opt): what the rounding of out left, same type; lse (opt) fp32 [B][H][Nq].  A query without a key: out 0, lse -inf.  Keys that do not exist are not read for their value.
- * At most 1024 heads, and B * Nq * H / Hk rows within 256 of 2^31; scale * log2 e within fp32.
+ * At most 1024 heads and 2^31 - 256 rows (B * Nq * H / Hk); scale * log2 e within fp32 (scale at most 2e38).
  * scratch: vidseg_context_attention_scratch_kib(...) KiB (0: none; -1: sizes refused). */
 int vidseg_context_attention_scratch_kib(int B, int Nq, int Np, int Nk, int H, int Hk, int d);
 int vidseg_context_attention_fwd(const void* q, long long q_b, long long q_n, long long q_h, const void* k_prefix, long long kp_n, long long kp_h,
