@@ -154,3 +154,38 @@ def test_small_spreads_without_an_eps(eps):
     x, gamma, beta, dy = data(2, (33, 7), 640, torch.float32, 5, dev)
     check_all(x, gamma, beta, dy, 32, True, eps)
     check_all(x * 2.0 ** -60, gamma, beta, dy, 32, False, eps)
+
+
+@pytest.mark.parametrize("Nk", [77, 300])
+def test_captured_calls_on_one_context(Nk):
+    """One context for the batch, forward and gradients captured once and replayed with other lengths, samples without a key among them; beside it a causal call
+    without a prefix."""
+    dev = torch.device("cuda:0")
+    B, Nq, H = 4, 150, 2
+    q, dout = (randn((B, Nq, H * 64), s, F16).to(dev) for s in (1, 4))
+    k, v = (randn((1, Nk, H * 64), s, F16).to(dev) for s in (2, 3))
+    own = k.expand(B, Nk, H * 64)
+    lens = torch.tensor([Nk, 0, 5, 9], dtype=torch.int32, device=dev)
+
+    def calls(leaves):
+        out = ops.cross_attention(*leaves, H, k_lens=lens)
+        with torch.no_grad():
+            late = ops.prefix_attention(q, own[0, :0], own[0, :0], own, own, H, k_lens=lens, causal=True)
+        return (out.detach(), *torch.autograd.grad(out, leaves, dout), late)
+    fresh = lambda: [t.detach().clone().requires_grad_(True) for t in (q, k, v)]               # noqa: E731
+    calls(fresh())
+    leaves = fresh()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = calls(leaves)
+    for seed, n in ((11, (0, Nk, 0, 3)), (12, (0, 0, 0, Nk)), (13, (Nk, Nk, Nk, Nk)), (14, (0, 0, 0, 0))):
+        with torch.no_grad():
+            q.copy_(randn(q.shape, seed, F16))
+            leaves[0].copy_(q)
+            lens.copy_(torch.tensor(n, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = calls(fresh())
+        assert all(torch.equal(a, b) for a, b in zip(held, want))
+        Reference(q, k, v, H, None, lens).check_gradients(dout, *want[1:4], True)
+        Reference(q, own, own, H, None, lens, causal=True).check(want[4])
